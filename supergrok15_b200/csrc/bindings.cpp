@@ -157,4 +157,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     sgb::register_gemm(m);
     sgb::register_nn(m);
     sgb::register_llm(m);
+    sgb::register_packed(m);
 }

@@ -1,0 +1,26 @@
+// Arguments of the packed-attention kernels (packed_attn.cu: CUDA cores, packed_attn_sm100.cu: tensor cores).
+#pragma once
+#include "packed_seq.cuh"
+
+namespace sg {
+
+struct PackedAttn {
+    const void *q, *k, *v;              // [total, heads, hd], [total, heads / group, hd]; the last index is contiguous
+    int64_t q_ld, k_ld, v_ld;           // elements between rows
+    int64_t q_hs, k_hs, v_hs;           // elements between heads
+    void* out;                          // [total, heads, hd], dense
+    void* out_lo;                       // 16-bit training: what the rounding took from `out`, in the same type and layout; else null
+    float* lse;                         // [heads, total], null without a backward pass
+    const void* dout;                   // backward: dense like out
+    float* delta;                       // scratch [heads, total]
+    void *dq, *dk, *dv;                 // dense
+    PackedSeqs seqs;
+    int heads, group, hd, causal;
+    float scale;
+};
+
+// Return 0 or the number of the step that failed.
+int packed_attn_fwd(int dtype, const PackedAttn& p, cudaStream_t st);
+int packed_attn_bwd(int dtype, const PackedAttn& p, cudaStream_t st);
+
+}  // namespace sg

@@ -6,6 +6,8 @@
 ``rms_norm(x, residual, w)``        RMSNorm(x + residual), same kernels with the mean fixed at zero.
 ``rope(x, cos, sin)``               rotary position embedding of [B, S, H, hd] (interleaved pairs).
 ``swiglu(gate, up)``                silu(gate) * up in one pass; ``gelu(x)`` exact GELU.
+``attention_packed(q, k, v, cu)``   attention inside each of several sequences of different lengths that share one row axis, with
+                                    grouped key / value heads; the gradients of a key head are summed over its query heads.
 ``embedding(ids, weight)``          row gather; the gradient is a deterministic sorted segment sum (no atomics).
 ``cross_entropy(logits, target)``   mean softmax cross-entropy with ``ignore_index``; forward reads the logits once.
 ``linear(x, w, b)`` / ``grad_sink``  F.linear whose backward, inside a ``grad_sink`` block, adds the weight and bias gradients
@@ -325,6 +327,77 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
             return _build.require().flash_node(q, k, v, causal, _gemm._err_flag(q.device))
         return _FlashAttention.apply(q, k, v, causal)
     return attention_reference(q, k, v, causal)
+
+
+def attention_packed_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, causal: bool = True,
+                               scale: Optional[float] = None) -> torch.Tensor:
+    """``attention_packed`` sequence by sequence, 16-bit inputs in fp32; reads the offsets on the host."""
+    group, dtype = q.shape[1] // k.shape[1], q.dtype
+    k, v = (t.repeat_interleave(group, 1) for t in (k, v))
+    if dtype in (torch.bfloat16, torch.float16):
+        q, k, v = q.float(), k.float(), v.float()
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    offs = [min(max(int(c), 0), q.shape[0]) for c in cu_seqlens.tolist()]
+
+    def nothing(a, b):                                                   # rows of no sequence: zero, with zero gradients
+        return sum(t[a:b].masked_fill(torch.ones((), dtype=torch.bool, device=t.device), 0.0) for t in (q, k, v))
+    parts, done = [], 0
+    for a, b in zip(offs[:-1], offs[1:]):
+        if b <= a:
+            continue
+        s = torch.einsum("ihd,jhd->hij", q[a:b], k[a:b]) * scale
+        if causal:
+            s = s.masked_fill(torch.ones(b - a, b - a, dtype=torch.bool, device=s.device).triu(1), float("-inf"))
+        parts += [nothing(done, a), torch.einsum("hij,jhd->ihd", torch.softmax(s, -1), v[a:b])]
+        done = b
+    return torch.cat(parts + [nothing(done, q.shape[0])]).to(dtype)
+
+
+class _AttnPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu, causal, scale):
+        out, rest, lse = _build.require().packed_attn_fwd(q, k, v, cu, causal, scale, True)
+        ctx.save_for_backward(q, k, v, cu, out, rest, lse)
+        ctx.args = causal, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, cu, out, rest, lse = ctx.saved_tensors
+        return (*_build.require().packed_attn_bwd(q, k, v, cu, out, rest, lse, dout, *ctx.args), None, None, None)
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, causal: bool = True,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of ``q [rows, heads, hd]`` over ``k, v [rows, kv_heads, hd]`` inside each of the packed sequences
+    ``[cu_seqlens[i], cu_seqlens[i + 1])`` of the row axis (int32 or int64, ascending from 0 on; sequences without a row are allowed).
+    Returns ``[rows, heads, hd]``.
+
+    ``heads`` is a multiple of ``kv_heads``: query head ``h`` reads key head ``h // (heads // kv_heads)``.  ``causal``: a row sees the rows of
+    its sequence up to itself.  ``scale`` multiplies the scores (default ``hd ** -0.5``).  Rows of no sequence (padding behind the last one)
+    are neither read nor counted: their output and their gradients are zero.  The offsets stay on the device (no host synchronisation, and a
+    captured call follows offsets rewritten in place); offsets that do not ascend give undefined rows.  bf16, fp16 and fp32; head sizes up to
+    128 on CUDA.  Sums, softmax statistics and gradient accumulators are fp32 and added in a fixed order."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"attention_packed: q [rows, heads, hd] and k, v [rows, kv_heads, hd] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"attention_packed: {q.shape[1]} query heads are not a multiple of {k.shape[1]} key heads")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() == 0 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("attention_packed: cu_seqlens must be a vector of sequences + 1 int32 or int64 offsets")
+    if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device == cu_seqlens.device):
+        raise ValueError("attention_packed: q, k and v need one dtype, and all tensors one device")
+    if not q.is_cuda:
+        return attention_packed_reference(q, k, v, cu_seqlens, causal, scale)
+    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32) or not 1 <= q.shape[2] <= 128:
+        raise ValueError(f"attention_packed: bf16, fp16 or fp32 with head sizes up to 128 on CUDA, got {q.dtype} with {q.shape[2]}")
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    cu = cu_seqlens.to(torch.int32).contiguous()
+    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    if _cpp_node(q, k, v):
+        train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+        return _build.require().packed_attn_node(q, k, v, cu, causal, scale, train)
+    return _AttnPacked.apply(q, k, v, cu, causal, scale)
 
 
 def _native_ok(x: torch.Tensor) -> bool:
