@@ -1,8 +1,9 @@
-// Bindings of the operators of packed language-model training: attention over packed sequences.
+// Bindings of the operators of packed language-model training: attention over packed sequences, cross-entropy of a linear head.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include "bindings_decl.h"
 #include "mt_host.h"
+#include "linear_ce.h"
 #include "packed_attn.h"
 
 namespace sgb {
@@ -94,9 +95,154 @@ struct PackedAttnNode : Function<PackedAttnNode> {
         return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
+
+// ---- cross-entropy of a linear head
+// Rows of a piece: u (rows x vocabulary, the type of x) takes 256 MB at most, but at least 256 rows go together, so that w is not read for
+// less work than that.  A pass without gradients keeps two floats per row and tile of columns only.
+int64_t lce_piece_rows(int64_t rows, int64_t ldu, int64_t elem, bool train) {
+    int64_t most = train ? ((int64_t)256 << 20) / (ldu * elem) / 256 * 256 : 65536;
+    if (most < 256) most = 256;
+    if (rows <= most) return rows;
+    const int64_t pieces = (rows + most - 1) / most;
+    return ((rows + pieces - 1) / pieces + 255) / 256 * 256;
+}
+
+struct LceShape {
+    sg::LceArgs a{};
+    int dtype = 0;
+    int64_t rows = 0, piece = 0, elem = 0;
+    // the piece of rows [r0, r0 + n)
+    sg::LceArgs at(int64_t r0) const {
+        sg::LceArgs p = a;
+        p.rows = (int)(rows - r0 < piece ? rows - r0 : piece);
+        p.x = (const char*)a.x + r0 * a.ldx * elem;
+        p.target = a.target + r0;
+        p.loss = a.loss ? a.loss + r0 : nullptr;
+        return p;
+    }
+    int64_t last() const { return rows == 0 ? 0 : (rows - 1) / piece * piece; }      // first row of the last piece
+};
+
+LceShape lce_shape(const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool train) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2 && t.dim() == 1 && x.size(1) == w.size(1) && t.size(0) == x.size(0),
+                "linear_cross_entropy: x [rows, D], weight [vocabulary, D], target [rows]");
+    TORCH_CHECK(w.device() == x.device() && t.device() == x.device(), "linear_cross_entropy: all tensors on one device");
+    TORCH_CHECK(w.scalar_type() == x.scalar_type() && t.scalar_type() == at::kLong && t.is_contiguous(), "linear_cross_entropy: x and weight of one dtype, int64 targets");
+    TORCH_CHECK(w.size(0) >= 1 && w.size(0) < (1 << 22) && x.size(1) >= 1 && x.size(1) < (1 << 22) && x.size(0) < ((int64_t)1 << 31),
+                "linear_cross_entropy: vocabulary and width below 2^22");
+    TORCH_CHECK((x.stride(1) == 1 || x.size(1) == 1) && (w.stride(1) == 1 || w.size(1) == 1), "linear_cross_entropy: the last index must be contiguous");
+    LceShape s;
+    s.dtype = dtype_code(x);
+    s.elem = x.element_size();
+    s.rows = x.size(0);
+    s.a.x = x.data_ptr(); s.a.w = w.data_ptr(); s.a.ldx = x.stride(0); s.a.ldw = w.stride(0);
+    s.a.target = t.data_ptr<int64_t>(); s.a.ignore_index = ignore_index;
+    s.a.V = (int)w.size(0); s.a.D = (int)w.size(1);
+    const int64_t per = 16 / s.elem;
+    s.a.ldu = (w.size(0) + per - 1) / per * per;
+    s.piece = lce_piece_rows(s.rows, s.a.ldu, s.elem, train);
+    return s;
+}
+
+// Returns (loss, {mean, 1 / count}, d of the last piece [rows, pitch], and with several pieces: fp32 dx of the others, fp32 dw of the others).
+// The gradient products of the last piece are left to the backward pass, which writes them in the final type; of the pieces before it the
+// products are taken here, because their d makes room for the next one's.
+std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
+    const bool train = need_x || need_w;
+    LceShape s = lce_shape(x, w, t, ignore_index, train);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto st = at::cuda::getCurrentCUDAStream();
+    const auto fo = x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
+    const auto xo = x.options().memory_format(at::MemoryFormat::Contiguous);
+    Tensor loss = at::empty({s.rows}, fo), mean = s.rows > 0 ? at::empty({2}, fo) : at::zeros({2}, fo);
+    Tensor u = at::empty({train ? s.piece : 0, s.a.ldu}, xo), dx, dw;
+    if (s.rows > 0) {
+        s.a.loss = loss.data_ptr<float>();
+        const int cols = sg::lce_tile_columns(s.dtype, s.at(0));
+        Tensor stats = at::empty({2, (s.a.V + cols - 1) / cols, s.piece}, fo), zt = at::empty({s.piece}, fo);
+        s.a.tile_max = stats.data_ptr<float>();
+        s.a.tile_sum = s.a.tile_max + stats.numel() / 2;
+        s.a.z_target = zt.data_ptr<float>();
+        s.a.u = train ? u.data_ptr() : nullptr;
+        const int64_t last = s.last();
+        if (train && last > 0 && need_x) dx = at::empty({last, x.size(1)}, fo);
+        if (train && last > 0 && need_w) dw = at::empty(w.sizes(), fo);
+        for (int64_t r0 = 0; r0 < s.rows; r0 += s.piece) {
+            const sg::LceArgs a = s.at(r0);
+            int rc = sg::lce_logits(s.dtype, a, err.data_ptr<int>(), st);
+            if (rc == 0) rc = sg::lce_rows(s.dtype, a, st);
+            if (rc == 0 && train && r0 < last) {
+                sg::LceGrads g{};
+                g.dx = need_x ? dx.data_ptr<float>() + r0 * x.size(1) : nullptr;
+                g.dw = need_w ? dw.data_ptr() : nullptr;
+                g.dw_prev = need_w && r0 > 0 ? dw.data_ptr<float>() : nullptr;
+                g.f32_out = true;
+                rc = sg::lce_grads(s.dtype, a, g, err.data_ptr<int>(), st);
+            }
+            TORCH_CHECK(rc == 0, "linear_cross_entropy: launch failed (code ", rc, ")");
+        }
+        sg::ce_mean(s.a.loss, s.a.target, s.rows, s.a.V, ignore_index, mean.data_ptr<float>(), st);
+    }
+    const Tensor none = at::empty({0}, fo);
+    return {mean.narrow(0, 0, 1).reshape({}), mean, u, dx.defined() ? dx : none, dw.defined() ? dw : none};
+}
+
+std::vector<Tensor> lce_bwd(const Tensor& x, const Tensor& w, const Tensor& t, const Tensor& mean, const Tensor& u, const Tensor& dx32, const Tensor& dw32,
+                            const Tensor& gout_, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
+    LceShape s = lce_shape(x, w, t, ignore_index, true);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto st = at::cuda::getCurrentCUDAStream();
+    Tensor gout = gout_.to(at::kFloat).reshape({1}).contiguous();
+    Tensor dx, dw;
+    const auto xo = x.options().memory_format(at::MemoryFormat::Contiguous);
+    if (need_x) dx = s.rows > 0 ? at::empty(x.sizes(), xo) : at::zeros(x.sizes(), xo);
+    if (need_w) dw = s.rows > 0 ? at::empty(w.sizes(), xo) : at::zeros(w.sizes(), xo);
+    if (s.rows == 0 || !(need_x || need_w)) return {dx, dw};
+    const int64_t last = s.last(), D = x.size(1);
+    TORCH_CHECK(u.is_contiguous() && u.size(0) == s.piece && u.size(1) == s.a.ldu && u.scalar_type() == x.scalar_type() && mean.numel() == 2,
+                "linear_cross_entropy: not what the forward pass left");
+    TORCH_CHECK((!need_x || dx32.numel() == last * D) && (!need_w || dw32.numel() == (last > 0 ? w.numel() : 0)), "linear_cross_entropy: not what the forward pass left");
+    s.a.u = u.data_ptr();
+    const sg::LceArgs a = s.at(last);
+    sg::LceGrads g{};
+    g.dx = need_x ? (char*)dx.data_ptr() + last * D * s.elem : nullptr;
+    g.dw = need_w ? dw.data_ptr() : nullptr;
+    g.dw_prev = need_w && last > 0 ? dw32.data_ptr<float>() : nullptr;
+    g.gout = gout.data_ptr<float>();
+    g.inv_count = mean.data_ptr<float>() + 1;
+    int rc = sg::lce_grads(s.dtype, a, g, err.data_ptr<int>(), st);
+    if (rc == 0 && need_x) rc = sg::lce_finish(s.dtype, dx32.data_ptr<float>(), dx.data_ptr(), last * D, g.gout, g.inv_count, st);
+    TORCH_CHECK(rc == 0, "linear_cross_entropy: launch of the backward pass failed (code ", rc, ")");
+    return {dx, dw};
+}
+
+struct LceNode : Function<LceNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, const Tensor& err) {
+        auto r = lce_fwd(x, w, t, ignore_index, need_x, need_w, err);
+        if (need_x || need_w) ctx->save_for_backward({x, w, t, r[1], r[2], r[3], r[4]});
+        ctx->saved_data["err"] = err;                                     // the process's time-out flag itself, not a saved tensor
+        ctx->saved_data["ignore"] = ignore_index;
+        ctx->saved_data["need_x"] = need_x;
+        ctx->saved_data["need_w"] = need_w;
+        return r[0];
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list dy) {
+        refuse_second_order("linear_cross_entropy");
+        const auto s = ctx->get_saved_variables();
+        auto r = lce_bwd(s[0], s[1], s[2], s[3], s[4], s[5], s[6], dy[0], ctx->saved_data["ignore"].toInt(), ctx->saved_data["need_x"].toBool(),
+                         ctx->saved_data["need_w"].toBool(), ctx->saved_data["err"].toTensor());
+        return {r[0], r[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
 }  // namespace
 
 void register_packed(pybind11::module_& m) {
+    m.def("lce_fwd", &lce_fwd);
+    m.def("lce_bwd", &lce_bwd);
+    m.def("lce_piece_rows", &lce_piece_rows);
+    m.def("lce_node", [](const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, const Tensor& err) {
+        return LceNode::apply(x, w, t, ignore_index, need_x, need_w, err);
+    });
     m.def("packed_attn_fwd", &packed_attn_fwd);
     m.def("packed_attn_bwd", &packed_attn_bwd);
     m.def("packed_attn_node", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, bool causal, double scale, bool train) {

@@ -10,6 +10,7 @@
                                     grouped key / value heads; the gradients of a key head are summed over its query heads.
 ``embedding(ids, weight)``          row gather; the gradient is a deterministic sorted segment sum (no atomics).
 ``cross_entropy(logits, target)``   mean softmax cross-entropy with ``ignore_index``; forward reads the logits once.
+``linear_cross_entropy(x, w, target)``  the mean cross-entropy of ``x @ w.T`` without keeping the logits, with the gradients of both.
 ``linear(x, w, b)`` / ``grad_sink``  F.linear whose backward, inside a ``grad_sink`` block, adds the weight and bias gradients
                                     straight into ``w.grad`` / ``b.grad`` (the wgrad GEMM runs with beta = 1 on a side stream,
                                     next to the dgrad GEMM) instead of returning them for a separate accumulation kernel.
@@ -526,3 +527,58 @@ def cross_entropy(logits: torch.Tensor, target: torch.Tensor, ignore_index: int 
     if _cpp_node(logits, target):
         return _build.require().cross_entropy_node(logits, target, ignore_index)
     return _CrossEntropy.apply(logits, target, ignore_index)
+
+
+def linear_cross_entropy_reference(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+    """``linear_cross_entropy`` with stored logits."""
+    x, weight = (t.float() if t.dtype in (torch.bfloat16, torch.float16) else t for t in (x, weight))
+    z, target = F.linear(x.reshape(-1, x.shape[-1]), weight), target.reshape(-1)
+    counted = (target != ignore_index) & (target >= 0) & (target < weight.shape[0])
+    at = target.clamp(0, weight.shape[0] - 1).unsqueeze(1)
+    rows = (torch.logsumexp(z, 1) - z.gather(1, at).squeeze(1)).masked_fill(~counted, 0.0)
+    return rows.sum() / counted.sum().clamp(min=1)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index):
+        from . import gemm as _gemm
+        need = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        loss, *kept = _build.require().lce_fwd(x, weight, target, ignore_index, *need, _gemm._err_flag(x.device))
+        ctx.save_for_backward(x, weight, target, *kept)
+        ctx.args = ignore_index, *need
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        from . import gemm as _gemm
+        x = ctx.saved_tensors[0]
+        return (*_build.require().lce_bwd(*ctx.saved_tensors, gout, *ctx.args, _gemm._err_flag(x.device)), None, None)
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+    """Mean cross-entropy of the logits ``x @ weight.T`` against int64 ``target``, without keeping the logits: ``x [..., D]``,
+    ``weight [vocabulary, D]``, ``target [...]``; the result is an fp32 scalar.
+
+    Positions whose target is ``ignore_index`` or lies outside the vocabulary are not counted: they add nothing to the loss, and their rows of
+    the gradient are zero (no counted position: loss 0).  bf16, fp16 and fp32 on CUDA, for any vocabulary.  At most 256 MB (or 256 rows) of
+    [rows, vocabulary] values exist at a time, in the type of ``x``; a pass with gradients takes the rows in pieces of that size, and from the
+    second piece on holds the weight's gradient in fp32 between forward and backward.  The gradients' products of all pieces but the last
+    are formed in the forward pass.  Sums are fp32 and added in a fixed order."""
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or target.shape != x.shape[:-1] or 0 in weight.shape:
+        raise ValueError(f"linear_cross_entropy: x [..., D], weight [vocabulary, D] and target [...] expected, got {tuple(x.shape)}, {tuple(weight.shape)}, "
+                         f"{tuple(target.shape)}")
+    if x.dtype != weight.dtype or target.dtype != torch.int64 or not (x.device == weight.device == target.device):
+        raise ValueError("linear_cross_entropy: x and weight need one dtype, target int64, and all tensors one device")
+    if not x.is_cuda:
+        return linear_cross_entropy_reference(x, weight, target, ignore_index)
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"linear_cross_entropy: bf16, fp16 or fp32 on CUDA, got {x.dtype}")
+    x2, t = x.reshape(-1, x.shape[-1]), target.reshape(-1).contiguous()
+    x2, w = (a if a.stride(1) == 1 else a.contiguous() for a in (x2, weight))
+    if _cpp_node(x2, w, t):
+        from . import gemm as _gemm
+        grad = torch.is_grad_enabled()
+        return _build.require().lce_node(x2, w, t, ignore_index, grad and x2.requires_grad, grad and w.requires_grad, _gemm._err_flag(x.device))
+    return _LinearCrossEntropy.apply(x2, w, t, ignore_index)
