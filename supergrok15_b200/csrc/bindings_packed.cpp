@@ -21,6 +21,14 @@ void refuse_second_order(const char* what) {
 
 bool head_rows_ok(const Tensor& t) { return t.stride(2) == 1 || t.size(2) == 1; }
 
+// A 16-bit view whose base or pitches the tensor-core kernels cannot load from is copied once: they then take it (a few per cent of their time
+// for short sequences, less for long ones; the CUDA cores take over a hundred times longer).  Other views are used where they are.
+Tensor loadable(const Tensor& t) {
+    if (t.dim() != 3 || t.element_size() != 2 || t.size(2) % 8 != 0 || t.numel() == 0) return t;
+    if (sg::packed_tma_view(t.data_ptr(), t.stride(0), t.stride(1), t.size(0), t.size(1))) return t;
+    return t.clone(at::MemoryFormat::Contiguous);
+}
+
 sg::PackedAttn packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, bool causal, double scale) {
     TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(2) == k.size(2),
                 "attention_packed: q [rows, heads, head_dim], k and v [rows, kv_heads, head_dim]");
@@ -42,7 +50,8 @@ sg::PackedAttn packed_args(const Tensor& q, const Tensor& k, const Tensor& v, co
 }
 
 // returns (out, what the rounding took from it, lse [heads, rows]); without `train` the last two are empty
-std::vector<Tensor> packed_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, bool causal, double scale, bool train) {
+std::vector<Tensor> packed_attn_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu, bool causal, double scale, bool train, Tensor err) {
+    const Tensor q = loadable(q_), k = loadable(k_), v = loadable(v_);
     sg::PackedAttn p = packed_args(q, k, v, cu, causal, scale);
     c10::cuda::CUDAGuard guard(q.device());
     const auto dense = q.options().memory_format(at::MemoryFormat::Contiguous);
@@ -53,14 +62,17 @@ std::vector<Tensor> packed_attn_fwd(const Tensor& q, const Tensor& k, const Tens
     p.out = out.data_ptr();
     p.out_lo = lo.numel() ? lo.data_ptr() : nullptr;
     p.lse = train ? lse.data_ptr<float>() : nullptr;
-    const int rc = sg::packed_attn_fwd(dtype_code(q), p, at::cuda::getCurrentCUDAStream());
+    const int dt = dtype_code(q);
+    auto st = at::cuda::getCurrentCUDAStream();
+    const int rc = sg::packed_attn_sm100_takes(dt, p) ? sg::packed_attn_sm100_fwd(dt, p, err.data_ptr<int>(), st) : sg::packed_attn_fwd(dt, p, st);
     TORCH_CHECK(rc == 0, "attention_packed: launch failed (code ", rc, ")");
     return {out, lo, lse};
 }
 
 // gradients of packed_attn_fwd: (dq, dk, dv), dense
-std::vector<Tensor> packed_attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, const Tensor& out, const Tensor& lo, const Tensor& lse,
-                                    const Tensor& dout_, bool causal, double scale) {
+std::vector<Tensor> packed_attn_bwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu, const Tensor& out, const Tensor& lo, const Tensor& lse,
+                                    const Tensor& dout_, bool causal, double scale, Tensor err) {
+    const Tensor q = loadable(q_), k = loadable(k_), v = loadable(v_);
     sg::PackedAttn p = packed_args(q, k, v, cu, causal, scale);
     c10::cuda::CUDAGuard guard(q.device());
     Tensor dout = dout_.contiguous();
@@ -80,10 +92,12 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& q, const Tensor& k, const Tens
 }
 
 struct PackedAttnNode : Function<PackedAttnNode> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, bool causal, double scale, bool train) {
-        auto r = packed_attn_fwd(q, k, v, cu, causal, scale, train);
+    static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu, bool causal, double scale, bool train, const Tensor& err) {
+        const Tensor q = loadable(q_), k = loadable(k_), v = loadable(v_);   // the copy, where there is one, is what the backward pass reads
+        auto r = packed_attn_fwd(q, k, v, cu, causal, scale, train, err);
         if (!train) return r[0];
         ctx->save_for_backward({q, k, v, cu, r[0], r[1], r[2]});
+        ctx->saved_data["err"] = err;                                     // the process's time-out flag itself, not a saved tensor
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["scale"] = scale;
         return r[0];
@@ -91,8 +105,9 @@ struct PackedAttnNode : Function<PackedAttnNode> {
     static variable_list backward(AutogradContext* ctx, variable_list dy) {
         refuse_second_order("attention_packed");
         const auto s = ctx->get_saved_variables();
-        auto r = packed_attn_bwd(s[0], s[1], s[2], s[3], s[4], s[5], s[6], dy[0], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
-        return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor(), Tensor()};
+        auto r = packed_attn_bwd(s[0], s[1], s[2], s[3], s[4], s[5], s[6], dy[0], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(),
+                                 ctx->saved_data["err"].toTensor());
+        return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -245,8 +260,8 @@ void register_packed(pybind11::module_& m) {
     });
     m.def("packed_attn_fwd", &packed_attn_fwd);
     m.def("packed_attn_bwd", &packed_attn_bwd);
-    m.def("packed_attn_node", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, bool causal, double scale, bool train) {
-        return PackedAttnNode::apply(q, k, v, cu, causal, scale, train);
+    m.def("packed_attn_node", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, bool causal, double scale, bool train, const Tensor& err) {
+        return PackedAttnNode::apply(q, k, v, cu, causal, scale, train, err);
     });
 }
 }  // namespace sgb

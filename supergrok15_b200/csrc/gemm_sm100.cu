@@ -580,6 +580,13 @@ bool tc::make_map_batched(CUtensorMap* map, const void* base, int64_t batch, int
     const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
     return encode_map(map, base, 3, dims, strides, box, bf16, swizzle128);
 }
+bool tc::make_map_heads(CUtensorMap* map, const void* base, int64_t rows, int64_t heads, int64_t hd, int64_t ld_elems, int64_t head_elems, int box_rows) {
+    // the pitch of an axis of length one is never used, but has to be one that the encoder accepts
+    const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)(heads == 1 ? 256 : head_elems * 2), (cuuint64_t)(rows == 1 ? 256 : ld_elems * 2)};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
+    return encode_map(map, base, 3, dims, strides, box, true, true);
+}
 int tc::last_map_error() { return g_map_error; }
 namespace {
 

@@ -22,5 +22,13 @@ struct PackedAttn {
 // Return 0 or the number of the step that failed.
 int packed_attn_fwd(int dtype, const PackedAttn& p, cudaStream_t st);
 int packed_attn_bwd(int dtype, const PackedAttn& p, cudaStream_t st);
+// what the tensor-core kernels' loads ask of a 16-bit [rows, heads, hd] view: a 16-byte aligned base, pitches of whole 16 bytes below 2^39
+inline bool packed_tma_view(const void* base, int64_t ld, int64_t hs, int64_t rows, int64_t heads) {
+    const auto pitch = [](int64_t n, int64_t count) { return count <= 1 || (n > 0 && n % 8 == 0 && n < (int64_t)1 << 38); };
+    return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && pitch(ld, rows) && pitch(hs, heads);
+}
+// The tensor-core kernels; `err` (a device word) becomes non-zero when a wait inside a kernel ran out.
+bool packed_attn_sm100_takes(int dtype, const PackedAttn& p);
+int packed_attn_sm100_fwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st);
 
 }  // namespace sg

@@ -1,0 +1,470 @@
+// Attention over packed sequences with grouped heads on the 5th-generation tensor cores (tcgen05 / TMEM / TMA), sm_100a only.  16-bit
+// operands (bf16, fp16), head sizes that are multiples of 8 up to 128, fp32 scores, sums and accumulators.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = softmax_j(scale q_i . k_j),  j over the rows of i's sequence (causal: j <= i)
+//
+// q, k, v are read where they are ([rows, heads, hd] views with any row and head pitch that TMA takes): a map of three dimensions
+// (hd, heads, rows), boxes of 64 columns x 128 rows of one head, columns past hd filled with zeros, so a head of 80 runs as two boxes.
+//
+// Work is handed out by the hardware: the grid has one CTA per item, one CTA fits an SM, and a running CTA takes over the items of CTAs
+// that have not started (cluster launch control).  Lengths are known on the device only, so no static split balances them; the barriers,
+// the tensor memory and the loads of the next item carry over from item to item without a counter in memory to be zeroed.
+//
+// Rows behind a sequence's end belong to the next sequence or to nobody.  As keys they are masked in the scores by selection, and as rows of
+// an operand that is multiplied by a zero probability they are zeroed in shared memory, because zero times NaN or infinity is NaN.
+#include "sg_native.h"
+#include "tc_sm100.cuh"
+#include "per_device.h"
+#include "packed_attn.h"
+#include <cuda_fp16.h>
+#include <cfloat>
+
+namespace sg {
+namespace {
+using namespace tc;
+
+constexpr uint32_t HALF_TILE = 128 * 128;                                // [128 rows x 64 elements of 2 bytes] = 16 KB
+constexpr int STAGE_PITCH = 80;                                          // 64 bytes of a row and a pad: conflict-free 16-byte accesses
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T> struct Half2;
+template <> struct Half2<__nv_bfloat16> {
+    static constexpr uint32_t FMT = 1;                                    // operand format of the instruction descriptor
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
+};
+template <> struct Half2<__half> {
+    static constexpr uint32_t FMT = 0;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+};
+// instruction descriptor of kind::f16: fp32 accumulator, both operands of format FMT, b_mn = 1 when B is MN-major
+__device__ __forceinline__ uint32_t idesc_f16(uint32_t fmt, int M, int N, int b_mn) {
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void fma2(float x0, float x1, float a0, float a1, float b0, float b1, float& y0, float& y1) {
+    asm("{\n\t.reg .b64 vx, va, vb, vy;\n\tmov.b64 vx, {%2, %3};\n\tmov.b64 va, {%4, %5};\n\tmov.b64 vb, {%6, %7};\n\t"
+        "fma.rn.f32x2 vy, vx, va, vb;\n\tmov.b64 {%0, %1}, vy;\n\t}"
+        : "=f"(y0), "=f"(y1) : "f"(x0), "f"(x1), "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Cluster launch control: ask for a CTA of this grid that has not started; its index comes back as 16 bytes in shared memory.
+__device__ __forceinline__ void clc_ask(uint4* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool clc_answer(const uint4* answer, int& item) {
+    uint32_t got, x;
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b128 a;\n\tld.shared.b128 a, [%2];\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+                 : "=r"(got), "=r"(x) : "r"(smem_u32(answer)) : "memory");
+    item = (int)x;
+    return got != 0;
+}
+
+// a wait of a whole warp that ends the same way for every lane
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
+// What the scheduling warp tells the others about an item.
+struct Item {
+    int lo, hi, row0, head, kind;                                        // kind: 0 end of the work, 1 rows of a sequence, 2 rows of none
+};
+
+// rows [first, 128) of a tile (HALVES boxes of 64 columns) become zero; called by a whole warp between the arrival of the tile and its use
+template <int HALVES> __device__ __forceinline__ void zero_rows(uint8_t* tile, int first) {
+    const int lane = (int)(threadIdx.x & 31);
+    const int n16 = (128 - first) * 8;                                    // a row of a box is 128 consecutive bytes, however swizzled
+#pragma unroll
+    for (int hf = 0; hf < HALVES; ++hf) {
+        uint4* p = reinterpret_cast<uint4*>(tile + hf * HALF_TILE + first * 128);
+        for (int i = lane; i < n16; i += 32) p[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// Forward.  An item is 256 query rows of one head: two tiles A and B of 128 rows that share every key tile, each with its own score
+// buffer and accumulator in tensor memory and its own group of 128 softmax threads (one row per thread).  The tensor cores alternate
+//     O_A += P_A(j) V_j,  S_A(j+1) = Q_A K_{j+1}^T,  O_B += P_B(j) V_j,  S_B(j+1)
+// so a group's softmax runs under the other tile's products.  P overwrites S in place (the first 64 columns of its buffer) and is read
+// from tensor memory; O stays there, and a row is rescaled only when its maximum has grown by more than 2^8.
+//   warps 0-3, 4-7   softmax and epilogue of tile A, of tile B
+//   warp 8           takes items, loads Q and the rings of two K and two V tiles      warp 9   issues the products
+// A row of 128 scores is held in registers: the softmax warpgroups take 208 per thread and leave 88 to the third (256 x 208 + 128 x 88 =
+// 384 x 168, the registers of the launch).
+constexpr int FWD_THREADS = 384;
+constexpr int REGS_SOFTMAX = 208, REGS_OTHERS = 88;
+struct FwdBars {
+    uint64_t item_full[2], item_empty[2], clc, q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], v_tail;
+    uint64_t s_full[2], p_full[2], o_done[2], o_empty[2];
+    uint4 answer;
+    Item item[2];
+    uint32_t tmem_slot;
+};
+
+struct FwdArgs {
+    void *out, *out_lo;
+    float* lse;
+    PackedSeqs seqs;
+    int heads, group, hd, causal, slots;
+    float scale;
+    int* err;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdArgs a) {
+    constexpr int HALVES = HD / 64;
+    constexpr uint32_t TILE = HALVES * HALF_TILE;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sQ = smem;                                                   // [2 tiles]
+    uint8_t* sK = sQ + 2 * TILE;                                          // [2]
+    uint8_t* sV = sK + 2 * TILE;                                          // [2]
+    uint8_t* s_stage = sV + 2 * TILE;                                     // [8 warps][32 rows][STAGE_PITCH]
+    FwdBars* b = reinterpret_cast<FwdBars*>(s_stage + 8 * 32 * STAGE_PITCH);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 9);
+            mbar_init(&b->k_full[i], 1); mbar_init(&b->k_empty[i], 1); mbar_init(&b->v_full[i], 1); mbar_init(&b->v_empty[i], 1);
+            mbar_init(&b->s_full[i], 1); mbar_init(&b->p_full[i], 128); mbar_init(&b->o_done[i], 1); mbar_init(&b->o_empty[i], 128);
+        }
+        mbar_init(&b->clc, 1); mbar_init(&b->q_full, 1); mbar_init(&b->q_empty, 1); mbar_init(&b->v_tail, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&b->tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = b->tmem_slot;                                   // tile t: S / P at 128 t, O at 256 + 128 t
+
+    // key tiles that tile t of an item meets
+    auto blocks = [&](const Item& w, int t) {
+        const int r = w.row0 + 128 * t;
+        if (r >= w.hi) return 0;
+        const int last = a.causal && r + 128 < w.hi ? r + 128 : w.hi;
+        return (last - w.lo + 127) / 128;
+    };
+
+    if (warp < 8) {
+        reg_inc<REGS_SOFTMAX>();
+        const int t = warp >> 2, q = warp & 3, row = q * 32 + lane;  // tile of the group, TMEM lane quarter of the warp, row of the thread
+        const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
+        const uint32_t ts = tmem + t * 128 + lane_addr, to = tmem + 256 + t * 128 + lane_addr;
+        const float c2 = a.scale * LOG2E;
+        uint8_t* stg = s_stage + warp * 32 * STAGE_PITCH;
+        uint32_t n_item = 0, n_s = 0, n_o = 0;
+        bool ok = true;
+        while (ok) {
+            const uint32_t si = n_item & 1;
+            if (!warp_wait(&b->item_full[si], (n_item >> 1) & 1)) { atomicExch(a.err, 74); break; }
+            const Item w = b->item[si];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b->item_empty[si]);
+            ++n_item;
+            if (w.kind == 0) break;
+            const int row0 = w.row0 + 128 * t + q * 32;                   // first row of this warp
+            const int n = w.kind == 1 ? blocks(w, t) : 0;
+            float m_ref = -FLT_MAX, l = 0.f;
+            for (int j = 0; j < n && ok; ++j, ++n_s) {
+                if (!warp_wait(&b->s_full[t], n_s & 1)) { atomicExch(a.err, 75); ok = false; break; }
+                tc_fence_after();
+                uint32_t r[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc_ld32(ts + c * 32, r[c]);
+                tc_wait_ld();
+                // columns that this row sees: up to the diagonal in the last tile of a causal row block (it holds the sequence's end too),
+                // up to the sequence's end in the last tile otherwise.  Masked scores are -inf: no score is smaller.
+                if (j + 1 == n) {
+                    const int see = a.causal ? row + 1 : w.hi - (w.lo + j * 128);
+                    if (a.causal || see < 128) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) if (c * 32 + i >= see) r[c][i] = __float_as_uint(-INFINITY);
+                    }
+                }
+                float mx = -FLT_MAX;                                       // finite, so that a tile of -inf scores gives zeros, not NaN
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) mx = max3f(mx, __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+                float alpha = 1.f;
+                bool move = false;
+                if (j == 0) m_ref = mx;
+                else if ((mx - m_ref) * c2 > 8.f) { alpha = ex2f((m_ref - mx) * c2); m_ref = mx; move = true; }
+                // S_j was issued behind P_{j-1} V_{j-1}: O is complete up to there
+                if (j > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t u[32];
+                        tc_ld32(to + c * 32, u);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * alpha);
+                        tc_st32(to + c * 32, u);
+                    }
+                }
+                const float mc = -m_ref * c2;
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int k0 = c * 64 + 2 * i;
+                        float e0, e1;
+                        fma2(__uint_as_float(r[k0 >> 5][k0 & 31]), __uint_as_float(r[(k0 + 1) >> 5][(k0 + 1) & 31]), c2, c2, mc, mc, e0, e1);
+                        const float p0 = ex2f(e0), p1 = ex2f(e1);
+                        sum0 += p0; sum1 += p1;
+                        pk[i] = Half2<T>::pack(p0, p1);
+                    }
+                    tc_st32(ts + c * 32, pk);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&b->p_full[t]);
+                l = l * alpha + (sum0 + sum1);
+            }
+            if (!ok) break;
+            float inv = 0.f;
+            if (n > 0) {
+                ok = warp_wait(&b->o_done[t], n_o & 1);
+                if (!ok) { atomicExch(a.err, 76); break; }
+                ++n_o;
+                tc_fence_after();
+                inv = 1.f / l;
+            }
+            if (row0 < w.hi) {                                            // rows of no sequence: n = 0, zeros
+                const int live = w.hi - row0;                             // rows of this warp that belong to the item
+                const int64_t ld = (int64_t)a.heads * a.hd;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t u[32];
+                    if (n > 0) {
+                        tc_ld32(to + c * 32, u);
+                        tc_wait_ld();
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) u[i] = n > 0 ? __float_as_uint(__uint_as_float(u[i]) * inv) : 0u;
+#pragma unroll
+                    for (int pass = 0; pass < 2; ++pass) {                 // the rounded output, then what the rounding took
+                        T* base = (T*)(pass ? a.out_lo : a.out);
+                        if (base == nullptr) break;
+                        base += (int64_t)row0 * ld + (int64_t)w.head * a.hd + c * 32;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t pk[4];
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) {
+                                const float x = __uint_as_float(u[8 * k + 2 * v]), y = __uint_as_float(u[8 * k + 2 * v + 1]);
+                                pk[v] = Half2<T>::pack(x, y);
+                                if (pass) { const float2 f = Half2<T>::unpack(pk[v]); pk[v] = Half2<T>::pack(x - f.x, y - f.y); }
+                            }
+                            *reinterpret_cast<uint4*>(stg + lane * STAGE_PITCH + k * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {                      // four lanes store 64 consecutive bytes of a row
+                            const int rr = k * 8 + (lane >> 2), piece = lane & 3;
+                            if (rr < live && c * 32 + piece * 8 < a.hd)
+                                *reinterpret_cast<uint4*>(base + rr * ld + piece * 8) = *reinterpret_cast<const uint4*>(stg + rr * STAGE_PITCH + piece * 16);
+                        }
+                        __syncwarp();
+                    }
+                }
+                if (a.lse && lane < live) a.lse[(int64_t)w.head * a.seqs.total + row0 + lane] = n > 0 ? m_ref * a.scale + logf(l) : 0.f;
+            }
+            if (n > 0) { tc_fence_before(); mbar_arrive(&b->o_empty[t]); }
+        }
+    } else {
+        reg_dec<REGS_OTHERS>();
+        if (warp == 8) {
+            int item = (int)blockIdx.x;
+            uint32_t n_item = 0, n_clc = 0, n_q = 0, n_k = 0, n_tail = 0;
+            bool ok = true, more = true;
+            while (ok && more) {
+                if (lane == 0) {
+                    mbar_expect_tx(&b->clc, 16);
+                    clc_ask(&b->answer, &b->clc);
+                }
+                const PackedTile t = packed_tile<256>(a.seqs, a.slots - 1 - item / a.heads);    // late tiles see most keys: they start first
+                if (t.live) {
+                    const Item w{t.lo, t.hi, t.row0, item % a.heads, t.pad ? 2 : 1};
+                    const uint32_t s = n_item & 1;
+                    if (n_item >= 2) ok = warp_wait(&b->item_empty[s], ((n_item >> 1) & 1) ^ 1);
+                    if (!ok) { if (lane == 0) atomicExch(a.err, 61); break; }
+                    if (lane == 0) { b->item[s] = w; mbar_arrive(&b->item_full[s]); }
+                    ++n_item;
+                    if (!t.pad) {
+                        const int hk = w.head / a.group, live_b = t.row0 + 128 < t.hi ? 1 : 0;
+                        int n = blocks(w, 0);
+                        if (live_b) n = blocks(w, 1);
+                        if (n_q > 0) ok = warp_wait(&b->q_empty, (n_q - 1) & 1);
+                        if (!ok) { if (lane == 0) atomicExch(a.err, 62); break; }
+                        ++n_q;
+                        if (lane == 0) {
+                            mbar_expect_tx(&b->q_full, (1 + live_b) * TILE);
+                            for (int q = 0; q <= live_b; ++q)
+                                for (int hf = 0; hf < HALVES; ++hf) tma_load_3d(sQ + q * TILE + hf * HALF_TILE, &map_q, hf * 64, w.head, t.row0 + q * 128, &b->q_full);
+                        }
+                        for (int j = 0; j < n && ok; ++j, ++n_k) {
+                            const uint32_t r = n_k & 1, par = ((n_k >> 1) & 1) ^ 1;
+                            const int row = t.lo + j * 128, have = t.hi - row;
+                            if (n_k >= 2) ok = warp_wait(&b->k_empty[r], par);
+                            if (!ok) { if (lane == 0) atomicExch(a.err, 63); break; }
+                            if (lane == 0) {
+                                mbar_expect_tx(&b->k_full[r], TILE);
+                                for (int hf = 0; hf < HALVES; ++hf) tma_load_3d(sK + r * TILE + hf * HALF_TILE, &map_k, hf * 64, hk, row, &b->k_full[r]);
+                            }
+                            if (n_k >= 2) ok = warp_wait(&b->v_empty[r], par);
+                            if (!ok) { if (lane == 0) atomicExch(a.err, 64); break; }
+                            uint64_t* bar = have < 128 ? &b->v_tail : &b->v_full[r];
+                            if (lane == 0) {
+                                mbar_expect_tx(bar, TILE);
+                                for (int hf = 0; hf < HALVES; ++hf) tma_load_3d(sV + r * TILE + hf * HALF_TILE, &map_v, hf * 64, hk, row, bar);
+                            }
+                            if (have < 128) {
+                                ok = warp_wait(&b->v_tail, n_tail & 1);
+                                if (!ok) { if (lane == 0) atomicExch(a.err, 65); break; }
+                                ++n_tail;
+                                zero_rows<HALVES>(sV + r * TILE, have);
+                                if (lane == 0) mbar_arrive(&b->v_full[r]);
+                            }
+                        }
+                    }
+                }
+                if (!warp_wait(&b->clc, n_clc & 1)) { if (lane == 0) atomicExch(a.err, 66); ok = false; break; }
+                ++n_clc;
+                more = clc_answer(&b->answer, item);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the answer has been read before the next one is written over it
+                __syncwarp();
+            }
+            if (ok && (n_item < 2 || warp_wait(&b->item_empty[n_item & 1], ((n_item >> 1) & 1) ^ 1)) && lane == 0) {
+                b->item[n_item & 1].kind = 0;
+                mbar_arrive(&b->item_full[n_item & 1]);
+            }
+        } else if (warp == 9) {
+            if (lane == 0) {
+                const uint32_t idesc_qk = idesc_f16(Half2<T>::FMT, 128, 128, 0), idesc_pv = idesc_f16(Half2<T>::FMT, 128, (a.hd + 15) / 16 * 16, 1);
+                const int ksteps = (a.hd + 15) / 16;
+                uint32_t n_item = 0, n_q = 0, n_k = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};
+                bool ok = true;
+                while (ok) {
+                    const uint32_t si = n_item & 1;
+                    if (!mbar_wait(&b->item_full[si], (n_item >> 1) & 1)) { atomicExch(a.err, 67); break; }
+                    const Item w = b->item[si];
+                    mbar_arrive(&b->item_empty[si]);
+                    ++n_item;
+                    if (w.kind == 0) break;
+                    if (w.kind == 2) continue;
+                    const int nA = blocks(w, 0), nB = blocks(w, 1), n = nB > 0 ? nB : nA, lastt = nB > 0 ? 1 : 0;
+                    if (!mbar_wait(&b->q_full, n_q & 1)) { atomicExch(a.err, 68); ok = false; break; }
+                    ++n_q;
+                    auto issue_qk = [&](int t, int j) {
+                        const uint32_t r = (n_k + j) & 1, q0 = smem_u32(sQ + t * TILE), k0 = smem_u32(sK + r * TILE);
+                        for (int kk = 0; kk < ksteps; ++kk)
+                            tc_mma_bf16(tmem + t * 128, make_desc_sw128(q0 + (kk / 4) * HALF_TILE) + 2 * (kk % 4), make_desc_sw128(k0 + (kk / 4) * HALF_TILE) + 2 * (kk % 4),
+                                        idesc_qk, kk > 0 ? 1u : 0u);
+                        if (t == lastt) { tc_commit(&b->k_empty[r]); if (j + 1 == n) tc_commit(&b->q_empty); }
+                        tc_commit(&b->s_full[t]);
+                    };
+                    auto issue_pv = [&](int t, int j, int nt) {
+                        const uint32_t r = (n_k + j) & 1, v0 = smem_u32(sV + r * TILE);
+    #pragma unroll
+                        for (int kk = 0; kk < 8; ++kk)
+                            tc_mma_bf16_ta(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, make_desc_sw128_mn(v0 + kk * 2048, HALF_TILE, 1024), idesc_pv,
+                                           (j > 0 || kk > 0) ? 1u : 0u);
+                        if (t == lastt) tc_commit(&b->v_empty[r]);
+                        if (j + 1 == nt) tc_commit(&b->o_done[t]);
+                    };
+                    if (!mbar_wait(&b->k_full[n_k & 1], (n_k >> 1) & 1)) { atomicExch(a.err, 69); ok = false; break; }
+                    tc_fence_after();
+                    issue_qk(0, 0);
+                    if (nB > 0) issue_qk(1, 0);
+                    for (int j = 0; j < n && ok; ++j) {
+                        const uint32_t g = n_k + j;
+                        if (!mbar_wait(&b->v_full[g & 1], (g >> 1) & 1)) { atomicExch(a.err, 70); ok = false; break; }
+                        if (j + 1 < n && !mbar_wait(&b->k_full[(g + 1) & 1], ((g + 1) >> 1) & 1)) { atomicExch(a.err, 71); ok = false; break; }
+                        for (int t = 0; t < 2 && ok; ++t) {
+                            const int nt = t == 0 ? nA : nB;
+                            if (j >= nt) continue;
+                            if (j == 0 && n_o[t] > 0 && !mbar_wait(&b->o_empty[t], (n_o[t] - 1) & 1)) { atomicExch(a.err, 72); ok = false; break; }
+                            if (!mbar_wait(&b->p_full[t], n_p[t] & 1)) { atomicExch(a.err, 73); ok = false; break; }
+                            ++n_p[t];
+                            tc_fence_after();
+                            issue_pv(t, j, nt);
+                            if (j + 1 < nt) issue_qk(t, j + 1);
+                        }
+                    }
+                    n_k += n;
+                    ++n_o[0];
+                    if (nB > 0) ++n_o[1];
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+bool head_map(CUtensorMap* m, const void* base, const PackedAttn& p, int heads, int64_t ld, int64_t hs) {
+    return make_map_heads(m, base, p.seqs.total, heads, p.hd, ld, hs, 128);
+}
+
+template <typename T, int HD> int fwd(const PackedAttn& p, int* err, cudaStream_t st) {
+    CUtensorMap mq, mk, mv;
+    const int hk = p.heads / p.group;
+    if (!head_map(&mq, p.q, p, p.heads, p.q_ld, p.q_hs) || !head_map(&mk, p.k, p, hk, p.k_ld, p.k_hs) || !head_map(&mv, p.v, p, hk, p.v_ld, p.v_hs)) return 10;
+    constexpr size_t smem = 6 * (HD / 64) * HALF_TILE + 8 * 32 * STAGE_PITCH + sizeof(FwdBars) + 1024;
+    static std::atomic<uint64_t> done{0};
+    if (!once_per_device(done, current_device(), [&] {
+            return cudaFuncSetAttribute(packed_fwd_sm100_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess;
+        })) return 11;
+    const FwdArgs a{p.out, p.out_lo, p.lse, p.seqs, p.heads, p.group, p.hd, p.causal, packed_slots(p.seqs.n, p.seqs.total, 256), p.scale, err};
+    count_launch();
+    packed_fwd_sm100_kernel<T, HD><<<(unsigned)a.slots * (unsigned)p.heads, FWD_THREADS, smem, st>>>(mq, mk, mv, a);
+    return cudaGetLastError() == cudaSuccess ? 0 : 12;
+}
+
+}  // namespace
+
+// Scores are compared before they are scaled, so the scale has to be positive.
+bool packed_attn_sm100_takes(int dtype, const PackedAttn& p) {
+    const int hk = p.heads / p.group;
+    return dtype != F32 && p.hd % 8 == 0 && p.hd <= 128 && p.scale > 0.f && p.scale < 1e30f && packed_tma_view(p.q, p.q_ld, p.q_hs, p.seqs.total, p.heads) &&
+           packed_tma_view(p.k, p.k_ld, p.k_hs, p.seqs.total, hk) && packed_tma_view(p.v, p.v_ld, p.v_hs, p.seqs.total, hk) &&
+           (int64_t)packed_slots(p.seqs.n, p.seqs.total, 128) * p.heads < ((int64_t)1 << 31);
+}
+
+int packed_attn_sm100_fwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st) {
+    if (p.hd > 64) return dtype == BF16 ? fwd<__nv_bfloat16, 128>(p, err, st) : fwd<__half, 128>(p, err, st);
+    return dtype == BF16 ? fwd<__nv_bfloat16, 64>(p, err, st) : fwd<__half, 64>(p, err, st);
+}
+
+}  // namespace sg

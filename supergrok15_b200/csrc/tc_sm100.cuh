@@ -119,6 +119,9 @@ bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, in
 // swizzle128 = false leaves the box dense in shared memory
 bool make_map_batched(CUtensorMap* map, const void* base, int64_t batch, int64_t rows, int64_t cols, int64_t ld_elems, int box_rows, int box_cols, bool bf16,
                       bool swizzle128);
+// host: 3-D map (hd, heads, rows) over a [rows, heads, hd] view of 16-bit elements with any pitch between rows and between heads; a box is
+// box_rows rows x 64 columns of one head with 128-byte swizzle, columns past hd and rows past the end are filled with zeros
+bool make_map_heads(CUtensorMap* map, const void* base, int64_t rows, int64_t heads, int64_t hd, int64_t ld_elems, int64_t head_elems, int box_rows);
 int last_map_error();                            // CUresult of the most recent encode, -1 if the encoder could not be resolved
 
 }  // namespace tc

@@ -357,7 +357,8 @@ def attention_packed_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
 class _AttnPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, causal, scale):
-        out, rest, lse = _build.require().packed_attn_fwd(q, k, v, cu, causal, scale, True)
+        from . import gemm as _gemm
+        out, rest, lse = _build.require().packed_attn_fwd(q, k, v, cu, causal, scale, True, _gemm._err_flag(q.device))
         ctx.save_for_backward(q, k, v, cu, out, rest, lse)
         ctx.args = causal, scale
         return out
@@ -366,7 +367,8 @@ class _AttnPacked(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, cu, out, rest, lse = ctx.saved_tensors
-        return (*_build.require().packed_attn_bwd(q, k, v, cu, out, rest, lse, dout, *ctx.args), None, None, None)
+        from . import gemm as _gemm
+        return (*_build.require().packed_attn_bwd(q, k, v, cu, out, rest, lse, dout, *ctx.args, _gemm._err_flag(q.device)), None, None, None)
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, causal: bool = True,
@@ -397,7 +399,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
     if _cpp_node(q, k, v):
         train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-        return _build.require().packed_attn_node(q, k, v, cu, causal, scale, train)
+        from . import gemm as _gemm
+        return _build.require().packed_attn_node(q, k, v, cu, causal, scale, train, _gemm._err_flag(q.device))
     return _AttnPacked.apply(q, k, v, cu, causal, scale)
 
 
