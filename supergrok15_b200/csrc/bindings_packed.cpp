@@ -75,7 +75,7 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& q_, const Tensor& k_, const Te
     const Tensor q = loadable(q_), k = loadable(k_), v = loadable(v_);
     sg::PackedAttn p = packed_args(q, k, v, cu, causal, scale);
     c10::cuda::CUDAGuard guard(q.device());
-    Tensor dout = dout_.contiguous();
+    Tensor dout = loadable(dout_.contiguous());
     TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() &&
                 out.scalar_type() == q.scalar_type() && dout.device() == q.device(), "attention_packed: out and its gradient like q");
     TORCH_CHECK(lo.numel() == (q.scalar_type() == at::kFloat ? 0 : q.numel()) && lo.is_contiguous() && lo.scalar_type() == q.scalar_type(), "attention_packed: rest of out");
@@ -86,7 +86,9 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& q_, const Tensor& k_, const Te
     p.out = out.data_ptr(); p.out_lo = lo.numel() ? lo.data_ptr() : nullptr;
     p.lse = lse.data_ptr<float>(); p.dout = dout.data_ptr(); p.delta = delta.data_ptr<float>();
     p.dq = dq.data_ptr(); p.dk = dk.data_ptr(); p.dv = dv.data_ptr();
-    const int rc = sg::packed_attn_bwd(dtype_code(q), p, at::cuda::getCurrentCUDAStream());
+    const int dt = dtype_code(q);
+    auto st = at::cuda::getCurrentCUDAStream();
+    const int rc = sg::packed_attn_sm100_takes(dt, p) ? sg::packed_attn_sm100_bwd(dt, p, err.data_ptr<int>(), st) : sg::packed_attn_bwd(dt, p, st);
     TORCH_CHECK(rc == 0, "attention_packed: launch of the backward pass failed (code ", rc, ")");
     return {dq, dk, dv};
 }

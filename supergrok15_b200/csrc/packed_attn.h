@@ -30,5 +30,6 @@ inline bool packed_tma_view(const void* base, int64_t ld, int64_t hs, int64_t ro
 // The tensor-core kernels; `err` (a device word) becomes non-zero when a wait inside a kernel ran out.
 bool packed_attn_sm100_takes(int dtype, const PackedAttn& p);
 int packed_attn_sm100_fwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st);
+int packed_attn_sm100_bwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st);
 
 }  // namespace sg

@@ -433,6 +433,423 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------
+// Backward, without atomics: delta = rowsum(dO (O + rest)), then two kernels of one form, X = R0 T0^T and Y = R1 T1^T with R resident
+// and T streamed:
+//   KV = true:  an item is 128 keys of a key head (R = K, V); over the query tiles of all heads of its group (T = Q, dO)
+//               X = S^T, Y = dP^T,  dV += P^T dO,  dK += dS^T Q
+//   KV = false: an item is 128 queries of a head (R = Q, dO); over its key tiles (T = K, V)
+//               X = S, Y = dP,  dQ += dS K
+// with P = exp(scale S - lse), dS = P (dP - delta); the factor scale of dS is applied once at the end.  The second operand of every
+// accumulating product is the tile that served as K-major operand of the first, read again through an MN-major descriptor.  Two groups of
+// 128 threads share a tile, a thread has one row and 64 columns; P and dS go back to tensor memory as 16-bit A operands.  The next tile's
+// X is issued as soon as this tile's scores have been taken out, its Y as soon as dS is stored, so the tensor cores work on dV and X
+// while the threads form dS, on dK and Y while they form the next P.
+// P and dS are rounded to 16 bits to be operands (half a step of each value); everything they come from and are added to is fp32.
+struct BwdBars {
+    uint64_t item_full[2], item_empty[2], clc, res_full, res_empty, ring_full[2], ring_empty[2], tail, a_full, b_full, pa_full, pb_full, vec_full, done;
+    uint4 answer;
+    Item item[2];
+    uint32_t tmem_slot;
+};
+
+struct BwdArgs {
+    const float *lse, *delta;
+    void *out0, *out1;                                                    // dV, dK, or dQ
+    PackedSeqs seqs;
+    int heads, group, hd, causal, slots;
+    float scale;
+    int* err;
+};
+
+template <typename T, int HD, bool KV>
+__global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                                                                          const __grid_constant__ BwdArgs a) {
+    constexpr int HALVES = HD / 64;
+    constexpr uint32_t TILE = HALVES * HALF_TILE;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sR0 = smem;
+    uint8_t* sR1 = sR0 + TILE;
+    uint8_t* sT0 = sR1 + TILE;                                            // [2]
+    uint8_t* sT1 = sT0 + 2 * TILE;                                        // [2]
+    float* s_lse = reinterpret_cast<float*>(sT1 + 2 * TILE);              // [2][128]  -lse * log2(e)
+    float* s_del = s_lse + 256;                                           // [2][128]
+    uint8_t* s_stage = reinterpret_cast<uint8_t*>(s_del + 256);
+    BwdBars* b = reinterpret_cast<BwdBars*>(s_stage + 8 * 32 * STAGE_PITCH);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_heads = KV ? a.heads / a.group : a.heads;                 // heads of the items
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 9); mbar_init(&b->ring_full[i], 1); mbar_init(&b->ring_empty[i], 1);
+        }
+        mbar_init(&b->clc, 1); mbar_init(&b->res_full, 1); mbar_init(&b->res_empty, 1); mbar_init(&b->tail, 1); mbar_init(&b->a_full, 1); mbar_init(&b->b_full, 1);
+        mbar_init(&b->pa_full, 256); mbar_init(&b->pb_full, 256); mbar_init(&b->vec_full, 256); mbar_init(&b->done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&b->tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = b->tmem_slot, tm_x = tmem, tm_y = tmem + 128, tm_acc0 = tmem + 256, tm_acc1 = tmem + 384;
+
+    // tiles of the other axis that one head of an item meets: [first, first + count) in tiles of 128 rows from the sequence's begin
+    auto first_tile = [&](const Item& w) { return KV && a.causal ? (w.row0 - w.lo) / 128 : 0; };
+    auto tiles = [&](const Item& w) {
+        if (!KV && a.causal) return (w.row0 - w.lo) / 128 + 1;
+        return (w.hi - w.lo + 127) / 128 - first_tile(w);
+    };
+
+    if (warp < 8) {
+        reg_inc<REGS_SOFTMAX>();
+        const int q = warp & 3, g = warp >> 2, row = q * 32 + lane, tl = (int)threadIdx.x;
+        const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
+        const uint32_t my_x = tm_x + lane_addr + g * 64, my_y = tm_y + lane_addr + g * 64;
+        const float c2 = a.scale * LOG2E;
+        uint8_t* stg = s_stage + warp * 32 * STAGE_PITCH;
+        uint32_t n_item = 0, n = 0, n_done = 0;
+        bool ok = true;
+        auto take = [&](Item& w) {
+            const uint32_t si = n_item & 1;
+            if (!warp_wait(&b->item_full[si], (n_item >> 1) & 1)) { atomicExch(a.err, 81); return false; }
+            w = b->item[si];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b->item_empty[si]);
+            ++n_item;
+            return true;
+        };
+        // KV: the per-query vectors of a tile, one value per thread (threads 0..127 -lse log2 e, 128..255 delta); queries past the end get
+        // probability zero.  Else: both values of the thread's own query.
+        auto fetch = [&](const Item& w, int h, int i) {
+            const int r = w.lo + i * 128 + (tl & 127);
+            if (r >= w.hi) return tl < 128 ? -INFINITY : 0.f;
+            const int64_t at = (int64_t)h * a.seqs.total + r;
+            return tl < 128 ? -LOG2E * a.lse[at] : a.delta[at];
+        };
+        float v0 = 0.f, v1 = 0.f;
+        auto fetch_first = [&](const Item& w) {
+            if (w.kind != 1) return;
+            if (KV) v0 = fetch(w, w.head * a.group, first_tile(w));
+            else if (w.row0 + row < w.hi) {
+                const int64_t at = (int64_t)w.head * a.seqs.total + w.row0 + row;
+                v0 = a.lse[at]; v1 = a.delta[at];
+            }
+        };
+        Item w;
+        ok = take(w);
+        if (ok) fetch_first(w);
+        while (ok && w.kind != 0) {
+            const int per_head = w.kind == 1 ? tiles(w) : 0, n_it = KV ? per_head * a.group : per_head;
+            const float lse_row = v0 * LOG2E, del_row = v1;
+            if (KV && n_it > 0) {
+                (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = v0;    // buffer n & 1: every thread has left iteration n - 2
+                mbar_arrive(&b->vec_full);
+            }
+            int h = KV ? w.head * a.group : w.head, i = first_tile(w);
+            const int i0 = i, i1 = i + per_head;
+            for (int it = 0; it < n_it; ++it, ++n) {
+                const int bs = n & 1;
+                // the vectors of the NEXT tile are fetched now and parked in the other buffer at the end of this iteration
+                float nx = 0.f;
+                const bool diag = a.causal && i == (KV ? i0 : i1 - 1);
+                const int see = KV ? 128 : w.hi - (w.lo + i * 128);      // keys of this tile that exist
+                if (++i == i1 && KV) { i = i0; ++h; }
+                if (KV && it + 1 < n_it) nx = fetch(w, h, i);
+                if (KV && !warp_wait(&b->vec_full, n & 1)) { atomicExch(a.err, 82); ok = false; break; }
+                if (!warp_wait(&b->a_full, n & 1)) { atomicExch(a.err, 83); ok = false; break; }
+                tc_fence_after();
+                uint32_t r[2][32];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) tc_ld32(my_x + c * 32, r[c]);
+                tc_wait_ld();
+                if (!KV) { tc_fence_before(); mbar_arrive(&b->pa_full); }         // P stays in registers: X is free
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        float4 nl = make_float4(-lse_row, -lse_row, -lse_row, -lse_row);
+                        if (KV) nl = *reinterpret_cast<const float4*>(s_lse + bs * 128 + g * 64 + c * 32 + k);
+                        float e0, e1, e2, e3;
+                        fma2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1]), c2, c2, nl.x, nl.y, e0, e1);
+                        fma2(__uint_as_float(r[c][k + 2]), __uint_as_float(r[c][k + 3]), c2, c2, nl.z, nl.w, e2, e3);
+                        r[c][k] = __float_as_uint(ex2f(e0)); r[c][k + 1] = __float_as_uint(ex2f(e1));
+                        r[c][k + 2] = __float_as_uint(ex2f(e2)); r[c][k + 3] = __float_as_uint(ex2f(e3));
+                    }
+                if (diag || see < 128) {
+                    // KV: key `row` is seen by the queries (columns) from the diagonal on; else query `row` sees the keys up to it, and those
+                    // that exist
+                    const int from = KV ? row - g * 64 : 0, to = KV ? 64 : (diag ? row + 1 : see) - g * 64;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) if (c * 32 + k < from || c * 32 + k >= to) r[c][k] = 0u;
+                }
+                uint32_t d[2][32];                                       // dP; d[0] also takes the packed operands, in place
+                if (KV) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) d[0][k] = Half2<T>::pack(__uint_as_float(r[k >> 4][(2 * k) & 31]), __uint_as_float(r[k >> 4][(2 * k + 1) & 31]));
+                    tc_st32(my_x, d[0]);
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&b->pa_full);
+                }
+                if (!warp_wait(&b->b_full, n & 1)) { atomicExch(a.err, 84); ok = false; break; }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 2; ++c) tc_ld32(my_y + c * 32, d[c]);
+                tc_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {                         // columns 2k .. 2k+3 of this group
+                    float4 de = make_float4(del_row, del_row, del_row, del_row);
+                    if (KV) de = *reinterpret_cast<const float4*>(s_del + bs * 128 + g * 64 + 2 * k);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int c = k >> 4, k0 = (2 * k + 2 * u) & 31;
+                        float t0, t1, s0, s1;
+                        fma2(u ? de.z : de.x, u ? de.w : de.y, -1.f, -1.f, __uint_as_float(d[c][k0]), __uint_as_float(d[c][k0 + 1]), t0, t1);   // dP - delta
+                        fma2(__uint_as_float(r[c][k0]), __uint_as_float(r[c][k0 + 1]), t0, t1, 0.f, 0.f, s0, s1);
+                        d[0][k + u] = Half2<T>::pack(s0, s1);             // its own columns or ones already used
+                    }
+                }
+                tc_st32(my_y, d[0]);                                      // this group alone has read these columns
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&b->pb_full);
+                if (KV && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = nx; mbar_arrive(&b->vec_full); }
+            }
+            if (!ok) break;
+            const Item cur = w;
+            ok = take(w);
+            if (!ok) break;
+            fetch_first(w);
+            if (n_it > 0) {
+                if (!warp_wait(&b->done, n_done & 1)) { atomicExch(a.err, 85); ok = false; break; }
+                ++n_done;
+                tc_fence_after();
+            }
+            // KV: group 0 writes dV, group 1 dK; else each group writes half of the columns of dQ.  Rows of no sequence: zeros
+            const int row0 = cur.row0 + q * 32, live = cur.hi - row0;
+            if (live > 0) {
+                const int64_t ld = (int64_t)n_heads * a.hd;
+                T* base = (T*)(KV && g == 1 ? a.out1 : a.out0) + (int64_t)row0 * ld + (int64_t)cur.head * a.hd;
+                const float f = KV && g == 0 ? 1.f : a.scale;
+                const uint32_t acc = (KV && g == 1 ? tm_acc1 : tm_acc0) + lane_addr;
+                const int c0 = KV ? 0 : g * (HD / 64), c1 = KV ? HD / 32 : c0 + HD / 64;
+#pragma unroll 1
+                for (int c = c0; c < c1; ++c) {
+                    uint32_t t[32];
+                    if (n_it > 0) {
+                        tc_ld32(acc + c * 32, t);
+                        tc_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) t[k] = 0u;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) pk[e] = Half2<T>::pack(__uint_as_float(t[8 * u + 2 * e]) * f, __uint_as_float(t[8 * u + 2 * e + 1]) * f);
+                        *reinterpret_cast<uint4*>(stg + lane * STAGE_PITCH + u * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int rr = u * 8 + (lane >> 2), piece = lane & 3;
+                        if (rr < live && c * 32 + piece * 8 < a.hd)
+                            *reinterpret_cast<uint4*>(base + rr * ld + c * 32 + piece * 8) = *reinterpret_cast<const uint4*>(stg + rr * STAGE_PITCH + piece * 16);
+                    }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();                                            // the accumulators have been read: the next item's products wait for this
+        }                                                                 // group's pa_full / pb_full
+    } else {
+        reg_dec<REGS_OTHERS>();
+        if (warp == 8) {
+            int item = (int)blockIdx.x;
+            uint32_t n_item = 0, n_clc = 0, n_res = 0, n = 0, n_tail = 0;
+            bool ok = true, more = true;
+            while (ok && more) {
+                if (lane == 0) {
+                    mbar_expect_tx(&b->clc, 16);
+                    clc_ask(&b->answer, &b->clc);
+                }
+                // the tiles with the most work start first: early keys are seen by most queries, late queries see most keys
+                const int ord = item / n_heads;
+                const PackedTile t = packed_tile<128>(a.seqs, KV ? ord : a.slots - 1 - ord);
+                if (t.live) {
+                    const Item w{t.lo, t.hi, t.row0, item % n_heads, t.pad ? 2 : 1};
+                    const uint32_t s = n_item & 1;
+                    if (n_item >= 2) ok = warp_wait(&b->item_empty[s], ((n_item >> 1) & 1) ^ 1);
+                    if (!ok) { if (lane == 0) atomicExch(a.err, 86); break; }
+                    if (lane == 0) { b->item[s] = w; mbar_arrive(&b->item_full[s]); }
+                    ++n_item;
+                    const int per_head = t.pad ? 0 : tiles(w), n_it = KV ? per_head * a.group : per_head, i0 = first_tile(w);
+                    const int hk = KV ? w.head : w.head / a.group;
+                    int h = KV ? w.head * a.group : w.head, i = i0;
+                    for (int it = 0; it < n_it; ++it, ++n) {
+                        const uint32_t r = n & 1;
+                        const int row = t.lo + i * 128, have = t.hi - row;
+                        if (n >= 2) ok = warp_wait(&b->ring_empty[r], ((n >> 1) & 1) ^ 1);
+                        if (!ok) { if (lane == 0) atomicExch(a.err, 87); break; }
+                        uint64_t* bar = have < 128 ? &b->tail : &b->ring_full[r];
+                        if (lane == 0) {
+                            mbar_expect_tx(bar, 2 * TILE);
+                            for (int hf = 0; hf < HALVES; ++hf) {
+                                tma_load_3d(sT0 + r * TILE + hf * HALF_TILE, KV ? &map_q : &map_k, hf * 64, KV ? h : hk, row, bar);
+                                tma_load_3d(sT1 + r * TILE + hf * HALF_TILE, KV ? &map_do : &map_v, hf * 64, KV ? h : hk, row, bar);
+                            }
+                        }
+                        if (it == 0) {
+                            if (n_res > 0) ok = warp_wait(&b->res_empty, (n_res - 1) & 1);
+                            if (!ok) { if (lane == 0) atomicExch(a.err, 88); break; }
+                            ++n_res;
+                            if (lane == 0) {
+                                mbar_expect_tx(&b->res_full, 2 * TILE);
+                                for (int hf = 0; hf < HALVES; ++hf) {
+                                    tma_load_3d(sR0 + hf * HALF_TILE, KV ? &map_k : &map_q, hf * 64, w.head, t.row0, &b->res_full);
+                                    tma_load_3d(sR1 + hf * HALF_TILE, KV ? &map_v : &map_do, hf * 64, w.head, t.row0, &b->res_full);
+                                }
+                            }
+                        }
+                        if (have < 128) {
+                            ok = warp_wait(&b->tail, n_tail & 1);
+                            if (!ok) { if (lane == 0) atomicExch(a.err, 89); break; }
+                            ++n_tail;
+                            zero_rows<HALVES>(sT0 + r * TILE, have);
+                            zero_rows<HALVES>(sT1 + r * TILE, have);
+                            if (lane == 0) mbar_arrive(&b->ring_full[r]);
+                        }
+                        if (++i == i0 + per_head) { i = i0; ++h; }
+                    }
+                    if (!ok) break;
+                }
+                if (!warp_wait(&b->clc, n_clc & 1)) { if (lane == 0) atomicExch(a.err, 90); ok = false; break; }
+                ++n_clc;
+                more = clc_answer(&b->answer, item);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the answer has been read before the next one is written over it
+                __syncwarp();
+            }
+            if (ok && (n_item < 2 || warp_wait(&b->item_empty[n_item & 1], ((n_item >> 1) & 1) ^ 1)) && lane == 0) {
+                b->item[n_item & 1].kind = 0;
+                mbar_arrive(&b->item_full[n_item & 1]);
+            }
+        } else if (warp == 9 && lane == 0) {
+            const uint32_t idesc_first = idesc_f16(Half2<T>::FMT, 128, 128, 0), idesc_acc = idesc_f16(Half2<T>::FMT, 128, (a.hd + 15) / 16 * 16, 1);
+            const int ksteps = (a.hd + 15) / 16;
+            uint32_t n_item = 0, n_res = 0;
+            // iterations of the next item; 0 at the end of the work, -1 when a wait ran out, -2 for rows of no sequence
+            auto take = [&]() {
+                const uint32_t si = n_item & 1;
+                if (!mbar_wait(&b->item_full[si], (n_item >> 1) & 1)) { atomicExch(a.err, 91); return -1; }
+                const Item w = b->item[si];
+                mbar_arrive(&b->item_empty[si]);
+                ++n_item;
+                if (w.kind != 1) return w.kind == 0 ? 0 : -2;
+                return KV ? tiles(w) * a.group : tiles(w);
+            };
+            auto first_product = [&](uint32_t tm, const uint8_t* res, const uint8_t* ring) {
+                const uint32_t r0 = smem_u32(res), t0 = smem_u32(ring);
+                for (int kk = 0; kk < ksteps; ++kk)
+                    tc_mma_bf16(tm, make_desc_sw128(r0 + (kk / 4) * HALF_TILE) + 2 * (kk % 4), make_desc_sw128(t0 + (kk / 4) * HALF_TILE) + 2 * (kk % 4), idesc_first,
+                                kk > 0 ? 1u : 0u);
+            };
+            // acc += A T, A the 16-bit operand in the columns of X or Y (its second half starts at column 64), T a ring tile read MN-major
+            auto acc_product = [&](uint32_t acc, uint32_t tm, const uint8_t* ring, bool add) {
+                const uint32_t t0 = smem_u32(ring);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    tc_mma_bf16_ta(acc, tm + (kk >> 2) * 64 + (kk & 3) * 8, make_desc_sw128_mn(t0 + kk * 2048, HALF_TILE, 1024), idesc_acc, (add || kk > 0) ? 1u : 0u);
+            };
+            auto tiles_ready = [&](uint32_t n, bool first_it) {
+                if (first_it) {
+                    if (!mbar_wait(&b->res_full, n_res & 1)) { atomicExch(a.err, 92); return false; }
+                    ++n_res;
+                }
+                if (!mbar_wait(&b->ring_full[n & 1], (n >> 1) & 1)) { atomicExch(a.err, 93); return false; }
+                tc_fence_after();
+                return true;
+            };
+            bool ok = true;
+            int n_it = -2;
+            for (uint32_t n = 0; ok && n_it != 0;) {
+                if (n_it < 0) {                                           // no item's first products are on their way
+                    do n_it = take(); while (n_it == -2);
+                    if (n_it <= 0) break;
+                    if (!tiles_ready(n, true)) break;
+                    first_product(tm_x, sR0, sT0 + (n & 1) * TILE);
+                    tc_commit(&b->a_full);
+                    first_product(tm_y, sR1, sT1 + (n & 1) * TILE);
+                    tc_commit(&b->b_full);
+                    if (n_it == 1) tc_commit(&b->res_empty);
+                }
+                int n_next = 0;
+                for (int it = 0; it < n_it; ++it, ++n) {
+                    const int s = n & 1, ns = s ^ 1;
+                    const bool last = it + 1 == n_it;
+                    // one item ahead, no further: the other warps take the item behind it only when this one is done
+                    if (last) { n_next = take(); if (n_next == -1) { ok = false; break; } }
+                    const bool next = !last || n_next > 0;
+                    if (!mbar_wait(&b->pa_full, n & 1)) { atomicExch(a.err, 94); ok = false; break; }
+                    tc_fence_after();
+                    if (KV) acc_product(tm_acc0, tm_x, sT1 + s * TILE, it > 0);                          // dV += P^T dO
+                    if (next) {
+                        if (!tiles_ready(n + 1, last)) { ok = false; break; }
+                        first_product(tm_x, sR0, sT0 + ns * TILE);
+                        tc_commit(&b->a_full);
+                    }
+                    if (!mbar_wait(&b->pb_full, n & 1)) { atomicExch(a.err, 95); ok = false; break; }
+                    tc_fence_after();
+                    acc_product(KV ? tm_acc1 : tm_acc0, tm_y, sT0 + s * TILE, it > 0);                   // dK += dS^T Q / dQ += dS K
+                    tc_commit(&b->ring_empty[s]);
+                    if (last) tc_commit(&b->done);
+                    if (next) {
+                        first_product(tm_y, sR1, sT1 + ns * TILE);
+                        tc_commit(&b->b_full);
+                        if (last ? n_next == 1 : it + 2 == n_it) tc_commit(&b->res_empty);               // the last first products of their item
+                    }
+                }
+                n_it = n_next;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// delta[head][row] = dO . (O + rest): 16 bytes of each per lane, 8 or 16 lanes per (row, head)
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) packed_delta_sm100_kernel(PackedAttn p) {
+    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+    const int part = (int)(threadIdx.x % LANES);
+    const bool live = item < (int64_t)p.seqs.total * p.heads;
+    float acc = 0.f;
+    if (live && part * 8 < p.hd) {
+        const int64_t at = item * p.hd + part * 8;
+        const uint4 o = *reinterpret_cast<const uint4*>((const T*)p.out + at), e = *reinterpret_cast<const uint4*>((const T*)p.out_lo + at),
+                    d = *reinterpret_cast<const uint4*>((const T*)p.dout + at);
+        const uint32_t ov[4] = {o.x, o.y, o.z, o.w}, ev[4] = {e.x, e.y, e.z, e.w}, dv[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 x = Half2<T>::unpack(ov[k]), y = Half2<T>::unpack(ev[k]), z = Half2<T>::unpack(dv[k]);
+            acc = fmaf(x.x + y.x, z.x, fmaf(x.y + y.y, z.y, acc));
+        }
+    }
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (live && part == 0) p.delta[(item % p.heads) * p.seqs.total + item / p.heads] = acc;
+}
+
 bool head_map(CUtensorMap* m, const void* base, const PackedAttn& p, int heads, int64_t ld, int64_t hs) {
     return make_map_heads(m, base, p.seqs.total, heads, p.hd, ld, hs, 128);
 }
@@ -452,6 +869,28 @@ template <typename T, int HD> int fwd(const PackedAttn& p, int* err, cudaStream_
     return cudaGetLastError() == cudaSuccess ? 0 : 12;
 }
 
+template <typename T, int HD> int bwd(const PackedAttn& p, int* err, cudaStream_t st) {
+    CUtensorMap mq, mk, mv, md;
+    const int hk = p.heads / p.group;
+    if (!head_map(&mq, p.q, p, p.heads, p.q_ld, p.q_hs) || !head_map(&mk, p.k, p, hk, p.k_ld, p.k_hs) || !head_map(&mv, p.v, p, hk, p.v_ld, p.v_hs) ||
+        !head_map(&md, p.dout, p, p.heads, (int64_t)p.heads * p.hd, p.hd)) return 10;
+    constexpr size_t smem = 6 * (HD / 64) * HALF_TILE + 2048 + 8 * 32 * STAGE_PITCH + sizeof(BwdBars) + 1024;
+    static std::atomic<uint64_t> done{0};
+    if (!once_per_device(done, current_device(), [&] {
+            return cudaFuncSetAttribute(packed_bwd_sm100_kernel<T, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
+                   cudaFuncSetAttribute(packed_bwd_sm100_kernel<T, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess;
+        })) return 11;
+    constexpr int LANES = HD / 8;
+    const int slots = packed_slots(p.seqs.n, p.seqs.total, 128);
+    BwdArgs a{p.lse, p.delta, p.dv, p.dk, p.seqs, p.heads, p.group, p.hd, p.causal, slots, p.scale, err};
+    count_launch(3);
+    packed_delta_sm100_kernel<T, LANES><<<(unsigned)(((int64_t)p.seqs.total * p.heads * LANES + 255) / 256), 256, 0, st>>>(p);
+    packed_bwd_sm100_kernel<T, HD, true><<<(unsigned)slots * (unsigned)hk, FWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
+    a.out0 = p.dq; a.out1 = nullptr;
+    packed_bwd_sm100_kernel<T, HD, false><<<(unsigned)slots * (unsigned)p.heads, FWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
+    return cudaGetLastError() == cudaSuccess ? 0 : 12;
+}
+
 }  // namespace
 
 // Scores are compared before they are scaled, so the scale has to be positive.
@@ -465,6 +904,10 @@ bool packed_attn_sm100_takes(int dtype, const PackedAttn& p) {
 int packed_attn_sm100_fwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st) {
     if (p.hd > 64) return dtype == BF16 ? fwd<__nv_bfloat16, 128>(p, err, st) : fwd<__half, 128>(p, err, st);
     return dtype == BF16 ? fwd<__nv_bfloat16, 64>(p, err, st) : fwd<__half, 64>(p, err, st);
+}
+int packed_attn_sm100_bwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st) {
+    if (p.hd > 64) return dtype == BF16 ? bwd<__nv_bfloat16, 128>(p, err, st) : bwd<__half, 128>(p, err, st);
+    return dtype == BF16 ? bwd<__nv_bfloat16, 64>(p, err, st) : bwd<__half, 64>(p, err, st);
 }
 
 }  // namespace sg

@@ -82,6 +82,14 @@ def test_many_sequences(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_mostly_padding(dtype):
+    """Long runs of work items without a sequence, before, between and behind items with one."""
+    q, k, v, do, cu = inputs([300], 30000, 4, 4, 64, dtype)
+    for start in (0, 15000, 30000):
+        check(q, k, v, do, cu + start, True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides(dtype):
     """Views of one fused projection, heads before rows, a row pitch TMA cannot take, a base that is not 16-byte aligned, a broadcast head."""
     q, k, v, do, cu = inputs([70, 200], 2, 4, 4, 64, dtype)
