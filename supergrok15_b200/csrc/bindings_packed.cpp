@@ -124,6 +124,13 @@ int64_t lce_piece_rows(int64_t rows, int64_t ldu, int64_t elem, bool train) {
     return ((rows + pieces - 1) / pieces + 255) / 256 * 256;
 }
 
+// 16-bit rows that the tensor-core kernels cannot load (base or pitch not on 16 bytes) are copied once
+Tensor loadable_rows(const Tensor& t) {
+    if (t.dim() != 2 || t.element_size() != 2 || t.size(1) % 8 != 0 || t.numel() == 0) return t;
+    if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(1) == 1 && t.stride(0) > 0 && t.stride(0) % 8 == 0) return t;
+    return t.clone(at::MemoryFormat::Contiguous);
+}
+
 struct LceShape {
     sg::LceArgs a{};
     int dtype = 0;
@@ -164,7 +171,8 @@ LceShape lce_shape(const Tensor& x, const Tensor& w, const Tensor& t, int64_t ig
 // Returns (loss, {mean, 1 / count}, d of the last piece [rows, pitch], and with several pieces: fp32 dx of the others, fp32 dw of the others).
 // The gradient products of the last piece are left to the backward pass, which writes them in the final type; of the pieces before it the
 // products are taken here, because their d makes room for the next one's.
-std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
+std::vector<Tensor> lce_fwd(const Tensor& x_, const Tensor& w_, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
+    const Tensor x = loadable_rows(x_), w = loadable_rows(w_);
     const bool train = need_x || need_w;
     LceShape s = lce_shape(x, w, t, ignore_index, train);
     c10::cuda::CUDAGuard guard(x.device());
@@ -194,7 +202,8 @@ std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w, const Tensor& t, i
                 g.dw = need_w ? dw.data_ptr() : nullptr;
                 g.dw_prev = need_w && r0 > 0 ? dw.data_ptr<float>() : nullptr;
                 g.f32_out = true;
-                rc = sg::lce_grads(s.dtype, a, g, err.data_ptr<int>(), st);
+                Tensor scratch = at::empty({sg::lce_scratch(s.dtype, a, need_x, need_w)}, fo);
+                rc = sg::lce_grads(s.dtype, a, g, scratch.data_ptr<float>(), err.data_ptr<int>(), st);
             }
             TORCH_CHECK(rc == 0, "linear_cross_entropy: launch failed (code ", rc, ")");
         }
@@ -204,8 +213,9 @@ std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w, const Tensor& t, i
     return {mean.narrow(0, 0, 1).reshape({}), mean, u, dx.defined() ? dx : none, dw.defined() ? dw : none};
 }
 
-std::vector<Tensor> lce_bwd(const Tensor& x, const Tensor& w, const Tensor& t, const Tensor& mean, const Tensor& u, const Tensor& dx32, const Tensor& dw32,
+std::vector<Tensor> lce_bwd(const Tensor& x_, const Tensor& w_, const Tensor& t, const Tensor& mean, const Tensor& u, const Tensor& dx32, const Tensor& dw32,
                             const Tensor& gout_, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
+    const Tensor x = loadable_rows(x_), w = loadable_rows(w_);
     LceShape s = lce_shape(x, w, t, ignore_index, true);
     c10::cuda::CUDAGuard guard(x.device());
     auto st = at::cuda::getCurrentCUDAStream();
@@ -227,14 +237,16 @@ std::vector<Tensor> lce_bwd(const Tensor& x, const Tensor& w, const Tensor& t, c
     g.dw_prev = need_w && last > 0 ? dw32.data_ptr<float>() : nullptr;
     g.gout = gout.data_ptr<float>();
     g.inv_count = mean.data_ptr<float>() + 1;
-    int rc = sg::lce_grads(s.dtype, a, g, err.data_ptr<int>(), st);
+    Tensor scratch = at::empty({sg::lce_scratch(s.dtype, a, need_x, need_w)}, gout.options());
+    int rc = sg::lce_grads(s.dtype, a, g, scratch.data_ptr<float>(), err.data_ptr<int>(), st);
     if (rc == 0 && need_x) rc = sg::lce_finish(s.dtype, dx32.data_ptr<float>(), dx.data_ptr(), last * D, g.gout, g.inv_count, st);
     TORCH_CHECK(rc == 0, "linear_cross_entropy: launch of the backward pass failed (code ", rc, ")");
     return {dx, dw};
 }
 
 struct LceNode : Function<LceNode> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, const Tensor& err) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, const Tensor& err) {
+        const Tensor x = loadable_rows(x_), w = loadable_rows(w_);        // the copy, where there is one, is what the backward pass reads
         auto r = lce_fwd(x, w, t, ignore_index, need_x, need_w, err);
         if (need_x || need_w) ctx->save_for_backward({x, w, t, r[1], r[2], r[3], r[4]});
         ctx->saved_data["err"] = err;                                     // the process's time-out flag itself, not a saved tensor

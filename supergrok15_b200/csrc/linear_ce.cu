@@ -23,8 +23,6 @@
 #include <cfloat>
 
 namespace sg {
-template <> struct LceUnit<__half> { static constexpr float value = 32768.f; };
-
 namespace {
 
 constexpr int CT = 64, CK = 16, CTHREADS = 256;
@@ -210,10 +208,15 @@ template <typename T, typename TO> int grads(const LceArgs& a, const LceGrads& g
 }  // namespace
 
 #define SG_LCE_GO(fn, ...) { if (dtype == F32) return fn<float>(__VA_ARGS__); if (dtype == BF16) return fn<__nv_bfloat16>(__VA_ARGS__); return fn<__half>(__VA_ARGS__); }
-int lce_tile_columns(int, const LceArgs&) { return CT; }
-int lce_logits(int dtype, const LceArgs& a, int*, cudaStream_t st) SG_LCE_GO(logits, a, st)
+int lce_tile_columns(int dtype, const LceArgs& a) { return lce_sm100_takes(dtype, a) ? LCE_SM100_COLUMNS : CT; }
+int64_t lce_scratch(int dtype, const LceArgs& a, bool dx, bool dw) { return dx && lce_sm100_takes(dtype, a) ? lce_sm100_scratch(a.rows, a.V, a.D, dw) : 0; }
+int lce_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st) {
+    if (lce_sm100_takes(dtype, a)) return lce_sm100_logits(dtype, a, err, st);
+    SG_LCE_GO(logits, a, st)
+}
 int lce_rows(int dtype, const LceArgs& a, cudaStream_t st) SG_LCE_GO(rows, a, lce_tile_columns(dtype, a), st)
-int lce_grads(int dtype, const LceArgs& a, const LceGrads& g, int*, cudaStream_t st) {
+int lce_grads(int dtype, const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
+    if (lce_sm100_takes(dtype, a)) return lce_sm100_grads(dtype, a, g, scratch, err, st);
     if (dtype == F32) return grads<float, float>(a, g, st);
     if (dtype == BF16) return g.f32_out ? grads<__nv_bfloat16, float>(a, g, st) : grads<__nv_bfloat16, __nv_bfloat16>(a, g, st);
     return g.f32_out ? grads<__half, float>(a, g, st) : grads<__half, __half>(a, g, st);

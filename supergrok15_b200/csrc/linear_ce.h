@@ -2,6 +2,7 @@
 // linear_ce_sm100.cu: tensor cores).
 #pragma once
 #include <cstdint>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 namespace sg {
@@ -31,16 +32,25 @@ struct LceGrads {
 
 // u holds d times this: fp16 has no exponent to spare for probabilities (2^-17 for a flat row of 128,000 columns), bf16 and fp32 have
 template <typename T> struct LceUnit { static constexpr float value = 1.f; };
+template <> struct LceUnit<__half> { static constexpr float value = 32768.f; };
 
 // columns per statistics tile of the kernels that will run
 int lce_tile_columns(int dtype, const LceArgs& a);
+// floats that lce_grads needs besides (partial sums of dx)
+int64_t lce_scratch(int dtype, const LceArgs& a, bool dx, bool dw);
 
 // Return 0 or the number of the step that failed.
 int lce_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st);
 int lce_rows(int dtype, const LceArgs& a, cudaStream_t st);
-int lce_grads(int dtype, const LceArgs& a, const LceGrads& g, int* err, cudaStream_t st);
+int lce_grads(int dtype, const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st);
 // out = in * gout * inv_count / (the factor of u), rounded to dtype
 int lce_finish(int dtype, const float* in, void* out, int64_t n, const float* gout, const float* inv_count, cudaStream_t st);
+// The tensor-core kernels; `err` (a device word) becomes non-zero when a wait inside a kernel ran out.
+constexpr int LCE_SM100_COLUMNS = 128;
+bool lce_sm100_takes(int dtype, const LceArgs& a);
+int64_t lce_sm100_scratch(int rows, int V, int D, bool with_dw);
+int lce_sm100_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st);
+int lce_sm100_grads(int dtype, const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st);
 // out[0] = mean of the counted rows' losses, out[1] = 1 / max(count, 1)
 void ce_mean(const float* loss, const int64_t* target, int64_t rows, int V, int64_t ignore_index, float* out, cudaStream_t st);
 

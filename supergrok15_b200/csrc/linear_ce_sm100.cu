@@ -1,0 +1,428 @@
+// Products of the linear-head cross-entropy on the 5th-generation tensor cores (tcgen05 / TMEM / TMA), sm_100a only: 16-bit operands,
+// fp32 accumulators.  linear_ce.cu has the mathematics and the pass over the rows that stands between the two kernels.
+//
+//   LOGITS   z = x w^T, a tile of 128 rows x 256 columns at a time; the epilogue leaves maximum, sum and u = exp(z - max) of each row and
+//            half tile: the logits never reach memory
+//   GRADS    dx = d w and dw = d^T x in one launch.  dx has few tiles with a long sum (the vocabulary), dw many with a short one; the long
+//            ones start first and are cut along the sum when one alone would take longer than everything spread over the SMs.  d, w and x are
+//            read where they are, in whichever order their rows run (K-major or MN-major descriptors).
+//
+// One CTA per SM: eight warps read accumulators (two per 32 rows, 128 columns each), one loads, one issues.  The accumulator is
+// double-buffered in tensor memory, so an epilogue runs under the next tile's products; a running CTA takes over the tiles of CTAs that
+// have not started (cluster launch control), so long and short tiles balance without a counter in memory.
+#include "sg_native.h"
+#include "tc_half.cuh"
+#include "per_device.h"
+#include "linear_ce.h"
+#include <cfloat>
+
+namespace sg {
+namespace {
+using namespace tc;
+
+constexpr int BM = 128, BN = 256, BK = 64, STAGES = 4, THREADS = 320;
+constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES, OUT_BYTES = 32 * 128;
+constexpr int GROUP_M = 32;                                               // tile rows that sweep over the columns together
+
+struct LItem {
+    int m0, n0, kb0, nkb, kind, split;                                    // kind: 0 end of the work, 1 logits or dx, 2 dw
+};
+struct LBars {
+    uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], item_full[2], item_empty[2], clc;
+    uint4 answer;
+    LItem item[2];
+    uint32_t tmem_slot;
+};
+
+struct LArgs {
+    // LOGITS
+    const int64_t* target;
+    int64_t ignore_index;
+    float *tile_max, *tile_sum, *z_target;
+    int store_u;
+    // GRADS
+    const float* dw_prev;
+    const float *gout, *inv;
+    int splits, f32_x, f32_w;                                             // f32: that output is fp32 (for dx also: partial sums)
+    int items_x;                                                          // items below this are dx
+    int rows, V, D;
+    int* err;
+};
+
+// tile of the logits: m fastest inside a group of GROUP_M tile rows, so that w is streamed once per group
+__device__ __forceinline__ void logits_tile(int i, int tm, int tn, int& m, int& n) {
+    const int per = GROUP_M * tn, first = (i / per) * GROUP_M, g = tm - first < GROUP_M ? tm - first : GROUP_M, r = i % per;
+    m = first + r % g;
+    n = r / g;
+}
+
+template <typename T, bool GRADS>
+__global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
+                                                               const __grid_constant__ CUtensorMap map_c1, const __grid_constant__ CUtensorMap map_a2,
+                                                               const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ CUtensorMap map_c2,
+                                                               const __grid_constant__ LArgs a) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* s_out = smem + STAGES * STAGE;                               // [8 warps][OUT_BYTES]
+    LBars* b = reinterpret_cast<LBars*>(s_out + 8 * OUT_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&b->full[s], 1); mbar_init(&b->empty[s], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&b->acc_full[i], 1); mbar_init(&b->acc_empty[i], 8); mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 9); }
+        mbar_init(&b->clc, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&b->tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = b->tmem_slot;
+
+    if (warp == 8) {
+        int i = (int)blockIdx.x;
+        uint32_t n_item = 0, n_clc = 0, it = 0;
+        bool ok = true, more = true;
+        while (ok && more) {
+            if (lane == 0) {
+                mbar_expect_tx(&b->clc, 16);
+                clc_ask(&b->answer, &b->clc);
+            }
+            LItem w{0, 0, 0, 0, 1, 0};
+            if constexpr (!GRADS) {
+                int m, n;
+                logits_tile(i, (a.rows + BM - 1) / BM, (a.V + BN - 1) / BN, m, n);
+                w.m0 = m * BM; w.n0 = n * BN; w.nkb = (a.D + BK - 1) / BK;
+            } else {
+                const int tn = (a.D + BN - 1) / BN;
+                if (i < a.items_x) {
+                    const int tm = (a.rows + BM - 1) / BM, kb = (a.V + BK - 1) / BK, per = (kb + a.splits - 1) / a.splits;
+                    w.split = i / (tm * tn);
+                    const int r = i % (tm * tn);
+                    w.m0 = r % tm * BM; w.n0 = r / tm * BN;
+                    w.kb0 = w.split * per;
+                    w.nkb = kb - w.kb0 < per ? kb - w.kb0 : per;          // 0 or less: a split past the end, all zeros
+                    if (w.nkb < 0) w.nkb = 0;
+                } else {
+                    const int r = i - a.items_x;
+                    w.kind = 2;
+                    w.m0 = r / tn * BM; w.n0 = r % tn * BN; w.nkb = (a.rows + BK - 1) / BK;
+                }
+            }
+            const uint32_t s = n_item & 1;
+            if (n_item >= 2) ok = warp_wait(&b->item_empty[s], ((n_item >> 1) & 1) ^ 1);
+            if (!ok) { if (lane == 0) atomicExch(a.err, 101); break; }
+            ++n_item;
+            if (lane == 0) {
+                b->item[s] = w;
+                mbar_arrive(&b->item_full[s]);
+                for (int k = 0; k < w.nkb; ++k, ++it) {                   // what lies past the end of an operand is filled with zeros
+                    const uint32_t st = it % STAGES;
+                    if (it >= STAGES && !mbar_wait(&b->empty[st], ((it / STAGES) & 1) ^ 1)) { atomicExch(a.err, 102); ok = false; break; }
+                    uint8_t* dst = smem + st * STAGE;
+                    const int kc = (w.kb0 + k) * BK;
+                    mbar_expect_tx(&b->full[st], STAGE);
+                    if constexpr (!GRADS) {
+                        tma_load_2d(dst, &map_a1, kc, w.m0, &b->full[st]);
+                        tma_load_2d(dst + A_BYTES, &map_b1, kc, w.n0, &b->full[st]);
+                    } else {
+                        if (w.kind == 1) tma_load_2d(dst, &map_a1, kc, w.m0, &b->full[st]);
+                        else
+#pragma unroll
+                            for (int c = 0; c < BM / 64; ++c) tma_load_2d(dst + c * (BK * 128), &map_a2, w.m0 + 64 * c, kc, &b->full[st]);
+#pragma unroll
+                        for (int c = 0; c < BN / 64; ++c) tma_load_2d(dst + A_BYTES + c * (BK * 128), w.kind == 1 ? &map_b1 : &map_b2, w.n0 + 64 * c, kc, &b->full[st]);
+                    }
+                }
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (!warp_wait(&b->clc, n_clc & 1)) { if (lane == 0) atomicExch(a.err, 103); ok = false; break; }
+            ++n_clc;
+            more = clc_answer(&b->answer, i);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        }
+        if (ok && (n_item < 2 || warp_wait(&b->item_empty[n_item & 1], ((n_item >> 1) & 1) ^ 1)) && lane == 0) {
+            b->item[n_item & 1].kind = 0;
+            mbar_arrive(&b->item_full[n_item & 1]);
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            uint32_t n_item = 0, it = 0;
+            bool ok = true;
+            while (ok) {
+                const uint32_t s = n_item & 1;
+                if (!mbar_wait(&b->item_full[s], (n_item >> 1) & 1)) { atomicExch(a.err, 104); break; }
+                const LItem w = b->item[s];
+                mbar_arrive(&b->item_empty[s]);
+                if (w.kind == 0) break;
+                if (n_item >= 2 && !mbar_wait(&b->acc_empty[s], ((n_item >> 1) & 1) ^ 1)) { atomicExch(a.err, 105); break; }
+                ++n_item;
+                tc_fence_after();
+                const bool a_mn = GRADS && w.kind == 2, b_mn = GRADS;
+                const uint32_t idesc = idesc_f16(Half2<T>::FMT, BM, BN, b_mn) | ((uint32_t)a_mn << 15), d = tmem + s * BN;
+                for (int k = 0; k < w.nkb; ++k, ++it) {
+                    const uint32_t st = it % STAGES;
+                    if (!mbar_wait(&b->full[st], (it / STAGES) & 1)) { atomicExch(a.err, 106); ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t pa = smem_u32(smem + st * STAGE);
+                    const uint64_t da = a_mn ? make_desc_sw128_mn(pa, BK * 128, 1024) : make_desc_sw128(pa);
+                    const uint64_t db = b_mn ? make_desc_sw128_mn(pa + A_BYTES, BK * 128, 1024) : make_desc_sw128(pa + A_BYTES);
+#pragma unroll
+                    for (int k4 = 0; k4 < BK / 16; ++k4)
+                        tc_mma_bf16(d, da + (a_mn ? 128 : 2) * k4, db + (b_mn ? 128 : 2) * k4, idesc, (k > 0 || k4 > 0) ? 1u : 0u);
+                    tc_commit(&b->empty[st]);
+                }
+                tc_commit(&b->acc_full[s]);
+            }
+        }
+    } else {
+        const int q = warp & 3, half = warp >> 2;
+        const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
+        uint8_t* stg = s_out + warp * OUT_BYTES;
+        const float f = GRADS && a.gout ? a.gout[0] * a.inv[0] / LceUnit<T>::value : 1.f;
+        uint32_t n_item = 0;
+        // a box of 128 bytes x 32 rows leaves through shared memory (16-byte piece k of row r at piece k ^ (r & 7))
+        auto store_box = [&](const CUtensorMap* map, int col, int row) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(map, stg, col, row);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+            __syncwarp();
+        };
+        auto put = [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(stg + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v; };
+        while (true) {
+            const uint32_t s = n_item & 1;
+            if (!warp_wait(&b->item_full[s], (n_item >> 1) & 1)) { atomicExch(a.err, 107); break; }
+            const LItem w = b->item[s];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b->item_empty[s]);
+            if (w.kind == 0) break;
+            if (!warp_wait(&b->acc_full[s], (n_item >> 1) & 1)) { atomicExch(a.err, 108); break; }
+            ++n_item;
+            tc_fence_after();
+            const uint32_t acc = tmem + s * BN + half * 128 + lane_addr;
+            const int row = w.m0 + q * 32 + lane, n0 = w.n0 + half * 128;
+            if constexpr (!GRADS) {
+                uint32_t r[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc_ld32(acc + c * 32, r[c]);
+                tc_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b->acc_empty[s]);             // everything is in registers
+                if (n0 < a.V) {
+                    const int64_t t = row < a.rows ? a.target[row] : -1;
+                    const int tc = t >= n0 && t < n0 + 128 && t < a.V ? (int)(t - n0) : -1;        // the target's column, if it is here
+                    if (n0 + 128 > a.V) {                                 // columns past the vocabulary
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) if (n0 + c * 32 + i >= a.V) r[c][i] = __float_as_uint(-INFINITY);
+                    }
+                    float mx = -FLT_MAX;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) mx = max3f(mx, __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+                    const float mc = -mx * LOG2E;
+                    float sum0 = 0.f, sum1 = 0.f;
+                    auto chunk = [&](uint32_t (&rc)[32], int c) {         // 32 columns
+                        uint32_t zt = 0u;
+                        float et = 0.f;
+                        const bool here = (tc >> 5) == c;
+                        if (__any_sync(0xffffffffu, here)) {              // one tile in a few per row block: the target's logit, kept out of the sum
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)                  // written as a selection in C++ this becomes an index into r[], which then lives in memory
+                                asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, %2;\n\t@p mov.b32 %0, %3;\n\t}" : "+r"(zt) : "r"(tc & 31), "r"(i), "r"(rc[i]));
+                            if (here) a.z_target[row] = __uint_as_float(zt);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float e0, e1;
+                            fma2(__uint_as_float(rc[i]), __uint_as_float(rc[i + 1]), LOG2E, LOG2E, mc, mc, e0, e1);
+                            rc[i] = __float_as_uint(ex2f(e0)); rc[i + 1] = __float_as_uint(ex2f(e1));
+                        }
+                        if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) if (!here || (tc & 31) != i) et += __uint_as_float(rc[i]);
+                            sum0 += et;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) { sum0 += __uint_as_float(rc[i]); sum1 += __uint_as_float(rc[i + 1]); }
+                        }
+                        if (a.store_u) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                uint32_t pk[4];
+#pragma unroll
+                                for (int v = 0; v < 4; ++v)
+                                    pk[v] = Half2<T>::pack(__uint_as_float(rc[8 * k + 2 * v]) * LceUnit<T>::value, __uint_as_float(rc[8 * k + 2 * v + 1]) * LceUnit<T>::value);
+                                put((c & 1) * 4 + k, make_uint4(pk[0], pk[1], pk[2], pk[3]));
+                            }
+                            if ((c & 1) && n0 + (c - 1) * 32 < a.V && w.m0 + q * 32 < a.rows) store_box(&map_c1, n0 + (c - 1) * 32, w.m0 + q * 32);
+                        }
+                    };
+                    chunk(r[0], 0); chunk(r[1], 1); chunk(r[2], 2); chunk(r[3], 3);
+                    if (row < a.rows) {
+                        const int64_t at = (int64_t)(n0 / 128) * a.rows + row;
+                        a.tile_max[at] = mx;
+                        a.tile_sum[at] = sum0 + sum1;
+                    }
+                }
+            } else {
+                const bool is_x = w.kind == 1, f32 = is_x ? a.f32_x : a.f32_w;
+                const CUtensorMap* map = is_x ? &map_c1 : &map_c2;
+                const int tm = (a.rows + BM - 1) / BM, mrow = w.m0 + q * 32 + (is_x ? w.split * tm * BM : 0);      // partial sums of dx: [split][rows]
+                const float* prev = !is_x && a.dw_prev && row < a.V ? a.dw_prev + (int64_t)row * a.D : nullptr;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    const int col = n0 + c * 32;
+                    if (col >= a.D || w.m0 + q * 32 >= (is_x ? a.rows : a.V)) break;
+                    uint32_t r[32];
+                    if (w.nkb > 0) { tc_ld32(acc + c * 32, r); tc_wait_ld(); }
+                    else
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = 0u;
+                    if (prev) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            if (col + i < a.D) {                          // D is a multiple of 8
+                                const float4 p = *reinterpret_cast<const float4*>(prev + col + i);
+                                r[i] = __float_as_uint(__uint_as_float(r[i]) + p.x); r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) + p.y);
+                                r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) + p.z); r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) + p.w);
+                            }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+                    if (f32) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) put(k, make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]));
+                        store_box(map, col, mrow);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t pk[4];
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) pk[v] = Half2<T>::pack(__uint_as_float(r[8 * k + 2 * v]), __uint_as_float(r[8 * k + 2 * v + 1]));
+                            put((c & 1) * 4 + k, make_uint4(pk[0], pk[1], pk[2], pk[3]));
+                        }
+                        if ((c & 1) || col + 32 >= a.D) store_box(map, col - (c & 1) * 32, mrow);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b->acc_empty[s]);
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// dx = its partial sums (scaled already), added in order: four columns per thread
+template <typename T, bool F32>
+__global__ void __launch_bounds__(256) lce_sum_dx_kernel(const float* __restrict__ part, int splits, int64_t pitch, int64_t n, void* __restrict__ out) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float4 s = *reinterpret_cast<const float4*>(part + i);
+    for (int k = 1; k < splits; ++k) {
+        const float4 p = *reinterpret_cast<const float4*>(part + k * pitch + i);
+        s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+    }
+    if (F32) *reinterpret_cast<float4*>((float*)out + i) = s;
+    else *reinterpret_cast<uint2*>((T*)out + i) = make_uint2(Half2<T>::pack(s.x, s.y), Half2<T>::pack(s.z, s.w));
+}
+
+constexpr size_t SMEM = STAGES * STAGE + 8 * OUT_BYTES + sizeof(LBars) + 1024;
+
+template <typename T, bool GRADS> bool allow() {
+    static std::atomic<uint64_t> done{0};
+    return once_per_device(done, current_device(), [&] {
+        return cudaFuncSetAttribute(lce_sm100_kernel<T, GRADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM) == cudaSuccess;
+    });
+}
+
+template <typename T> int logits(const LceArgs& a, int* err, cudaStream_t st) {
+    CUtensorMap mx, mw, mu;
+    if (!make_map(&mx, a.x, a.rows, a.D, a.ldx, BM, BK, true) || !make_map(&mw, a.w, a.V, a.D, a.ldw, BN, BK, true)) return 10;
+    if (a.u && !make_map(&mu, a.u, a.rows, a.ldu, a.ldu, 32, 64, true)) return 10;
+    if (!allow<T, false>()) return 11;
+    LArgs k{};
+    k.target = a.target; k.ignore_index = a.ignore_index; k.tile_max = a.tile_max; k.tile_sum = a.tile_sum; k.z_target = a.z_target;
+    k.store_u = a.u != nullptr; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err;
+    const unsigned items = (unsigned)((a.rows + BM - 1) / BM) * (unsigned)((a.V + BN - 1) / BN);
+    count_launch();
+    const CUtensorMap& c = a.u ? mu : mx;                                 // without u no map of it is used
+    lce_sm100_kernel<T, false><<<items, THREADS, SMEM, st>>>(mx, mw, c, mx, mw, c, k);
+    return cudaGetLastError() == cudaSuccess ? 0 : 12;
+}
+
+// Pieces that a tile of dx is cut into along the vocabulary: so many that one takes at most half of what each SM does on average.  A tile
+// costs its 64-deep steps and about six more for its epilogue.
+int dx_splits(int rows, int V, int D, bool with_dw) {
+    const int64_t tn = (D + BN - 1) / BN, tx = (rows + BM - 1) / BM * tn, kx = (V + BK - 1) / BK, tw = with_dw ? (V + BM - 1) / BM * tn : 0, kw = (rows + BK - 1) / BK;
+    const int64_t share = (tx * (kx + 6) + tw * (kw + 6)) / device_sms() + 1;
+    int64_t s = (2 * kx + share - 1) / share;
+    if (s > kx / 8) s = kx / 8;                                           // eight steps at least, or the partial sums cost more than the products
+    if (s > 64) s = 64;
+    return s < 1 ? 1 : (int)s;
+}
+
+template <typename T> int grads(const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
+    CUtensorMap ua, wb, cx, um, xb, cw;
+    const int splits = g.dx ? dx_splits(a.rows, a.V, a.D, g.dw != nullptr) : 1;
+    const int tm = (a.rows + BM - 1) / BM, tn = (a.D + BN - 1) / BN;
+    const bool part = splits > 1;
+    if (!make_map(&ua, a.u, a.rows, a.V, a.ldu, BM, BK, true) || !make_map(&um, a.u, a.rows, a.V, a.ldu, BK, 64, true) ||
+        !make_map(&wb, a.w, a.V, a.D, a.ldw, BK, 64, true) || !make_map(&xb, a.x, a.rows, a.D, a.ldx, BK, 64, true)) return 10;
+    const bool x32 = g.f32_out || part;
+    cx = ua; cw = ua;
+    if (g.dx && !make_map(&cx, part ? (void*)scratch : g.dx, part ? (int64_t)splits * tm * BM : a.rows, a.D, a.D, 32, x32 ? 32 : 64, !x32)) return 10;
+    if (g.dw && !make_map(&cw, g.dw, a.V, a.D, a.D, 32, g.f32_out ? 32 : 64, !g.f32_out)) return 10;
+    if (!allow<T, true>()) return 11;
+    LArgs k{};
+    k.dw_prev = g.dw_prev; k.splits = splits; k.f32_x = x32; k.f32_w = g.f32_out; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err;
+    k.gout = g.gout; k.inv = g.inv_count;
+    k.items_x = g.dx ? splits * tm * tn : 0;
+    const unsigned items = (unsigned)k.items_x + (g.dw ? (unsigned)((a.V + BM - 1) / BM) * (unsigned)tn : 0u);
+    count_launch();
+    lce_sm100_kernel<T, true><<<items, THREADS, SMEM, st>>>(ua, wb, cx, um, xb, cw, k);
+    if (part) {
+        const int64_t n = (int64_t)a.rows * a.D;
+        count_launch();
+        const unsigned grid = (unsigned)((n / 4 + 255) / 256);
+        if (g.f32_out) lce_sum_dx_kernel<T, true><<<grid, 256, 0, st>>>(scratch, splits, (int64_t)tm * BM * a.D, n, g.dx);
+        else lce_sum_dx_kernel<T, false><<<grid, 256, 0, st>>>(scratch, splits, (int64_t)tm * BM * a.D, n, g.dx);
+    }
+    return cudaGetLastError() == cudaSuccess ? 0 : 12;
+}
+
+}  // namespace
+
+bool lce_sm100_takes(int dtype, const LceArgs& a) {
+    const auto ok = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld > 0 && ld % 8 == 0; };
+    return dtype != F32 && a.D % 8 == 0 && ok(a.x, a.ldx) && ok(a.w, a.ldw);
+}
+int64_t lce_sm100_scratch(int rows, int V, int D, bool with_dw) {
+    const int s = dx_splits(rows, V, D, with_dw);
+    return s > 1 ? (int64_t)s * ((rows + BM - 1) / BM * BM) * D : 0;
+}
+int lce_sm100_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st) { return dtype == BF16 ? logits<__nv_bfloat16>(a, err, st) : logits<__half>(a, err, st); }
+int lce_sm100_grads(int dtype, const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
+    return dtype == BF16 ? grads<__nv_bfloat16>(a, g, scratch, err, st) : grads<__half>(a, g, scratch, err, st);
+}
+
+}  // namespace sg
