@@ -7,9 +7,14 @@
 //            ones start first and are cut along the sum when one alone would take longer than everything spread over the SMs.  d, w and x are
 //            read where they are, in whichever order their rows run (K-major or MN-major descriptors).
 //
-// One CTA per SM: eight warps read accumulators (two per 32 rows, 128 columns each), one loads, one issues.  The accumulator is
-// double-buffered in tensor memory, so an epilogue runs under the next tile's products; a running CTA takes over the tiles of CTAs that
-// have not started (cluster launch control), so long and short tiles balance without a counter in memory.
+// Two SMs work on a tile of 256 rows x 256 columns (cta_group::2): each loads its 128 rows of A and half of B's 256, one thread of the
+// first issues the products of both, and each holds its own rows' accumulators.  A step of 64 then costs an SM 32 KB from L2 and 512
+// clocks of products; a CTA alone (128 x 256) needs 48 KB for the same time, more than L2 gives every SM at once.  Eight warps of each CTA
+// read accumulators (two per 32 rows, 128 columns each), one loads.  The accumulator is double-buffered in tensor memory, so an epilogue
+// runs under the next tile's products; a running pair takes over the tiles of pairs that have not started (cluster launch control), so
+// long and short tiles balance without a counter in memory.  Up to 128 rows a CTA works alone (PAIR = false, 128 x 256): the pair's second
+// half of A would be empty, and what counts is how fast w streams in (13 rows x 32,000 x 2,048, both products 83 us in pairs, 59 alone).
+// 4,096 rows, logits and both products: 387 and 734 us in pairs, 367 and 837 alone.
 #include "sg_native.h"
 #include "tc_half.cuh"
 #include "per_device.h"
@@ -20,15 +25,21 @@ namespace sg {
 namespace {
 using namespace tc;
 
-constexpr int BM = 128, BN = 256, BK = 64, STAGES = 4, THREADS = 320;
-constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES, OUT_BYTES = 32 * 128;
-constexpr int GROUP_M = 32;                                               // tile rows that sweep over the columns together
-
-struct LItem {
-    int m0, n0, kb0, nkb, kind, split;                                    // kind: 0 end of the work, 1 logits or dx, 2 dw
+constexpr int BN = 256, BK = 64, THREADS = 352;
+constexpr uint32_t A_BYTES = 128 * BK * 2, OUT_BYTES = 32 * 128;
+// a tile (of the pair, or of a CTA alone) and what one CTA holds of its operands
+template <bool PAIR> struct Shape {
+    static constexpr int CTAS = PAIR ? 2 : 1, BM = 128 * CTAS, B_ROWS = BN / CTAS, STAGES = PAIR ? 6 : 4;
+    static constexpr uint32_t B_BYTES = B_ROWS * BK * 2, STAGE = A_BYTES + B_BYTES;
 };
+constexpr int GROUP_M = 16;                                               // tile rows that sweep over the columns together
+
+struct alignas(16) LItem {
+    int m0, n0, kb0, nkb, kind, split, unused[2];                         // kind: 0 end of the work, 1 logits or dx, 2 dw
+};
+// full, acc_empty, item_empty and clc are used in the first CTA of the pair
 struct LBars {
-    uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], item_full[2], item_empty[2], clc;
+    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], item_full[2], item_empty[2], clc;
     uint4 answer;
     LItem item[2];
     uint32_t tmem_slot;
@@ -56,110 +67,196 @@ __device__ __forceinline__ void logits_tile(int i, int tm, int tn, int& m, int& 
     n = r / g;
 }
 
-template <typename T, bool GRADS>
+__device__ __forceinline__ uint32_t cta_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+// the address of a shared variable of CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+// Arrivals at barriers of the other CTA carry no data through generic memory (operands and accumulators are ordered by the asynchronous
+// units' own completions), so they are plain arrivals: cluster-scope releases and acquires cost each waiting warp a fence.
+__device__ __forceinline__ void cluster_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void cluster_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// 16 bytes into a CTA's shared memory, counted by a barrier there
+__device__ __forceinline__ void cluster_store(uint32_t addr, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a load whose arrival is counted by a barrier of the (pair's first) CTA
+template <bool PAIR> __device__ __forceinline__ void tile_load(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+template <bool PAIR> __device__ __forceinline__ void tile_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+    else tc_mma_bf16(d, da, db, idesc, accumulate);
+}
+// arrives at the barrier (of both CTAs) when the products issued so far are done
+template <bool PAIR> __device__ __forceinline__ void tile_commit(uint64_t* bar) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+    else tc_commit(bar);
+}
+
+template <typename T, bool GRADS, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_b1,
                                                                const __grid_constant__ CUtensorMap map_c1, const __grid_constant__ CUtensorMap map_a2,
                                                                const __grid_constant__ CUtensorMap map_b2, const __grid_constant__ CUtensorMap map_c2,
                                                                const __grid_constant__ LArgs a) {
+    using S = Shape<PAIR>;
+    constexpr int BM = S::BM, STAGES = S::STAGES;
+    constexpr uint32_t STAGE = S::STAGE;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
+    // the same offset in both CTAs: the dynamic part starts at the same address in every CTA of a kernel
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* s_out = smem + STAGES * STAGE;                               // [8 warps][OUT_BYTES]
     LBars* b = reinterpret_cast<LBars*>(s_out + 8 * OUT_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cta_rank() : 0u;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&b->full[s], 1); mbar_init(&b->empty[s], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&b->acc_full[i], 1); mbar_init(&b->acc_empty[i], 8); mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 9); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&b->acc_full[i], 1); mbar_init(&b->acc_empty[i], 8 * S::CTAS);
+            mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 9 * S::CTAS + 1);     // per CTA a loading and eight reading warps, and the issuing one
+        }
         mbar_init(&b->clc, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&b->tmem_slot)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&b->tmem_slot)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&b->tmem_slot)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = b->tmem_slot;
+    // the item that every warp of both CTAs works on next
+    auto take = [&](uint32_t n, LItem& w) {
+        const uint32_t s = n & 1;
+        if (!mbar_wait(&b->item_full[s], (n >> 1) & 1)) return false;
+        w = b->item[s];
+        return true;
+    };
+    auto arrive_first = [&](uint64_t* bar) { if (rank == 0) mbar_arrive(bar); else cluster_arrive(in_cta(bar, 0)); };
+    auto release = [&](uint32_t n) { arrive_first(&b->item_empty[n & 1]); };
 
-    if (warp == 8) {
-        int i = (int)blockIdx.x;
-        uint32_t n_item = 0, n_clc = 0, it = 0;
-        bool ok = true, more = true;
-        while (ok && more) {
-            if (lane == 0) {
-                mbar_expect_tx(&b->clc, 16);
-                clc_ask(&b->answer, &b->clc);
-            }
-            LItem w{0, 0, 0, 0, 1, 0};
-            if constexpr (!GRADS) {
-                int m, n;
-                logits_tile(i, (a.rows + BM - 1) / BM, (a.V + BN - 1) / BN, m, n);
-                w.m0 = m * BM; w.n0 = n * BN; w.nkb = (a.D + BK - 1) / BK;
-            } else {
-                const int tn = (a.D + BN - 1) / BN;
-                if (i < a.items_x) {
-                    const int tm = (a.rows + BM - 1) / BM, kb = (a.V + BK - 1) / BK, per = (kb + a.splits - 1) / a.splits;
-                    w.split = i / (tm * tn);
-                    const int r = i % (tm * tn);
-                    w.m0 = r % tm * BM; w.n0 = r / tm * BN;
-                    w.kb0 = w.split * per;
-                    w.nkb = kb - w.kb0 < per ? kb - w.kb0 : per;          // 0 or less: a split past the end, all zeros
-                    if (w.nkb < 0) w.nkb = 0;
-                } else {
-                    const int r = i - a.items_x;
-                    w.kind = 2;
-                    w.m0 = r / tn * BM; w.n0 = r % tn * BN; w.nkb = (a.rows + BK - 1) / BK;
+    if (warp == 10) {
+        // the scheduler, one thread of the first CTA: writes the items of both
+        if (rank == 0 && lane == 0) {
+            int i = (int)blockIdx.x / S::CTAS;
+            uint32_t n_item = 0, n_clc = 0;
+            bool more = true;
+            while (true) {
+                LItem w{};
+                if (more) {
+                    mbar_expect_tx(&b->clc, 16);
+                    clc_ask(&b->answer, &b->clc);
+                    w.kind = 1;
+                    if constexpr (!GRADS) {
+                        int m, n;
+                        logits_tile(i, (a.rows + BM - 1) / BM, (a.V + BN - 1) / BN, m, n);
+                        w.m0 = m * BM; w.n0 = n * BN; w.nkb = (a.D + BK - 1) / BK;
+                    } else {
+                        const int tn = (a.D + BN - 1) / BN;
+                        if (i < a.items_x) {
+                            const int tm = (a.rows + BM - 1) / BM, kb = (a.V + BK - 1) / BK, per = (kb + a.splits - 1) / a.splits;
+                            w.split = i / (tm * tn);
+                            const int r = i % (tm * tn);
+                            w.m0 = r % tm * BM; w.n0 = r / tm * BN;
+                            w.kb0 = w.split * per;
+                            w.nkb = kb - w.kb0 < per ? kb - w.kb0 : per;
+                            if (w.nkb < 0) w.nkb = 0;                     // a split past the end: all zeros
+                        } else {
+                            const int r = i - a.items_x;
+                            w.kind = 2;
+                            w.m0 = r / tn * BM; w.n0 = r % tn * BN; w.nkb = (a.rows + BK - 1) / BK;
+                        }
+                    }
                 }
+                const uint32_t s = n_item & 1;
+                if (n_item >= 2 && !mbar_wait(&b->item_empty[s], ((n_item >> 1) & 1) ^ 1)) { atomicExch(a.err, 101); break; }
+                ++n_item;
+                if constexpr (PAIR) {
+                    for (uint32_t r = 0; r < 2; ++r) {
+                        const uint32_t bar = in_cta(&b->item_full[s], r), to = in_cta(&b->item[s], r);
+                        cluster_expect(bar, 32);
+                        cluster_store(to, w.m0, w.n0, w.kb0, w.nkb, bar);
+                        cluster_store(to + 16, w.kind, w.split, 0, 0, bar);
+                    }
+                } else {
+                    b->item[s] = w;
+                    mbar_arrive(&b->item_full[s]);
+                }
+                if (!more) break;
+                if (!mbar_wait(&b->clc, n_clc & 1)) { atomicExch(a.err, 103); break; }
+                ++n_clc;
+                more = clc_answer(&b->answer, i);
+                i /= S::CTAS;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
-            const uint32_t s = n_item & 1;
-            if (n_item >= 2) ok = warp_wait(&b->item_empty[s], ((n_item >> 1) & 1) ^ 1);
-            if (!ok) { if (lane == 0) atomicExch(a.err, 101); break; }
-            ++n_item;
-            if (lane == 0) {
-                b->item[s] = w;
-                mbar_arrive(&b->item_full[s]);
+        }
+    } else if (warp == 8) {
+        if (lane == 0) {
+            uint32_t n_item = 0, it = 0;
+            bool ok = true;
+            while (ok) {
+                LItem w;
+                if (!take(n_item, w)) { atomicExch(a.err, 100); break; }
+                release(n_item++);
+                if (w.kind == 0) break;
+                const int m0 = w.m0 + 128 * (int)rank, n0 = w.n0 + S::B_ROWS * (int)rank;       // this CTA's rows of A, of B
                 for (int k = 0; k < w.nkb; ++k, ++it) {                   // what lies past the end of an operand is filled with zeros
                     const uint32_t st = it % STAGES;
                     if (it >= STAGES && !mbar_wait(&b->empty[st], ((it / STAGES) & 1) ^ 1)) { atomicExch(a.err, 102); ok = false; break; }
                     uint8_t* dst = smem + st * STAGE;
                     const int kc = (w.kb0 + k) * BK;
-                    mbar_expect_tx(&b->full[st], STAGE);
+                    const uint32_t bar = in_cta(&b->full[st], 0);
+                    if (rank == 0) mbar_expect_tx(&b->full[st], S::CTAS * STAGE);       // what both CTAs load
                     if constexpr (!GRADS) {
-                        tma_load_2d(dst, &map_a1, kc, w.m0, &b->full[st]);
-                        tma_load_2d(dst + A_BYTES, &map_b1, kc, w.n0, &b->full[st]);
+                        tile_load<PAIR>(dst, &map_a1, kc, m0, bar);
+                        tile_load<PAIR>(dst + A_BYTES, &map_b1, kc, n0, bar);
                     } else {
-                        if (w.kind == 1) tma_load_2d(dst, &map_a1, kc, w.m0, &b->full[st]);
-                        else
+                        if (w.kind == 1) tile_load<PAIR>(dst, &map_a1, kc, m0, bar);
+                        else {
+                            tile_load<PAIR>(dst, &map_a2, m0, kc, bar);
+                            tile_load<PAIR>(dst + BK * 128, &map_a2, m0 + 64, kc, bar);
+                        }
 #pragma unroll
-                            for (int c = 0; c < BM / 64; ++c) tma_load_2d(dst + c * (BK * 128), &map_a2, w.m0 + 64 * c, kc, &b->full[st]);
-#pragma unroll
-                        for (int c = 0; c < BN / 64; ++c) tma_load_2d(dst + A_BYTES + c * (BK * 128), w.kind == 1 ? &map_b1 : &map_b2, w.n0 + 64 * c, kc, &b->full[st]);
+                        for (int c = 0; c < S::B_ROWS / 64; ++c) tile_load<PAIR>(dst + A_BYTES + c * (BK * 128), w.kind == 1 ? &map_b1 : &map_b2, n0 + 64 * c, kc, bar);
                     }
                 }
             }
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (!warp_wait(&b->clc, n_clc & 1)) { if (lane == 0) atomicExch(a.err, 103); ok = false; break; }
-            ++n_clc;
-            more = clc_answer(&b->answer, i);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-        }
-        if (ok && (n_item < 2 || warp_wait(&b->item_empty[n_item & 1], ((n_item >> 1) & 1) ^ 1)) && lane == 0) {
-            b->item[n_item & 1].kind = 0;
-            mbar_arrive(&b->item_full[n_item & 1]);
         }
     } else if (warp == 9) {
-        if (lane == 0) {
+        if (rank == 0 && lane == 0) {
             uint32_t n_item = 0, it = 0;
             bool ok = true;
             while (ok) {
-                const uint32_t s = n_item & 1;
-                if (!mbar_wait(&b->item_full[s], (n_item >> 1) & 1)) { atomicExch(a.err, 104); break; }
-                const LItem w = b->item[s];
-                mbar_arrive(&b->item_empty[s]);
+                LItem w;
+                if (!take(n_item, w)) { atomicExch(a.err, 104); break; }
+                release(n_item);
                 if (w.kind == 0) break;
+                const uint32_t s = n_item & 1;
                 if (n_item >= 2 && !mbar_wait(&b->acc_empty[s], ((n_item >> 1) & 1) ^ 1)) { atomicExch(a.err, 105); break; }
                 ++n_item;
                 tc_fence_after();
@@ -174,13 +271,13 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                     const uint64_t db = b_mn ? make_desc_sw128_mn(pa + A_BYTES, BK * 128, 1024) : make_desc_sw128(pa + A_BYTES);
 #pragma unroll
                     for (int k4 = 0; k4 < BK / 16; ++k4)
-                        tc_mma_bf16(d, da + (a_mn ? 128 : 2) * k4, db + (b_mn ? 128 : 2) * k4, idesc, (k > 0 || k4 > 0) ? 1u : 0u);
-                    tc_commit(&b->empty[st]);
+                        tile_mma<PAIR>(d, da + (a_mn ? 128 : 2) * k4, db + (b_mn ? 128 : 2) * k4, idesc, (k > 0 || k4 > 0) ? 1u : 0u);
+                    tile_commit<PAIR>(&b->empty[st]);
                 }
-                tc_commit(&b->acc_full[s]);
+                tile_commit<PAIR>(&b->acc_full[s]);
             }
         }
-    } else {
+    } else if (warp < 8) {
         const int q = warp & 3, half = warp >> 2;
         const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
         uint8_t* stg = s_out + warp * OUT_BYTES;
@@ -200,14 +297,15 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
         auto put = [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(stg + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v; };
         while (true) {
             const uint32_t s = n_item & 1;
-            if (!warp_wait(&b->item_full[s], (n_item >> 1) & 1)) { atomicExch(a.err, 107); break; }
-            const LItem w = b->item[s];
+            LItem w;
+            if (!__all_sync(0xffffffffu, take(n_item, w))) { atomicExch(a.err, 107); break; }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b->item_empty[s]);
+            if (lane == 0) release(n_item);
             if (w.kind == 0) break;
-            if (!warp_wait(&b->acc_full[s], (n_item >> 1) & 1)) { atomicExch(a.err, 108); break; }
+            if (!__all_sync(0xffffffffu, mbar_wait(&b->acc_full[s], (n_item >> 1) & 1))) { atomicExch(a.err, 108); break; }
             ++n_item;
             tc_fence_after();
+            w.m0 += 128 * (int)rank;                                      // this CTA's rows
             const uint32_t acc = tmem + s * BN + half * 128 + lane_addr;
             const int row = w.m0 + q * 32 + lane, n0 = w.n0 + half * 128;
             if constexpr (!GRADS) {
@@ -217,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                 tc_wait_ld();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&b->acc_empty[s]);             // everything is in registers
+                if (lane == 0) arrive_first(&b->acc_empty[s]);             // everything is in registers
                 if (n0 < a.V) {
                     const int64_t t = row < a.rows ? a.target[row] : -1;
                     const int tc = t >= n0 && t < n0 + 128 && t < a.V ? (int)(t - n0) : -1;        // the target's column, if it is here
@@ -319,16 +417,19 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&b->acc_empty[s]);
+                if (lane == 0) arrive_first(&b->acc_empty[s]);
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
+    __syncwarp();
+    if (PAIR) cluster_sync();                                             // neither CTA leaves while the other may still signal it
     if (warp == 9) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 
@@ -346,67 +447,74 @@ __global__ void __launch_bounds__(256) lce_sum_dx_kernel(const float* __restrict
     else *reinterpret_cast<uint2*>((T*)out + i) = make_uint2(Half2<T>::pack(s.x, s.y), Half2<T>::pack(s.z, s.w));
 }
 
-constexpr size_t SMEM = STAGES * STAGE + 8 * OUT_BYTES + sizeof(LBars) + 1024;
-
-template <typename T, bool GRADS> bool allow() {
+template <typename T, bool GRADS, bool PAIR>
+int launch(unsigned items, const CUtensorMap& a1, const CUtensorMap& b1, const CUtensorMap& c1, const CUtensorMap& a2, const CUtensorMap& b2, const CUtensorMap& c2,
+           const LArgs& k, cudaStream_t st) {
+    using S = Shape<PAIR>;
+    constexpr size_t smem = S::STAGES * S::STAGE + 8 * OUT_BYTES + sizeof(LBars) + 1024;
     static std::atomic<uint64_t> done{0};
-    return once_per_device(done, current_device(), [&] {
-        return cudaFuncSetAttribute(lce_sm100_kernel<T, GRADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM) == cudaSuccess;
-    });
+    if (!once_per_device(done, current_device(), [&] {
+            return cudaFuncSetAttribute(lce_sm100_kernel<T, GRADS, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess;
+        })) return 11;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = S::CTAS; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(items * S::CTAS); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = &at; cfg.numAttrs = 1;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, lce_sm100_kernel<T, GRADS, PAIR>, a1, b1, c1, a2, b2, c2, k) == cudaSuccess ? 0 : 12;
 }
 
-template <typename T> int logits(const LceArgs& a, int* err, cudaStream_t st) {
+template <typename T, bool PAIR> int logits(const LceArgs& a, int* err, cudaStream_t st) {
+    using S = Shape<PAIR>;
     CUtensorMap mx, mw, mu;
-    if (!make_map(&mx, a.x, a.rows, a.D, a.ldx, BM, BK, true) || !make_map(&mw, a.w, a.V, a.D, a.ldw, BN, BK, true)) return 10;
+    if (!make_map(&mx, a.x, a.rows, a.D, a.ldx, 128, BK, true) || !make_map(&mw, a.w, a.V, a.D, a.ldw, S::B_ROWS, BK, true)) return 10;
     if (a.u && !make_map(&mu, a.u, a.rows, a.ldu, a.ldu, 32, 64, true)) return 10;
-    if (!allow<T, false>()) return 11;
     LArgs k{};
     k.target = a.target; k.ignore_index = a.ignore_index; k.tile_max = a.tile_max; k.tile_sum = a.tile_sum; k.z_target = a.z_target;
     k.store_u = a.u != nullptr; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err;
-    const unsigned items = (unsigned)((a.rows + BM - 1) / BM) * (unsigned)((a.V + BN - 1) / BN);
-    count_launch();
     const CUtensorMap& c = a.u ? mu : mx;                                 // without u no map of it is used
-    lce_sm100_kernel<T, false><<<items, THREADS, SMEM, st>>>(mx, mw, c, mx, mw, c, k);
-    return cudaGetLastError() == cudaSuccess ? 0 : 12;
+    return launch<T, false, PAIR>((unsigned)((a.rows + S::BM - 1) / S::BM) * (unsigned)((a.V + BN - 1) / BN), mx, mw, c, mx, mw, c, k, st);
 }
 
-// Pieces that a tile of dx is cut into along the vocabulary: so many that one takes at most half of what each SM does on average.  A tile
-// costs its 64-deep steps and about six more for its epilogue.
+bool in_pairs(int rows) { return rows > 128; }
+
+// Pieces that a tile of dx is cut into along the vocabulary: so many that one takes at most half of what a CTA (or pair) does on average.
+// A tile costs its 64-deep steps and about six more for its epilogue.
 int dx_splits(int rows, int V, int D, bool with_dw) {
-    const int64_t tn = (D + BN - 1) / BN, tx = (rows + BM - 1) / BM * tn, kx = (V + BK - 1) / BK, tw = with_dw ? (V + BM - 1) / BM * tn : 0, kw = (rows + BK - 1) / BK;
-    const int64_t share = (tx * (kx + 6) + tw * (kw + 6)) / device_sms() + 1;
+    const int64_t bm = in_pairs(rows) ? 256 : 128, teams = device_sms() / (bm / 128);
+    const int64_t tn = (D + BN - 1) / BN, tx = (rows + bm - 1) / bm * tn, kx = (V + BK - 1) / BK, tw = with_dw ? (V + bm - 1) / bm * tn : 0, kw = (rows + BK - 1) / BK;
+    const int64_t share = (tx * (kx + 6) + tw * (kw + 6)) / (teams > 0 ? teams : 1) + 1;
     int64_t s = (2 * kx + share - 1) / share;
     if (s > kx / 8) s = kx / 8;                                           // eight steps at least, or the partial sums cost more than the products
     if (s > 64) s = 64;
     return s < 1 ? 1 : (int)s;
 }
 
-template <typename T> int grads(const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
+template <typename T, bool PAIR> int grads(const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
+    using S = Shape<PAIR>;
     CUtensorMap ua, wb, cx, um, xb, cw;
     const int splits = g.dx ? dx_splits(a.rows, a.V, a.D, g.dw != nullptr) : 1;
-    const int tm = (a.rows + BM - 1) / BM, tn = (a.D + BN - 1) / BN;
+    const int tm = (a.rows + S::BM - 1) / S::BM, tn = (a.D + BN - 1) / BN;
     const bool part = splits > 1;
-    if (!make_map(&ua, a.u, a.rows, a.V, a.ldu, BM, BK, true) || !make_map(&um, a.u, a.rows, a.V, a.ldu, BK, 64, true) ||
+    if (!make_map(&ua, a.u, a.rows, a.V, a.ldu, 128, BK, true) || !make_map(&um, a.u, a.rows, a.V, a.ldu, BK, 64, true) ||
         !make_map(&wb, a.w, a.V, a.D, a.ldw, BK, 64, true) || !make_map(&xb, a.x, a.rows, a.D, a.ldx, BK, 64, true)) return 10;
     const bool x32 = g.f32_out || part;
     cx = ua; cw = ua;
-    if (g.dx && !make_map(&cx, part ? (void*)scratch : g.dx, part ? (int64_t)splits * tm * BM : a.rows, a.D, a.D, 32, x32 ? 32 : 64, !x32)) return 10;
+    if (g.dx && !make_map(&cx, part ? (void*)scratch : g.dx, part ? (int64_t)splits * tm * S::BM : a.rows, a.D, a.D, 32, x32 ? 32 : 64, !x32)) return 10;
     if (g.dw && !make_map(&cw, g.dw, a.V, a.D, a.D, 32, g.f32_out ? 32 : 64, !g.f32_out)) return 10;
-    if (!allow<T, true>()) return 11;
     LArgs k{};
     k.dw_prev = g.dw_prev; k.splits = splits; k.f32_x = x32; k.f32_w = g.f32_out; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err;
     k.gout = g.gout; k.inv = g.inv_count;
     k.items_x = g.dx ? splits * tm * tn : 0;
-    const unsigned items = (unsigned)k.items_x + (g.dw ? (unsigned)((a.V + BM - 1) / BM) * (unsigned)tn : 0u);
+    const unsigned items = (unsigned)k.items_x + (g.dw ? (unsigned)((a.V + S::BM - 1) / S::BM) * (unsigned)tn : 0u);
+    const int rc = launch<T, true, PAIR>(items, ua, wb, cx, um, xb, cw, k, st);
+    if (rc != 0 || !part) return rc;
+    const int64_t n = (int64_t)a.rows * a.D, pitch = (int64_t)tm * S::BM * a.D;
+    const unsigned grid = (unsigned)((n / 4 + 255) / 256);
     count_launch();
-    lce_sm100_kernel<T, true><<<items, THREADS, SMEM, st>>>(ua, wb, cx, um, xb, cw, k);
-    if (part) {
-        const int64_t n = (int64_t)a.rows * a.D;
-        count_launch();
-        const unsigned grid = (unsigned)((n / 4 + 255) / 256);
-        if (g.f32_out) lce_sum_dx_kernel<T, true><<<grid, 256, 0, st>>>(scratch, splits, (int64_t)tm * BM * a.D, n, g.dx);
-        else lce_sum_dx_kernel<T, false><<<grid, 256, 0, st>>>(scratch, splits, (int64_t)tm * BM * a.D, n, g.dx);
-    }
+    if (g.f32_out) lce_sum_dx_kernel<T, true><<<grid, 256, 0, st>>>(scratch, splits, pitch, n, g.dx);
+    else lce_sum_dx_kernel<T, false><<<grid, 256, 0, st>>>(scratch, splits, pitch, n, g.dx);
     return cudaGetLastError() == cudaSuccess ? 0 : 12;
 }
 
@@ -417,12 +525,16 @@ bool lce_sm100_takes(int dtype, const LceArgs& a) {
     return dtype != F32 && a.D % 8 == 0 && ok(a.x, a.ldx) && ok(a.w, a.ldw);
 }
 int64_t lce_sm100_scratch(int rows, int V, int D, bool with_dw) {
-    const int s = dx_splits(rows, V, D, with_dw);
-    return s > 1 ? (int64_t)s * ((rows + BM - 1) / BM * BM) * D : 0;
+    const int s = dx_splits(rows, V, D, with_dw), bm = in_pairs(rows) ? 256 : 128;
+    return s > 1 ? (int64_t)s * ((rows + bm - 1) / bm * bm) * D : 0;
 }
-int lce_sm100_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st) { return dtype == BF16 ? logits<__nv_bfloat16>(a, err, st) : logits<__half>(a, err, st); }
+int lce_sm100_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st) {
+    if (in_pairs(a.rows)) return dtype == BF16 ? logits<__nv_bfloat16, true>(a, err, st) : logits<__half, true>(a, err, st);
+    return dtype == BF16 ? logits<__nv_bfloat16, false>(a, err, st) : logits<__half, false>(a, err, st);
+}
 int lce_sm100_grads(int dtype, const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
-    return dtype == BF16 ? grads<__nv_bfloat16>(a, g, scratch, err, st) : grads<__half>(a, g, scratch, err, st);
+    if (in_pairs(a.rows)) return dtype == BF16 ? grads<__nv_bfloat16, true>(a, g, scratch, err, st) : grads<__half, true>(a, g, scratch, err, st);
+    return dtype == BF16 ? grads<__nv_bfloat16, false>(a, g, scratch, err, st) : grads<__half, false>(a, g, scratch, err, st);
 }
 
 }  // namespace sg
