@@ -134,33 +134,27 @@ Tensor loadable_rows(const Tensor& t) {
 struct LceShape {
     sg::LceArgs a{};
     int dtype = 0;
-    int64_t rows = 0, piece = 0, elem = 0;
-    // the piece of rows [r0, r0 + n)
+    int64_t rows = 0, piece = 0, elem = 0, ldx = 0;
+    // the piece of the counted rows from r0 on (sized as if all rows were counted)
     sg::LceArgs at(int64_t r0) const {
         sg::LceArgs p = a;
+        p.first = (int)r0;
         p.rows = (int)(rows - r0 < piece ? rows - r0 : piece);
-        p.x = (const char*)a.x + r0 * a.ldx * elem;
-        p.target = a.target + r0;
+        p.x = (const char*)a.x + r0 * a.D * elem;
+        p.target = a.target ? a.target + r0 : nullptr;
         p.loss = a.loss ? a.loss + r0 : nullptr;
         return p;
     }
     int64_t last() const { return rows == 0 ? 0 : (rows - 1) / piece * piece; }      // first row of the last piece
 };
 
-LceShape lce_shape(const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool train) {
-    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2 && t.dim() == 1 && x.size(1) == w.size(1) && t.size(0) == x.size(0),
-                "linear_cross_entropy: x [rows, D], weight [vocabulary, D], target [rows]");
-    TORCH_CHECK(w.device() == x.device() && t.device() == x.device(), "linear_cross_entropy: all tensors on one device");
-    TORCH_CHECK(w.scalar_type() == x.scalar_type() && t.scalar_type() == at::kLong && t.is_contiguous(), "linear_cross_entropy: x and weight of one dtype, int64 targets");
-    TORCH_CHECK(w.size(0) >= 1 && w.size(0) < (1 << 22) && x.size(1) >= 1 && x.size(1) < (1 << 22) && x.size(0) < ((int64_t)1 << 31),
-                "linear_cross_entropy: vocabulary and width below 2^22");
-    TORCH_CHECK((x.stride(1) == 1 || x.size(1) == 1) && (w.stride(1) == 1 || w.size(1) == 1), "linear_cross_entropy: the last index must be contiguous");
+LceShape lce_shape(const Tensor& x, const Tensor& w, bool train) {
     LceShape s;
     s.dtype = dtype_code(x);
     s.elem = x.element_size();
     s.rows = x.size(0);
-    s.a.x = x.data_ptr(); s.a.w = w.data_ptr(); s.a.ldx = x.stride(0); s.a.ldw = w.stride(0);
-    s.a.target = t.data_ptr<int64_t>(); s.a.ignore_index = ignore_index;
+    s.ldx = x.stride(0);
+    s.a.w = w.data_ptr(); s.a.ldw = w.stride(0);
     s.a.V = (int)w.size(0); s.a.D = (int)w.size(1);
     const int64_t per = 16 / s.elem;
     s.a.ldu = (w.size(0) + per - 1) / per * per;
@@ -168,97 +162,134 @@ LceShape lce_shape(const Tensor& x, const Tensor& w, const Tensor& t, int64_t ig
     return s;
 }
 
-// Returns (loss, {mean, 1 / count}, d of the last piece [rows, pitch], and with several pieces: fp32 dx of the others, fp32 dw of the others).
-// The gradient products of the last piece are left to the backward pass, which writes them in the final type; of the pieces before it the
-// products are taken here, because their d makes room for the next one's.
-std::vector<Tensor> lce_fwd(const Tensor& x_, const Tensor& w_, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
-    const Tensor x = loadable_rows(x_), w = loadable_rows(w_);
+// What a training pass keeps from forward to backward: the counted rows xc, where they came from (keep: [rows] places, then the count, the
+// counter of the row pass and 1 / count as a float), d of the last piece, and with several pieces fp32 dx and dw of the others.
+enum { KEEP_COUNT = 0, KEEP_DONE = 1, KEEP_INV = 2, KEEP_MORE = 4 };
+
+// Returns (loss, xc, keep, d, dx of earlier pieces, dw of earlier pieces).  The gradient products of the last piece are left to the backward
+// pass, which writes them in the final type; of the pieces before it the products are taken here, because their d makes room for the next one's.
+std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w_, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w_.dim() == 2 && t.dim() == 1 && x.size(1) == w_.size(1) && t.size(0) == x.size(0),
+                "linear_cross_entropy: x [rows, D], weight [vocabulary, D], target [rows]");
+    TORCH_CHECK(w_.device() == x.device() && t.device() == x.device(), "linear_cross_entropy: all tensors on one device");
+    TORCH_CHECK(w_.scalar_type() == x.scalar_type() && t.scalar_type() == at::kLong && t.is_contiguous(), "linear_cross_entropy: x and weight of one dtype, int64 targets");
+    TORCH_CHECK(w_.size(0) >= 1 && w_.size(0) < (1 << 22) && x.size(1) >= 1 && x.size(1) < (1 << 22) && x.size(0) < ((int64_t)1 << 30),
+                "linear_cross_entropy: vocabulary and width below 2^22, fewer than 2^30 rows");
+    TORCH_CHECK((x.stride(1) == 1 || x.size(1) == 1) && (w_.stride(1) == 1 || w_.size(1) == 1), "linear_cross_entropy: the last index must be contiguous");
     const bool train = need_x || need_w;
-    LceShape s = lce_shape(x, w, t, ignore_index, train);
     c10::cuda::CUDAGuard guard(x.device());
+    const Tensor w = loadable_rows(w_);
+    LceShape s = lce_shape(x, w, train);
     auto st = at::cuda::getCurrentCUDAStream();
     const auto fo = x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
     const auto xo = x.options().memory_format(at::MemoryFormat::Contiguous);
-    Tensor loss = at::empty({s.rows}, fo), mean = s.rows > 0 ? at::empty({2}, fo) : at::zeros({2}, fo);
-    Tensor u = at::empty({train ? s.piece : 0, s.a.ldu}, xo), dx, dw;
-    if (s.rows > 0) {
-        s.a.loss = loss.data_ptr<float>();
-        const int cols = sg::lce_tile_columns(s.dtype, s.at(0));
-        Tensor stats = at::empty({2, (s.a.V + cols - 1) / cols, s.piece}, fo), zt = at::empty({s.piece}, fo);
-        s.a.tile_max = stats.data_ptr<float>();
-        s.a.tile_sum = s.a.tile_max + stats.numel() / 2;
-        s.a.z_target = zt.data_ptr<float>();
-        s.a.u = train ? u.data_ptr() : nullptr;
-        const int64_t last = s.last();
-        if (train && last > 0 && need_x) dx = at::empty({last, x.size(1)}, fo);
-        if (train && last > 0 && need_w) dw = at::empty(w.sizes(), fo);
-        for (int64_t r0 = 0; r0 < s.rows; r0 += s.piece) {
-            const sg::LceArgs a = s.at(r0);
-            int rc = sg::lce_logits(s.dtype, a, err.data_ptr<int>(), st);
-            if (rc == 0) rc = sg::lce_rows(s.dtype, a, st);
-            if (rc == 0 && train && r0 < last) {
-                sg::LceGrads g{};
-                g.dx = need_x ? dx.data_ptr<float>() + r0 * x.size(1) : nullptr;
-                g.dw = need_w ? dw.data_ptr() : nullptr;
-                g.dw_prev = need_w && r0 > 0 ? dw.data_ptr<float>() : nullptr;
-                g.f32_out = true;
-                Tensor scratch = at::empty({sg::lce_scratch(s.dtype, a, need_x, need_w)}, fo);
-                rc = sg::lce_grads(s.dtype, a, g, scratch.data_ptr<float>(), err.data_ptr<int>(), st);
-            }
-            TORCH_CHECK(rc == 0, "linear_cross_entropy: launch failed (code ", rc, ")");
-        }
-        sg::ce_mean(s.a.loss, s.a.target, s.rows, s.a.V, ignore_index, mean.data_ptr<float>(), st);
-    }
     const Tensor none = at::empty({0}, fo);
-    return {mean.narrow(0, 0, 1).reshape({}), mean, u, dx.defined() ? dx : none, dw.defined() ? dw : none};
+    if (s.rows == 0) return {at::zeros({}, fo), none, none, none, none, none};
+    Tensor loss = at::empty({}, fo), xc = at::empty({s.rows, x.size(1)}, xo), keep = at::empty({s.rows + KEEP_MORE}, fo.dtype(at::kInt));
+    Tensor u = train ? at::empty({s.piece, s.a.ldu}, xo) : none, dx = none, dw = none;
+    s.a.x = xc.data_ptr();
+    const int64_t tiles = (s.a.V + sg::lce_tile_columns(s.dtype, s.a) - 1) / sg::lce_tile_columns(s.dtype, s.a), blocks = sg::lce_gather_blocks((int)s.rows);
+    // scratch of this pass: targets [rows] (8 bytes each), statistics [piece][tiles] (8), target logits [piece], losses [rows], block counts
+    Tensor scratch = at::empty({2 * s.rows + 2 * s.piece * tiles + s.piece + s.rows + blocks}, fo);
+    float* f = scratch.data_ptr<float>();
+    int64_t* tc = reinterpret_cast<int64_t*>(f);
+    s.a.stats = reinterpret_cast<float2*>(f + 2 * s.rows);
+    s.a.z_target = f + 2 * s.rows + 2 * s.piece * tiles;
+    s.a.loss = s.a.z_target + s.piece;
+    int* kept = keep.data_ptr<int>() + s.rows;
+    s.a.target = tc;
+    s.a.count = kept + KEEP_COUNT;
+    s.a.u = train ? u.data_ptr() : nullptr;
+    s.a.loss_all = s.a.loss;
+    s.a.out_loss = loss.data_ptr<float>();
+    s.a.inv_count = reinterpret_cast<float*>(kept + KEEP_INV);
+    s.a.done = reinterpret_cast<unsigned*>(kept + KEEP_DONE);
+    int rc = sg::lce_gather(s.dtype, x.data_ptr(), s.ldx, t.data_ptr<int64_t>(), ignore_index, (int)s.rows, s.a.V, s.a.D, keep.data_ptr<int>(), xc.data_ptr(), tc,
+                            kept + KEEP_COUNT, s.a.done, reinterpret_cast<int*>(s.a.loss + s.rows), st);
+    const int64_t last = s.last();
+    if (train && last > 0 && need_x) dx = at::empty({last, x.size(1)}, fo);
+    if (train && last > 0 && need_w) dw = at::empty(w.sizes(), fo);
+    for (int64_t r0 = 0; r0 < s.rows && rc == 0; r0 += s.piece) {
+        const sg::LceArgs a = s.at(r0);
+        rc = sg::lce_logits(s.dtype, a, err.data_ptr<int>(), st);
+        if (rc == 0) rc = sg::lce_rows(s.dtype, a, r0 == last, st);
+        if (rc == 0 && train && r0 < last) {
+            sg::LceGrads g{};
+            Tensor part;
+            if (need_x) {
+                g.parts = sg::lce_dx_parts(s.dtype, a, need_w, &g.row_pitch);
+                part = g.parts == 1 && g.row_pitch == a.rows ? dx.narrow(0, r0, a.rows) : at::empty({g.parts * g.row_pitch, x.size(1)}, fo);
+                g.dx_part = part.data_ptr<float>();
+            }
+            g.dw = need_w ? dw.data_ptr() : nullptr;
+            g.dw_prev = need_w && r0 > 0 ? dw.data_ptr<float>() : nullptr;
+            g.f32_dw = true;
+            rc = sg::lce_grads(s.dtype, a, g, err.data_ptr<int>(), st);
+            if (rc == 0 && need_x && part.size(0) != a.rows)
+                rc = sg::lce_add_parts(g.dx_part, g.parts, g.row_pitch * x.size(1), a.rows * x.size(1), dx.data_ptr<float>() + r0 * x.size(1), st);
+        }
+    }
+    TORCH_CHECK(rc == 0, "linear_cross_entropy: launch failed (code ", rc, ")");
+    return {loss, xc, keep, u, dx, dw};
 }
 
-std::vector<Tensor> lce_bwd(const Tensor& x_, const Tensor& w_, const Tensor& t, const Tensor& mean, const Tensor& u, const Tensor& dx32, const Tensor& dw32,
-                            const Tensor& gout_, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
-    const Tensor x = loadable_rows(x_), w = loadable_rows(w_);
-    LceShape s = lce_shape(x, w, t, ignore_index, true);
-    c10::cuda::CUDAGuard guard(x.device());
+std::vector<Tensor> lce_bwd(const Tensor& w_, const Tensor& xc, const Tensor& keep, const Tensor& u, const Tensor& dx32, const Tensor& dw32, const Tensor& gout_,
+                            at::IntArrayRef x_size, bool need_x, bool need_w, Tensor err) {
+    c10::cuda::CUDAGuard guard(w_.device());
     auto st = at::cuda::getCurrentCUDAStream();
-    Tensor gout = gout_.to(at::kFloat).reshape({1}).contiguous();
     Tensor dx, dw;
-    const auto xo = x.options().memory_format(at::MemoryFormat::Contiguous);
-    if (need_x) dx = s.rows > 0 ? at::empty(x.sizes(), xo) : at::zeros(x.sizes(), xo);
-    if (need_w) dw = s.rows > 0 ? at::empty(w.sizes(), xo) : at::zeros(w.sizes(), xo);
-    if (s.rows == 0 || !(need_x || need_w)) return {dx, dw};
-    const int64_t last = s.last(), D = x.size(1);
-    TORCH_CHECK(u.is_contiguous() && u.size(0) == s.piece && u.size(1) == s.a.ldu && u.scalar_type() == x.scalar_type() && mean.numel() == 2,
-                "linear_cross_entropy: not what the forward pass left");
-    TORCH_CHECK((!need_x || dx32.numel() == last * D) && (!need_w || dw32.numel() == (last > 0 ? w.numel() : 0)), "linear_cross_entropy: not what the forward pass left");
+    const auto xo = w_.options().memory_format(at::MemoryFormat::Contiguous);
+    const int64_t rows = x_size[0], D = w_.size(1);
+    if (rows == 0) return {need_x ? at::zeros(x_size, xo) : dx, need_w ? at::zeros(w_.sizes(), xo) : dw};
+    const Tensor w = loadable_rows(w_);
+    LceShape s = lce_shape(xc, w, true);
+    Tensor gout = gout_.to(at::kFloat).reshape({1}).contiguous();
+    if (need_x) dx = at::empty(x_size, xo);
+    if (need_w) dw = at::empty(w.sizes(), xo);
+    const int64_t last = s.last();
+    TORCH_CHECK(xc.is_contiguous() && xc.size(0) == rows && xc.size(1) == D && u.is_contiguous() && u.dim() == 2 && u.size(0) == s.piece && u.size(1) == s.a.ldu &&
+                u.scalar_type() == w.scalar_type() && keep.numel() == rows + KEEP_MORE && (!need_x || dx32.numel() == last * D) &&
+                (!need_w || dw32.numel() == (last > 0 ? w.numel() : 0)), "linear_cross_entropy: not what the forward pass left");
+    const int* kept = keep.data_ptr<int>() + rows;
+    s.a.x = xc.data_ptr();
     s.a.u = u.data_ptr();
+    s.a.count = kept + KEEP_COUNT;
     const sg::LceArgs a = s.at(last);
     sg::LceGrads g{};
-    g.dx = need_x ? (char*)dx.data_ptr() + last * D * s.elem : nullptr;
+    Tensor part;
+    if (need_x) {
+        g.parts = sg::lce_dx_parts(s.dtype, a, need_w, &g.row_pitch);
+        part = at::empty({g.parts * g.row_pitch, D}, gout.options());
+        g.dx_part = part.data_ptr<float>();
+    }
     g.dw = need_w ? dw.data_ptr() : nullptr;
     g.dw_prev = need_w && last > 0 ? dw32.data_ptr<float>() : nullptr;
     g.gout = gout.data_ptr<float>();
-    g.inv_count = mean.data_ptr<float>() + 1;
-    Tensor scratch = at::empty({sg::lce_scratch(s.dtype, a, need_x, need_w)}, gout.options());
-    int rc = sg::lce_grads(s.dtype, a, g, scratch.data_ptr<float>(), err.data_ptr<int>(), st);
-    if (rc == 0 && need_x) rc = sg::lce_finish(s.dtype, dx32.data_ptr<float>(), dx.data_ptr(), last * D, g.gout, g.inv_count, st);
+    g.inv_count = reinterpret_cast<const float*>(kept + KEEP_INV);
+    int rc = sg::lce_grads(s.dtype, a, g, err.data_ptr<int>(), st);
+    if (rc == 0 && need_x)
+        rc = sg::lce_scatter(s.dtype, keep.data_ptr<int>(), (int)rows, (int)D, (int)last, last > 0 ? dx32.data_ptr<float>() : nullptr, g.dx_part, g.parts, g.row_pitch,
+                             g.gout, g.inv_count, dx.data_ptr(), st);
     TORCH_CHECK(rc == 0, "linear_cross_entropy: launch of the backward pass failed (code ", rc, ")");
     return {dx, dw};
 }
 
 struct LceNode : Function<LceNode> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, const Tensor& err) {
-        const Tensor x = loadable_rows(x_), w = loadable_rows(w_);        // the copy, where there is one, is what the backward pass reads
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, const Tensor& err) {
         auto r = lce_fwd(x, w, t, ignore_index, need_x, need_w, err);
-        if (need_x || need_w) ctx->save_for_backward({x, w, t, r[1], r[2], r[3], r[4]});
-        ctx->saved_data["err"] = err;                                     // the process's time-out flag itself, not a saved tensor
-        ctx->saved_data["ignore"] = ignore_index;
-        ctx->saved_data["need_x"] = need_x;
-        ctx->saved_data["need_w"] = need_w;
+        if (need_x || need_w) {
+            ctx->save_for_backward({w, r[1], r[2], r[3], r[4], r[5]});
+            ctx->saved_data["err"] = err;                                 // the process's time-out flag itself, not a saved tensor
+            ctx->saved_data["x"] = x.sizes();
+            ctx->saved_data["need_x"] = need_x;
+            ctx->saved_data["need_w"] = need_w;
+        }
         return r[0];
     }
     static variable_list backward(AutogradContext* ctx, variable_list dy) {
         refuse_second_order("linear_cross_entropy");
         const auto s = ctx->get_saved_variables();
-        auto r = lce_bwd(s[0], s[1], s[2], s[3], s[4], s[5], s[6], dy[0], ctx->saved_data["ignore"].toInt(), ctx->saved_data["need_x"].toBool(),
+        auto r = lce_bwd(s[0], s[1], s[2], s[3], s[4], s[5], dy[0], ctx->saved_data["x"].toIntVector(), ctx->saved_data["need_x"].toBool(),
                          ctx->saved_data["need_w"].toBool(), ctx->saved_data["err"].toTensor());
         return {r[0], r[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
@@ -267,7 +298,8 @@ struct LceNode : Function<LceNode> {
 
 void register_packed(pybind11::module_& m) {
     m.def("lce_fwd", &lce_fwd);
-    m.def("lce_bwd", &lce_bwd);
+    m.def("lce_bwd", [](const Tensor& w, const Tensor& xc, const Tensor& keep, const Tensor& u, const Tensor& dx, const Tensor& dw, const Tensor& gout,
+                        std::vector<int64_t> x_size, bool need_x, bool need_w, Tensor err) { return lce_bwd(w, xc, keep, u, dx, dw, gout, x_size, need_x, need_w, err); });
     m.def("lce_piece_rows", &lce_piece_rows);
     m.def("lce_node", [](const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, const Tensor& err) {
         return LceNode::apply(x, w, t, ignore_index, need_x, need_w, err);

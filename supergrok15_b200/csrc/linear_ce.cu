@@ -3,18 +3,19 @@
 //   loss = mean over counted rows of lse_r - z_{r,t_r},  lse_r = log sum_v exp z_rv
 //   d_rv = p_rv - [v = t_r],  p_rv = exp(z_rv - lse_r);   dx = f d w,  dw = f d^T x,  f = gout / count
 //
-// Rows go through in pieces.  (1) lce_logits: the product, tile by tile; a tile's epilogue leaves, per row, the maximum m and the sum of
-// u = exp(z - m), and, for a training pass, u itself in the type of x: the logits have been consumed when the tile's accumulators are
-// free.  (2) lce_rows: one pass over the statistics gives lse and the loss, one over u in place gives d = u exp(m - lse).  The sums leave
-// out the target's column: with s' the sum of the others and e_t = exp(z_t - max), 1 - p_t = s' / (s' + e_t) and the loss of a likely
-// target is log1p(s' / e_t), both to full precision however certain the target is (p_t - 1 from a rounded p_t, or lse - z_t, would be
-// rounding noise).  (3) lce_grads: both products with d.  Two roundings to 16 bits stand between z and a product, of u and of d, each at most half a
-// step of the value itself.
+// Rows without a counted target are left out first (lce_gather copies the others together): half of a fine-tuning batch is prompt, and what
+// stands there (padding, NaN) cannot reach a product.  The rows go through in pieces.  (1) lce_logits: the product, tile by tile; a tile's
+// epilogue leaves, per row, the maximum m and the sum of u = exp(z - m), and, for a training pass, u itself in the type of x: the logits
+// have been consumed when the tile's accumulators are free.  (2) lce_rows: one pass over the statistics gives lse and the loss, one over u
+// in place gives d = u exp(m - lse).  The sums leave out the target's column: with s' the sum of the others and e_t = exp(z_t - max),
+// 1 - p_t = s' / (s' + e_t) and the loss of a likely target is log1p(s' / e_t), both to full precision however certain the target is
+// (p_t - 1 from a rounded p_t, or lse - z_t, would be rounding noise).  (3) lce_grads: both products with d; (4) lce_scatter puts the rows
+// of dx back.  Two roundings to 16 bits stand between z and a product, of u and of d, each at most half a step of the value itself.
 //
 // Against a pass that recomputes z for the gradient this saves a fourth of all products (6 N V D operations instead of 8) and costs
 // reading and writing u once more.
 //
-// This file: the pass over the rows, and products on the CUDA cores for fp32 operands and for 16-bit ones that TMA cannot address.  Their
+// This file: the passes over the rows, and products on the CUDA cores for fp32 operands and for 16-bit ones that TMA cannot address.  Their
 // 64 x 64 tiles take 4 x 4 outputs per thread from shared memory in steps of 16, bound by the FMA pipe and its operand loads.
 #include "sg_native.h"
 #include "optim_math.cuh"
@@ -56,13 +57,14 @@ __device__ __forceinline__ void tile_product(const T* A, int64_t lda, const T* B
 
 template <typename T>
 __global__ void __launch_bounds__(CTHREADS) lce_logits_kernel(LceArgs a) {
-    const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, rows = lce_active(a);
+    if (m0 >= rows) return;
     float s[4][4] = {};
-    tile_product<T, false, false>((const T*)a.x, a.ldx, (const T*)a.w, a.ldw, a.rows, a.V, a.D, m0, n0, s);
+    tile_product<T, false, false>((const T*)a.x, a.D, (const T*)a.w, a.ldw, rows, a.V, a.D, m0, n0, s);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int row = m0 + ty * 4 + i;
-        const int64_t t = row < a.rows ? a.target[row] : -1;
+        const int64_t t = row < rows ? a.target[row] : -1;
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -80,73 +82,103 @@ __global__ void __launch_bounds__(CTHREADS) lce_logits_kernel(LceArgs a) {
             const int v = n0 + tx * 4 + j;
             const float e = expf(s[i][j] - ref);
             if (v != t) sum += e;
-            if (a.u && row < a.rows && v < a.V) ((T*)a.u)[(int64_t)row * a.ldu + v] = Cvt<T>::from(e * LceUnit<T>::value);
+            if (a.u && row < rows && v < a.V) ((T*)a.u)[(int64_t)row * a.ldu + v] = Cvt<T>::from(e * LceUnit<T>::value);
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (tx == 0 && row < a.rows) {
-            a.tile_max[(int64_t)blockIdx.x * a.rows + row] = mx;
-            a.tile_sum[(int64_t)blockIdx.x * a.rows + row] = sum;
-        }
+        if (tx == 0 && row < rows) a.stats[(int64_t)row * gridDim.x + blockIdx.x] = make_float2(mx, sum);
     }
 }
 
+// dx (AM = false: d [rows, V] times w [V, D]) or dw (AM = true: d^T times x [rows, D])
 template <typename T, typename TO, bool AM>
-__global__ void __launch_bounds__(CTHREADS) lce_grad_kernel(const T* A, int64_t lda, const T* B, int64_t ldb, int M, int N, int K, const float* prev, TO* out,
-                                                            const float* gout, const float* inv) {
-    const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+__global__ void __launch_bounds__(CTHREADS) lce_grad_kernel(LceArgs a, const float* prev, TO* out, const float* gout, const float* inv) {
+    const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, rows = lce_active(a);
+    const int M = AM ? a.V : rows;
+    if (m0 >= M) return;
     float s[4][4] = {};
-    tile_product<T, AM, true>(A, lda, B, ldb, M, N, K, m0, n0, s);
+    if (AM) tile_product<T, true, true>((const T*)a.u, a.ldu, (const T*)a.x, a.D, a.V, a.D, rows, m0, n0, s);
+    else tile_product<T, false, true>((const T*)a.u, a.ldu, (const T*)a.w, a.ldw, rows, a.D, a.V, m0, n0, s);
     const float f = gout ? gout[0] * inv[0] / LceUnit<T>::value : 1.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m < M && n < N) out[(int64_t)m * N + n] = Cvt<TO>::from(f * (prev ? s[i][j] + prev[(int64_t)m * N + n] : s[i][j]));
+            if (m < M && n < a.D) out[(int64_t)m * a.D + n] = Cvt<TO>::from(f * (prev ? s[i][j] + prev[(int64_t)m * a.D + n] : s[i][j]));
         }
 }
 
-// One CTA per row: the loss from the tiles' statistics, then u -> d in place (16 bytes per thread and step).
 constexpr int ROW_THREADS = 256;
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int tiles, int tile_cols) {
-    extern __shared__ float fac[];                                        // [tiles] factor of a tile's columns
-    __shared__ float red[ROW_THREADS / 32];
-    constexpr int PER = 16 / sizeof(T);
-    const int row = blockIdx.x;
-    float mx = -INFINITY;
-    for (int i = threadIdx.x; i < tiles; i += ROW_THREADS) mx = fmaxf(mx, a.tile_max[(int64_t)i * a.rows + row]);
+__device__ __forceinline__ float block_max(float v, float* red) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mx;
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < ROW_THREADS / 32; ++i) mx = fmaxf(mx, red[i]);
+    for (int i = 0; i < ROW_THREADS / 32; ++i) v = fmaxf(v, red[i]);
+    return v;
+}
+// the sum in every thread, added in a fixed order
+__device__ __forceinline__ float block_total(float v, float* red) {
+    v = block_sum(v, red);                                                // in the first warp
     __syncthreads();
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f;
-    for (int i = threadIdx.x; i < tiles; i += ROW_THREADS) sum += a.tile_sum[(int64_t)i * a.rows + row] * expf(a.tile_max[(int64_t)i * a.rows + row] - ref);
-    sum = block_sum(sum, red);                                            // in the first warp
-    if (threadIdx.x == 0) red[0] = sum;
+    if (threadIdx.x == 0) red[0] = v;
     __syncthreads();
-    const float others = red[0];                                          // sum of exp(z - max) over all columns but the target's
-    const int64_t t = a.target[row];
-    const bool counted = t != a.ignore_index && t >= 0 && t < a.V;
-    const float zt = counted ? a.z_target[row] : 0.f, et = counted ? expf(zt - ref) : 0.f, total = others + et;
+    return red[0];
+}
+
+// The loss of a row from its maximum, the sum of the other columns' exp(z - max) and the target's logit
+__device__ __forceinline__ float row_loss(float top, float others, float et, float zt) {
     // far below the maximum e_t loses digits and then vanishes, and the plain difference is exact enough
-    if (threadIdx.x == 0) a.loss[row] = !counted ? 0.f : (et > 1e-6f ? log1pf(others / et) : (ref - zt) + logf(total));
-    if (!a.u) return;
-    const float inv = 1.f / total;
-    for (int i = threadIdx.x; i < tiles; i += ROW_THREADS) fac[i] = expf(a.tile_max[(int64_t)i * a.rows + row] - ref) * inv;
+    return et > 1e-6f ? log1pf(others / et) : (top - zt) + logf(others + et);
+}
+
+// The CTA that finishes last adds up the losses of all pieces, in a fixed order.
+__device__ __forceinline__ void last_adds(const LceArgs& a, float* red) {
+    __shared__ bool is_last;
     __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        is_last = atomicAdd(a.done, 1u) + 1 == gridDim.x;
+    }
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+    const int n = *a.count;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x; i < n; i += 4 * ROW_THREADS)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) if (i + k * ROW_THREADS < n) s[k] += __ldcg(a.loss_all + i + k * ROW_THREADS);
+    const float total = block_total((s[0] + s[1]) + (s[2] + s[3]), red), inv = 1.f / (n > 0 ? n : 1);
+    if (threadIdx.x == 0) { *a.out_loss = total * inv; *a.inv_count = inv; }
+}
+
+// Training: one CTA per row: the loss from the tiles' statistics, then u -> d in place (16 bytes per thread and step).
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int tiles, int tile_cols, bool last) {
+    extern __shared__ float fac[];                                        // [tiles] factor of a tile's columns
+    __shared__ float red[32];
+    constexpr int PER = 16 / sizeof(T);
+    const int row = blockIdx.x, rows = lce_active(a);
     T* u = (T*)a.u + (int64_t)row * a.ldu;
-    for (int c = threadIdx.x * PER; c < a.ldu; c += ROW_THREADS * PER) {
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (counted) {
-            raw = *reinterpret_cast<const uint4*>(u + c);
+    if (row < rows) {
+        const float2* st = a.stats + (int64_t)row * tiles;
+        float mx = -INFINITY;
+        for (int i = threadIdx.x; i < tiles; i += ROW_THREADS) { fac[i] = st[i].x; mx = fmaxf(mx, fac[i]); }
+        mx = block_max(mx, red);
+        const float top = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f;
+        for (int i = threadIdx.x; i < tiles; i += ROW_THREADS) { fac[i] = expf(fac[i] - top); sum += st[i].y * fac[i]; }
+        const float others = block_total(sum, red);                       // without the target's column
+        const int64_t t = a.target[row];
+        const float zt = a.z_target[row], et = expf(zt - top), inv = 1.f / (others + et);
+        if (threadIdx.x == 0) a.loss[row] = row_loss(top, others, et, zt);
+        for (int c = threadIdx.x * PER; c < a.ldu; c += ROW_THREADS * PER) {
+            uint4 raw = *reinterpret_cast<const uint4*>(u + c);
             T* e = reinterpret_cast<T*>(&raw);
-            const float f = fac[c / tile_cols];                            // PER divides the tile's width
+            const float f = fac[c / tile_cols] * inv;                      // PER divides the tile's width
 #pragma unroll
             for (int k = 0; k < PER; ++k) {
                 float d = Cvt<T>::to(e[k]) * f;
@@ -154,22 +186,139 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int ti
                 if (c + k >= a.V) d = 0.f;                                 // columns between V and the pitch meet zeros of w
                 e[k] = Cvt<T>::from(d);
             }
+            *reinterpret_cast<uint4*>(u + c) = raw;
         }
-        *reinterpret_cast<uint4*>(u + c) = raw;
+    } else if (row < (rows + 63) / 64 * 64) {                              // the products take rows in steps of 64
+        for (int c = threadIdx.x * PER; c < a.ldu; c += ROW_THREADS * PER) *reinterpret_cast<uint4*>(u + c) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (last) last_adds(a, red);
+}
+
+// Evaluation: a warp per row.
+__global__ void __launch_bounds__(ROW_THREADS) lce_row_losses_kernel(LceArgs a, int tiles, bool last) {
+    __shared__ float red[32];
+    const int row = blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row < lce_active(a)) {
+        const float2* st = a.stats + (int64_t)row * tiles;
+        float mx = -INFINITY, sum = 0.f;
+        for (int i = lane; i < tiles; i += 32) mx = fmaxf(mx, st[i].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float top = mx == -INFINITY ? 0.f : mx;
+        for (int i = lane; i < tiles; i += 32) sum += st[i].y * expf(st[i].x - top);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) { const float zt = a.z_target[row]; a.loss[row] = row_loss(top, sum, expf(zt - top), zt); }
+    }
+    if (last) last_adds(a, red);
+}
+
+// ---- the counted rows
+constexpr int GATHER_ROWS = 32, COUNT_ROWS = 4096, GATHER_DIRECT = 16384;
+__device__ __forceinline__ bool counted(int64_t t, int64_t ignore_index, int V) { return t != ignore_index && t >= 0 && t < V; }
+
+// blocks[b] = counted rows among [4096 b, 4096 (b + 1))
+__global__ void __launch_bounds__(256) lce_count_kernel(const int64_t* __restrict__ target, int64_t ignore_index, int rows, int V, int* __restrict__ blocks) {
+    int n = 0;
+    for (int i = threadIdx.x; i < COUNT_ROWS; i += 256) {
+        const int r = blockIdx.x * COUNT_ROWS + i;
+        if (r < rows && counted(target[r], ignore_index, V)) ++n;
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    __shared__ int sh[8];
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) { int s = 0; for (int i = 0; i < 8; ++i) s += sh[i]; blocks[blockIdx.x] = s; }
+}
+
+// A CTA moves the counted ones of 32 rows: it counts the rows before its own (all of them up to 16,384 rows, else those of the
+// 4,096-row block it lies in, on top of the blocks' counts), so the order is kept and no CTA waits for another.
+__global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restrict__ x, int64_t pitch, const int64_t* __restrict__ target, int64_t ignore_index, int rows,
+                                                         int V, int row_bytes, int vec, int* __restrict__ place, uint8_t* __restrict__ xc, int64_t* __restrict__ tc,
+                                                         int* __restrict__ count, unsigned* __restrict__ done, const int* __restrict__ blocks) {
+    __shared__ int sh[8], base;
+    __shared__ int to[GATHER_ROWS];
+    const int r0 = blockIdx.x * GATHER_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int n = 0, from = 0;
+    if (blocks) {
+        from = r0 / COUNT_ROWS * COUNT_ROWS;
+        for (int i = threadIdx.x; i < r0 / COUNT_ROWS; i += 256) n += blocks[i];
+    }
+    for (int r = from + threadIdx.x; r < r0; r += 256) n += counted(target[r], ignore_index, V) ? 1 : 0;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) sh[warp] = n;
+    __syncthreads();
+    if (warp == 0) {
+        int b = 0;
+        for (int i = 0; i < 8; ++i) b += sh[i];
+        const int r = r0 + lane;
+        const int64_t t = r < rows ? target[r] : -1;
+        const bool on = r < rows && counted(t, ignore_index, V);
+        const unsigned m = __ballot_sync(0xffffffffu, on);
+        const int p = on ? b + __popc(m & ((1u << lane) - 1)) : -1;
+        to[lane] = p;
+        if (r < rows) place[r] = p;
+        if (on) tc[p] = t;
+        if (lane == 0) base = b + __popc(m);
+    }
+    __syncthreads();
+    for (int i = warp; i < GATHER_ROWS; i += 8) {
+        const int p = to[i];
+        if (p < 0) continue;
+        const uint8_t* src = x + (int64_t)(r0 + i) * pitch;
+        uint8_t* dst = xc + (int64_t)p * row_bytes;
+        if (vec) for (int c = lane * 16; c < row_bytes; c += 512) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+        else for (int c = lane * 2; c < row_bytes; c += 64) *reinterpret_cast<uint16_t*>(dst + c) = *reinterpret_cast<const uint16_t*>(src + c);
+    }
+    if (blockIdx.x == gridDim.x - 1) {
+        const int end = (base + 63) / 64 * 64 < rows ? (base + 63) / 64 * 64 : rows;
+        for (int64_t i = (int64_t)base * row_bytes + 2 * threadIdx.x; i < (int64_t)end * row_bytes; i += 512) *reinterpret_cast<uint16_t*>(xc + i) = 0;
+        if (threadIdx.x == 0) { *count = base; *done = 0u; }
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) lce_finish_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t n, const float* gout, const float* inv) {
-    const float f = gout[0] * inv[0] / LceUnit<T>::value;
-    const int64_t step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n / 4; i += step) {
-        const float4 v = reinterpret_cast<const float4*>(in)[i];
-        const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) out[4 * i + k] = Cvt<T>::from(e[k] * f);
+__global__ void __launch_bounds__(256) lce_add_parts_kernel(const float* __restrict__ part, int parts, int64_t pitch, int64_t n, float* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float s = 0.f;
+        for (int k = 0; k < parts; ++k) s += part[k * pitch + i];
+        out[i] = s;
     }
-    for (int64_t i = n / 4 * 4 + (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) out[i] = Cvt<T>::from(in[i] * f);
+}
+
+// A warp per row, eight columns (or one, where a row is not a whole number of eights) per lane and step
+template <typename T, int PER>
+__global__ void __launch_bounds__(256) lce_scatter_kernel(const int* __restrict__ place, int rows, int D, int first, const float* __restrict__ early,
+                                                          const float* __restrict__ part, int parts, int64_t row_pitch, const float* __restrict__ gout,
+                                                          const float* __restrict__ inv, T* __restrict__ dx) {
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    const int p = place[row];
+    const float f = p >= 0 && p < first ? gout[0] * inv[0] / LceUnit<T>::value : 1.f;
+    for (int c = lane * PER; c < D; c += 32 * PER) {
+        float v[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) v[k] = 0.f;
+        if (p >= 0) {
+            const float* src = p < first ? early + (int64_t)p * D + c : part + (int64_t)(p - first) * D + c;
+            const int n = p < first ? 1 : parts;
+            for (int s = 0; s < n; ++s) {
+                const float* q = src + s * row_pitch * D;
+                if constexpr (PER == 8) {
+                    const float4 x = reinterpret_cast<const float4*>(q)[0], y = reinterpret_cast<const float4*>(q)[1];
+                    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+                } else v[0] += q[0];
+            }
+        }
+        T o[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) o[k] = Cvt<T>::from(v[k] * f);
+        T* dst = dx + (int64_t)row * D + c;
+        if constexpr (PER == 8 && sizeof(T) == 2) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+        else if constexpr (PER == 8) {
+            reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(o)[0];
+            reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(o)[1];
+        } else dst[0] = o[0];
+    }
 }
 
 template <typename T> int logits(const LceArgs& a, cudaStream_t st) {
@@ -178,30 +327,41 @@ template <typename T> int logits(const LceArgs& a, cudaStream_t st) {
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
-template <typename T> int rows(const LceArgs& a, int tile_cols, cudaStream_t st) {
+template <typename T> int rows(const LceArgs& a, int tile_cols, bool last, cudaStream_t st) {
     const int tiles = (a.V + tile_cols - 1) / tile_cols;
+    count_launch();
+    if (!a.u) {
+        lce_row_losses_kernel<<<(a.rows + 7) / 8, ROW_THREADS, 0, st>>>(a, tiles, last);
+        return cudaGetLastError() == cudaSuccess ? 0 : 3;
+    }
     const size_t smem = tiles * sizeof(float);
     static std::atomic<uint64_t> done{0};
     if (!once_per_device(done, current_device(), [] { return cudaFuncSetAttribute(lce_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) == cudaSuccess; }))
         return 2;
     if (smem > 200 * 1024) return 4;
-    count_launch();
-    lce_rows_kernel<T><<<a.rows, ROW_THREADS, smem, st>>>(a, tiles, tile_cols);
+    lce_rows_kernel<T><<<a.rows, ROW_THREADS, smem, st>>>(a, tiles, tile_cols, last);
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
 template <typename T, typename TO> int grads(const LceArgs& a, const LceGrads& g, cudaStream_t st) {
-    const T *d = (const T*)a.u, *x = (const T*)a.x, *w = (const T*)a.w;
-    if (g.dx) {
+    if (g.dx_part) {
         count_launch();
-        lce_grad_kernel<T, TO, false><<<dim3((a.D + CT - 1) / CT, (a.rows + CT - 1) / CT), CTHREADS, 0, st>>>(d, a.ldu, w, a.ldw, a.rows, a.D, a.V, nullptr,
-                                                                                                           (TO*)g.dx, g.gout, g.inv_count);
+        lce_grad_kernel<T, float, false><<<dim3((a.D + CT - 1) / CT, (a.rows + CT - 1) / CT), CTHREADS, 0, st>>>(a, nullptr, g.dx_part, g.gout, g.inv_count);
     }
     if (g.dw) {
         count_launch();
-        lce_grad_kernel<T, TO, true><<<dim3((a.D + CT - 1) / CT, (a.V + CT - 1) / CT), CTHREADS, 0, st>>>(d, a.ldu, x, a.ldx, a.V, a.D, a.rows, g.dw_prev,
-                                                                                                       (TO*)g.dw, g.gout, g.inv_count);
+        lce_grad_kernel<T, TO, true><<<dim3((a.D + CT - 1) / CT, (a.V + CT - 1) / CT), CTHREADS, 0, st>>>(a, g.dw_prev, (TO*)g.dw, g.gout, g.inv_count);
     }
+    return cudaGetLastError() == cudaSuccess ? 0 : 3;
+}
+
+template <typename T>
+int scatter(const int* place, int rows, int D, int first, const float* early, const float* part, int parts, int64_t row_pitch, const float* gout, const float* inv,
+            void* dx, cudaStream_t st) {
+    count_launch();
+    const unsigned grid = (unsigned)((rows + 7) / 8);
+    if (D % 8 == 0) lce_scatter_kernel<T, 8><<<grid, 256, 0, st>>>(place, rows, D, first, early, part, parts, row_pitch, gout, inv, (T*)dx);
+    else lce_scatter_kernel<T, 1><<<grid, 256, 0, st>>>(place, rows, D, first, early, part, parts, row_pitch, gout, inv, (T*)dx);
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
@@ -209,28 +369,43 @@ template <typename T, typename TO> int grads(const LceArgs& a, const LceGrads& g
 
 #define SG_LCE_GO(fn, ...) { if (dtype == F32) return fn<float>(__VA_ARGS__); if (dtype == BF16) return fn<__nv_bfloat16>(__VA_ARGS__); return fn<__half>(__VA_ARGS__); }
 int lce_tile_columns(int dtype, const LceArgs& a) { return lce_sm100_takes(dtype, a) ? LCE_SM100_COLUMNS : CT; }
-int64_t lce_scratch(int dtype, const LceArgs& a, bool dx, bool dw) { return dx && lce_sm100_takes(dtype, a) ? lce_sm100_scratch(a.rows, a.V, a.D, dw) : 0; }
+int lce_dx_parts(int dtype, const LceArgs& a, bool with_dw, int64_t* row_pitch) {
+    if (lce_sm100_takes(dtype, a)) return lce_sm100_dx_parts(a.rows, a.V, a.D, with_dw, row_pitch);
+    *row_pitch = a.rows;
+    return 1;
+}
+int lce_gather_blocks(int rows) { return rows > GATHER_DIRECT ? (rows + COUNT_ROWS - 1) / COUNT_ROWS : 0; }
+int lce_gather(int dtype, const void* x, int64_t ldx, const int64_t* target, int64_t ignore_index, int rows, int V, int D, int* place, void* xc, int64_t* tc,
+               int* count, unsigned* done, int* blocks, cudaStream_t st) {
+    const int es = dtype == F32 ? 4 : 2, nb = lce_gather_blocks(rows);
+    const int vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * es) | (uintptr_t)(D * es)) & 15) == 0;
+    if (nb) {
+        count_launch();
+        lce_count_kernel<<<nb, 256, 0, st>>>(target, ignore_index, rows, V, blocks);
+    }
+    count_launch();
+    lce_gather_kernel<<<(rows + GATHER_ROWS - 1) / GATHER_ROWS, 256, 0, st>>>((const uint8_t*)x, ldx * es, target, ignore_index, rows, V, D * es, vec, place, (uint8_t*)xc, tc,
+                                                                            count, done, nb ? blocks : nullptr);
+    return cudaGetLastError() == cudaSuccess ? 0 : 3;
+}
 int lce_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st) {
     if (lce_sm100_takes(dtype, a)) return lce_sm100_logits(dtype, a, err, st);
     SG_LCE_GO(logits, a, st)
 }
-int lce_rows(int dtype, const LceArgs& a, cudaStream_t st) SG_LCE_GO(rows, a, lce_tile_columns(dtype, a), st)
-int lce_grads(int dtype, const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
-    if (lce_sm100_takes(dtype, a)) return lce_sm100_grads(dtype, a, g, scratch, err, st);
+int lce_rows(int dtype, const LceArgs& a, bool last, cudaStream_t st) SG_LCE_GO(rows, a, lce_tile_columns(dtype, a), last, st)
+int lce_grads(int dtype, const LceArgs& a, const LceGrads& g, int* err, cudaStream_t st) {
+    if (lce_sm100_takes(dtype, a)) return lce_sm100_grads(dtype, a, g, err, st);
     if (dtype == F32) return grads<float, float>(a, g, st);
-    if (dtype == BF16) return g.f32_out ? grads<__nv_bfloat16, float>(a, g, st) : grads<__nv_bfloat16, __nv_bfloat16>(a, g, st);
-    return g.f32_out ? grads<__half, float>(a, g, st) : grads<__half, __half>(a, g, st);
+    if (dtype == BF16) return g.f32_dw ? grads<__nv_bfloat16, float>(a, g, st) : grads<__nv_bfloat16, __nv_bfloat16>(a, g, st);
+    return g.f32_dw ? grads<__half, float>(a, g, st) : grads<__half, __half>(a, g, st);
 }
-#undef SG_LCE_GO
-int lce_finish(int dtype, const float* in, void* out, int64_t n, const float* gout, const float* inv, cudaStream_t st) {
-    if (n == 0) return 0;
-    const int64_t want = (n / 4 + 255) / 256 + 1;
-    const int grid = (int)(want < 148 * 8 ? want : 148 * 8);
+int lce_add_parts(const float* part, int parts, int64_t pitch, int64_t n, float* out, cudaStream_t st) {
     count_launch();
-    if (dtype == F32) lce_finish_kernel<float><<<grid, 256, 0, st>>>(in, (float*)out, n, gout, inv);
-    else if (dtype == BF16) lce_finish_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(in, (__nv_bfloat16*)out, n, gout, inv);
-    else lce_finish_kernel<__half><<<grid, 256, 0, st>>>(in, (__half*)out, n, gout, inv);
+    lce_add_parts_kernel<<<(unsigned)((n + 255) / 256 < 148 * 8 ? (n + 255) / 256 : 148 * 8), 256, 0, st>>>(part, parts, pitch, n, out);
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
+int lce_scatter(int dtype, const int* place, int rows, int D, int first, const float* early, const float* part, int parts, int64_t row_pitch, const float* gout,
+                const float* inv_count, void* dx, cudaStream_t st) SG_LCE_GO(scatter, place, rows, D, first, early, part, parts, row_pitch, gout, inv_count, dx, st)
+#undef SG_LCE_GO
 
 }  // namespace sg

@@ -48,15 +48,16 @@ struct LBars {
 struct LArgs {
     // LOGITS
     const int64_t* target;
-    int64_t ignore_index;
-    float *tile_max, *tile_sum, *z_target;
+    float2* stats;
+    float* z_target;
     int store_u;
     // GRADS
     const float* dw_prev;
     const float *gout, *inv;
-    int splits, f32_x, f32_w;                                             // f32: that output is fp32 (for dx also: partial sums)
+    int splits, f32_w;                                                    // dx is left as fp32 sums of its splits; f32_w: dw is fp32
     int items_x;                                                          // items below this are dx
-    int rows, V, D;
+    const int* count;                                                     // rows there are: *count - first, `rows` at most
+    int first, rows, V, D;
     int* err;
 };
 
@@ -150,6 +151,7 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
     if (PAIR) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = b->tmem_slot;
+    const int live = min(max(__ldg(a.count) - a.first, 0), a.rows);       // rows of this piece
     // the item that every warp of both CTAs works on next
     auto take = [&](uint32_t n, LItem& w) {
         const uint32_t s = n & 1;
@@ -168,6 +170,7 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
             bool more = true;
             while (true) {
                 LItem w{};
+                bool empty = false;                                       // a tile past the last row: nothing to do
                 if (more) {
                     mbar_expect_tx(&b->clc, 16);
                     clc_ask(&b->answer, &b->clc);
@@ -176,6 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                         int m, n;
                         logits_tile(i, (a.rows + BM - 1) / BM, (a.V + BN - 1) / BN, m, n);
                         w.m0 = m * BM; w.n0 = n * BN; w.nkb = (a.D + BK - 1) / BK;
+                        empty = w.m0 >= live;
                     } else {
                         const int tn = (a.D + BN - 1) / BN;
                         if (i < a.items_x) {
@@ -186,26 +190,29 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                             w.kb0 = w.split * per;
                             w.nkb = kb - w.kb0 < per ? kb - w.kb0 : per;
                             if (w.nkb < 0) w.nkb = 0;                     // a split past the end: all zeros
+                            empty = w.m0 >= live;
                         } else {
                             const int r = i - a.items_x;
                             w.kind = 2;
-                            w.m0 = r / tn * BM; w.n0 = r % tn * BN; w.nkb = (a.rows + BK - 1) / BK;
+                            w.m0 = r / tn * BM; w.n0 = r % tn * BN; w.nkb = (live + BK - 1) / BK;
                         }
                     }
                 }
-                const uint32_t s = n_item & 1;
-                if (n_item >= 2 && !mbar_wait(&b->item_empty[s], ((n_item >> 1) & 1) ^ 1)) { atomicExch(a.err, 101); break; }
-                ++n_item;
-                if constexpr (PAIR) {
-                    for (uint32_t r = 0; r < 2; ++r) {
-                        const uint32_t bar = in_cta(&b->item_full[s], r), to = in_cta(&b->item[s], r);
-                        cluster_expect(bar, 32);
-                        cluster_store(to, w.m0, w.n0, w.kb0, w.nkb, bar);
-                        cluster_store(to + 16, w.kind, w.split, 0, 0, bar);
+                if (!empty) {
+                    const uint32_t s = n_item & 1;
+                    if (n_item >= 2 && !mbar_wait(&b->item_empty[s], ((n_item >> 1) & 1) ^ 1)) { atomicExch(a.err, 101); break; }
+                    ++n_item;
+                    if constexpr (PAIR) {
+                        for (uint32_t r = 0; r < 2; ++r) {
+                            const uint32_t bar = in_cta(&b->item_full[s], r), to = in_cta(&b->item[s], r);
+                            cluster_expect(bar, 32);
+                            cluster_store(to, w.m0, w.n0, w.kb0, w.nkb, bar);
+                            cluster_store(to + 16, w.kind, w.split, 0, 0, bar);
+                        }
+                    } else {
+                        b->item[s] = w;
+                        mbar_arrive(&b->item_full[s]);
                     }
-                } else {
-                    b->item[s] = w;
-                    mbar_arrive(&b->item_full[s]);
                 }
                 if (!more) break;
                 if (!mbar_wait(&b->clc, n_clc & 1)) { atomicExch(a.err, 103); break; }
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                 __syncwarp();
                 if (lane == 0) arrive_first(&b->acc_empty[s]);             // everything is in registers
                 if (n0 < a.V) {
-                    const int64_t t = row < a.rows ? a.target[row] : -1;
+                    const int64_t t = row < live ? a.target[row] : -1;
                     const int tc = t >= n0 && t < n0 + 128 && t < a.V ? (int)(t - n0) : -1;        // the target's column, if it is here
                     if (n0 + 128 > a.V) {                                 // columns past the vocabulary
 #pragma unroll
@@ -369,14 +376,10 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                         }
                     };
                     chunk(r[0], 0); chunk(r[1], 1); chunk(r[2], 2); chunk(r[3], 3);
-                    if (row < a.rows) {
-                        const int64_t at = (int64_t)(n0 / 128) * a.rows + row;
-                        a.tile_max[at] = mx;
-                        a.tile_sum[at] = sum0 + sum1;
-                    }
+                    if (row < live) a.stats[(int64_t)row * ((a.V + 127) / 128) + n0 / 128] = make_float2(mx, sum0 + sum1);
                 }
             } else {
-                const bool is_x = w.kind == 1, f32 = is_x ? a.f32_x : a.f32_w;
+                const bool is_x = w.kind == 1, f32 = is_x || a.f32_w;
                 const CUtensorMap* map = is_x ? &map_c1 : &map_c2;
                 const int tm = (a.rows + BM - 1) / BM, mrow = w.m0 + q * 32 + (is_x ? w.split * tm * BM : 0);      // partial sums of dx: [split][rows]
                 const float* prev = !is_x && a.dw_prev && row < a.V ? a.dw_prev + (int64_t)row * a.D : nullptr;
@@ -433,20 +436,6 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
     }
 }
 
-// dx = its partial sums (scaled already), added in order: four columns per thread
-template <typename T, bool F32>
-__global__ void __launch_bounds__(256) lce_sum_dx_kernel(const float* __restrict__ part, int splits, int64_t pitch, int64_t n, void* __restrict__ out) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
-    float4 s = *reinterpret_cast<const float4*>(part + i);
-    for (int k = 1; k < splits; ++k) {
-        const float4 p = *reinterpret_cast<const float4*>(part + k * pitch + i);
-        s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
-    }
-    if (F32) *reinterpret_cast<float4*>((float*)out + i) = s;
-    else *reinterpret_cast<uint2*>((T*)out + i) = make_uint2(Half2<T>::pack(s.x, s.y), Half2<T>::pack(s.z, s.w));
-}
-
 template <typename T, bool GRADS, bool PAIR>
 int launch(unsigned items, const CUtensorMap& a1, const CUtensorMap& b1, const CUtensorMap& c1, const CUtensorMap& a2, const CUtensorMap& b2, const CUtensorMap& c2,
            const LArgs& k, cudaStream_t st) {
@@ -468,10 +457,10 @@ int launch(unsigned items, const CUtensorMap& a1, const CUtensorMap& b1, const C
 template <typename T, bool PAIR> int logits(const LceArgs& a, int* err, cudaStream_t st) {
     using S = Shape<PAIR>;
     CUtensorMap mx, mw, mu;
-    if (!make_map(&mx, a.x, a.rows, a.D, a.ldx, 128, BK, true) || !make_map(&mw, a.w, a.V, a.D, a.ldw, S::B_ROWS, BK, true)) return 10;
+    if (!make_map(&mx, a.x, a.rows, a.D, a.D, 128, BK, true) || !make_map(&mw, a.w, a.V, a.D, a.ldw, S::B_ROWS, BK, true)) return 10;
     if (a.u && !make_map(&mu, a.u, a.rows, a.ldu, a.ldu, 32, 64, true)) return 10;
     LArgs k{};
-    k.target = a.target; k.ignore_index = a.ignore_index; k.tile_max = a.tile_max; k.tile_sum = a.tile_sum; k.z_target = a.z_target;
+    k.target = a.target; k.stats = a.stats; k.z_target = a.z_target; k.count = a.count; k.first = a.first;
     k.store_u = a.u != nullptr; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err;
     const CUtensorMap& c = a.u ? mu : mx;                                 // without u no map of it is used
     return launch<T, false, PAIR>((unsigned)((a.rows + S::BM - 1) / S::BM) * (unsigned)((a.V + BN - 1) / BN), mx, mw, c, mx, mw, c, k, st);
@@ -491,50 +480,41 @@ int dx_splits(int rows, int V, int D, bool with_dw) {
     return s < 1 ? 1 : (int)s;
 }
 
-template <typename T, bool PAIR> int grads(const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
+template <typename T, bool PAIR> int grads(const LceArgs& a, const LceGrads& g, int* err, cudaStream_t st) {
     using S = Shape<PAIR>;
     CUtensorMap ua, wb, cx, um, xb, cw;
-    const int splits = g.dx ? dx_splits(a.rows, a.V, a.D, g.dw != nullptr) : 1;
     const int tm = (a.rows + S::BM - 1) / S::BM, tn = (a.D + BN - 1) / BN;
-    const bool part = splits > 1;
     if (!make_map(&ua, a.u, a.rows, a.V, a.ldu, 128, BK, true) || !make_map(&um, a.u, a.rows, a.V, a.ldu, BK, 64, true) ||
-        !make_map(&wb, a.w, a.V, a.D, a.ldw, BK, 64, true) || !make_map(&xb, a.x, a.rows, a.D, a.ldx, BK, 64, true)) return 10;
-    const bool x32 = g.f32_out || part;
+        !make_map(&wb, a.w, a.V, a.D, a.ldw, BK, 64, true) || !make_map(&xb, a.x, a.rows, a.D, a.D, BK, 64, true)) return 10;
     cx = ua; cw = ua;
-    if (g.dx && !make_map(&cx, part ? (void*)scratch : g.dx, part ? (int64_t)splits * tm * S::BM : a.rows, a.D, a.D, 32, x32 ? 32 : 64, !x32)) return 10;
-    if (g.dw && !make_map(&cw, g.dw, a.V, a.D, a.D, 32, g.f32_out ? 32 : 64, !g.f32_out)) return 10;
+    if (g.dx_part && !make_map(&cx, g.dx_part, g.parts * g.row_pitch, a.D, a.D, 32, 32, false)) return 10;
+    if (g.dw && !make_map(&cw, g.dw, a.V, a.D, a.D, 32, g.f32_dw ? 32 : 64, !g.f32_dw)) return 10;
     LArgs k{};
-    k.dw_prev = g.dw_prev; k.splits = splits; k.f32_x = x32; k.f32_w = g.f32_out; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err;
+    k.dw_prev = g.dw_prev; k.splits = g.parts; k.f32_w = g.f32_dw; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err; k.count = a.count; k.first = a.first;
     k.gout = g.gout; k.inv = g.inv_count;
-    k.items_x = g.dx ? splits * tm * tn : 0;
+    k.items_x = g.dx_part ? g.parts * tm * tn : 0;
     const unsigned items = (unsigned)k.items_x + (g.dw ? (unsigned)((a.V + S::BM - 1) / S::BM) * (unsigned)tn : 0u);
-    const int rc = launch<T, true, PAIR>(items, ua, wb, cx, um, xb, cw, k, st);
-    if (rc != 0 || !part) return rc;
-    const int64_t n = (int64_t)a.rows * a.D, pitch = (int64_t)tm * S::BM * a.D;
-    const unsigned grid = (unsigned)((n / 4 + 255) / 256);
-    count_launch();
-    if (g.f32_out) lce_sum_dx_kernel<T, true><<<grid, 256, 0, st>>>(scratch, splits, pitch, n, g.dx);
-    else lce_sum_dx_kernel<T, false><<<grid, 256, 0, st>>>(scratch, splits, pitch, n, g.dx);
-    return cudaGetLastError() == cudaSuccess ? 0 : 12;
+    return launch<T, true, PAIR>(items, ua, wb, cx, um, xb, cw, k, st);
 }
 
 }  // namespace
 
 bool lce_sm100_takes(int dtype, const LceArgs& a) {
     const auto ok = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld > 0 && ld % 8 == 0; };
-    return dtype != F32 && a.D % 8 == 0 && ok(a.x, a.ldx) && ok(a.w, a.ldw);
+    return dtype != F32 && a.D % 8 == 0 && ok(a.x, a.D) && ok(a.w, a.ldw);
 }
-int64_t lce_sm100_scratch(int rows, int V, int D, bool with_dw) {
-    const int s = dx_splits(rows, V, D, with_dw), bm = in_pairs(rows) ? 256 : 128;
-    return s > 1 ? (int64_t)s * ((rows + bm - 1) / bm * bm) * D : 0;
+int lce_sm100_dx_parts(int rows, int V, int D, bool with_dw, int64_t* row_pitch) {
+    const int bm = in_pairs(rows) ? 256 : 128;
+    *row_pitch = (int64_t)((rows + bm - 1) / bm) * bm;
+    return dx_splits(rows, V, D, with_dw);
 }
 int lce_sm100_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st) {
     if (in_pairs(a.rows)) return dtype == BF16 ? logits<__nv_bfloat16, true>(a, err, st) : logits<__half, true>(a, err, st);
     return dtype == BF16 ? logits<__nv_bfloat16, false>(a, err, st) : logits<__half, false>(a, err, st);
 }
-int lce_sm100_grads(int dtype, const LceArgs& a, const LceGrads& g, float* scratch, int* err, cudaStream_t st) {
-    if (in_pairs(a.rows)) return dtype == BF16 ? grads<__nv_bfloat16, true>(a, g, scratch, err, st) : grads<__half, true>(a, g, scratch, err, st);
-    return dtype == BF16 ? grads<__nv_bfloat16, false>(a, g, scratch, err, st) : grads<__half, false>(a, g, scratch, err, st);
+int lce_sm100_grads(int dtype, const LceArgs& a, const LceGrads& g, int* err, cudaStream_t st) {
+    if (in_pairs(a.rows)) return dtype == BF16 ? grads<__nv_bfloat16, true>(a, g, err, st) : grads<__half, true>(a, g, err, st);
+    return dtype == BF16 ? grads<__nv_bfloat16, false>(a, g, err, st) : grads<__half, false>(a, g, err, st);
 }
 
 }  // namespace sg

@@ -453,11 +453,6 @@ void ce_fwd(int dtype, const void* logits, const int64_t* target, float* lse, fl
     ce_mean_kernel<<<1, CE_MEAN_THREADS, 0, st>>>(loss, target, rows, V, ignore_index, mean_out);
 }
 
-void ce_mean(const float* loss, const int64_t* target, int64_t rows, int V, int64_t ignore_index, float* out, cudaStream_t st) {
-    count_launch();
-    ce_mean_kernel<<<1, CE_MEAN_THREADS, 0, st>>>(loss, target, rows, V, ignore_index, out);
-}
-
 void ce_bwd(int dtype, const void* logits, const int64_t* target, const float* lse, const float* mean_out, const float* gout, void* dlogits,
             int64_t rows, int V, int64_t ignore_index, cudaStream_t st) {
     if (rows <= 0) return;

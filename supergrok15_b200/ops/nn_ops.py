@@ -548,24 +548,23 @@ class _LinearCrossEntropy(torch.autograd.Function):
         from . import gemm as _gemm
         need = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         loss, *kept = _build.require().lce_fwd(x, weight, target, ignore_index, *need, _gemm._err_flag(x.device))
-        ctx.save_for_backward(x, weight, target, *kept)
-        ctx.args = ignore_index, *need
+        ctx.save_for_backward(weight, *kept)
+        ctx.args = x.shape, *need
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
         from . import gemm as _gemm
-        x = ctx.saved_tensors[0]
-        return (*_build.require().lce_bwd(*ctx.saved_tensors, gout, *ctx.args, _gemm._err_flag(x.device)), None, None)
+        return (*_build.require().lce_bwd(*ctx.saved_tensors, gout, *ctx.args, _gemm._err_flag(gout.device)), None, None)
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
     """Mean cross-entropy of the logits ``x @ weight.T`` against int64 ``target``, without keeping the logits: ``x [..., D]``,
     ``weight [vocabulary, D]``, ``target [...]``; the result is an fp32 scalar.
 
-    Positions whose target is ``ignore_index`` or lies outside the vocabulary are not counted: they add nothing to the loss, and their rows of
-    the gradient are zero (no counted position: loss 0).  bf16, fp16 and fp32 on CUDA, for any vocabulary.  At most 256 MB (or 256 rows) of
+    Positions whose target is ``ignore_index`` or lies outside the vocabulary are not counted: they are left out before anything is computed, so
+    they cost nothing, whatever stands in their rows of ``x`` reaches nothing, and their rows of the gradient are zero (no counted position: loss 0).  bf16, fp16 and fp32 on CUDA, for any vocabulary.  At most 256 MB (or 256 rows) of
     [rows, vocabulary] values exist at a time, in the type of ``x``; a pass with gradients takes the rows in pieces of that size, and from the
     second piece on holds the weight's gradient in fp32 between forward and backward.  The gradients' products of all pieces but the last
     are formed in the forward pass.  Sums are fp32 and added in a fixed order."""

@@ -54,6 +54,12 @@ def check(x, w, t, gout=1.0, repeat=True):
     return loss, gx, gw
 
 
+def check_quick(x, w, t):
+    x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = nn_ops.linear_cross_entropy(x, w, t)
+    return [loss, *torch.autograd.grad(loss, (x, w))]
+
+
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 LOSS_SCALE = {torch.float32: 1.0, torch.bfloat16: 0.3, torch.float16: 8192.0}
 
@@ -83,6 +89,26 @@ def test_pieces(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [33, 4096, 16384, 16385, 30000])
+def test_many_rows_few_counted(N, dtype):
+    """The counted rows are found across work items of 32 rows and, above 16,384 rows, blocks of 4,096; whole pieces may be empty."""
+    x, w, t = inputs(N, 300, 16, dtype)
+    for lo, hi in ((0, 40), (N // 2, N // 2 + 70), (N - 5, N)):
+        s = torch.full_like(t, -100)
+        s[lo:hi] = t[lo:hi]
+        check(x, w, s, gout=LOSS_SCALE[dtype])
+    check(x, w, torch.where(torch.arange(N, device="cuda") % 3 == 0, t, 300), gout=LOSS_SCALE[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pieces_without_counted_rows(dtype):
+    N, V, D = 1100, 200000, 16
+    x, w, t = inputs(N, V, D, dtype)
+    t[300:] = -100
+    check(x, w, t, gout=LOSS_SCALE[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_confident_and_hopeless_rows(dtype):
     """Targets with a probability of nearly one (p - 1 must not be the rounding of p) and logits hundreds apart."""
     for std, at in ((30.0, 1.0), (200.0, 1.0), (0.0, 1.0)):
@@ -105,6 +131,9 @@ def test_rows_that_are_not_counted(dtype):
     keep = (t >= 0) & (t < 500)
     loss, gx, gw = check(x[keep], w, t[keep])
     assert far(want[0], loss) < 1e-6 and far(want[1][keep], gx) <= 2 * HALF_STEP[dtype] and far(want[2], gw) <= 2 * HALF_STEP[dtype] + 1e-6
+    bad = x.clone()
+    bad[~keep] = float("nan")
+    assert all(torch.equal(a, b) for a, b in zip(check_quick(bad, w, t), want))        # what stands there reaches nothing
     none = torch.full_like(t, -100)
     loss, gx, gw = check(x, w, none)
     assert float(loss) == 0.0 and not gx.any() and not gw.any()
