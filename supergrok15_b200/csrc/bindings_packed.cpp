@@ -1,4 +1,5 @@
 // Bindings of the operators of packed language-model training: attention over packed sequences, cross-entropy of a linear head.
+#include <cmath>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include "bindings_decl.h"
@@ -30,15 +31,16 @@ Tensor loadable(const Tensor& t) {
 }
 
 sg::PackedAttn packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, bool causal, double scale) {
-    TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(2) == k.size(2),
-                "attention_packed: q [rows, heads, head_dim], k and v [rows, kv_heads, head_dim]");
-    TORCH_CHECK(k.device() == q.device() && v.device() == q.device() && cu.device() == q.device(), "attention_packed: all tensors on one device");
-    TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "attention_packed: q, k and v of one dtype");
-    TORCH_CHECK(q.size(0) < ((int64_t)1 << 30) && cu.numel() < ((int64_t)1 << 30), "attention_packed: fewer than 2^30 rows");
-    TORCH_CHECK(k.size(1) > 0 && q.size(1) % k.size(1) == 0 && q.size(1) <= 65535, "attention_packed: heads must be a multiple of kv_heads, 65,535 at most");
-    TORCH_CHECK(q.size(2) >= 1 && q.size(2) <= 128, "attention_packed: head_dim 1 to 128");
-    TORCH_CHECK(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.is_contiguous() && cu.numel() >= 1, "attention_packed: cu_seqlens [sequences + 1]");
-    TORCH_CHECK(head_rows_ok(q) && head_rows_ok(k) && head_rows_ok(v), "attention_packed: the last index must be contiguous");
+    TORCH_CHECK_VALUE(q.is_cuda() && q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(2) == k.size(2),
+                      "attention_packed: q [rows, heads, hd] and k, v [rows, kv_heads, hd] expected, got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+    TORCH_CHECK_VALUE(k.size(1) > 0 && q.size(1) % k.size(1) == 0, "attention_packed: ", q.size(1), " query heads are not a multiple of ", k.size(1), " key heads");
+    TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1 && cu.scalar_type() == at::kInt, "attention_packed: cu_seqlens must be a vector of sequences + 1 int32 or int64 offsets");
+    TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() && v.device() == q.device() &&
+                      cu.device() == q.device(), "attention_packed: q, k and v need one dtype, and all tensors one device");
+    TORCH_CHECK_VALUE((q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf || q.scalar_type() == at::kFloat) && q.size(2) >= 1 && q.size(2) <= 128,
+                      "attention_packed: bf16, fp16 or fp32 with head sizes up to 128 on CUDA, got ", q.scalar_type(), " with ", q.size(2));
+    TORCH_CHECK_VALUE(q.size(0) < ((int64_t)1 << 30) && cu.numel() < ((int64_t)1 << 30) && q.size(1) <= 65535, "attention_packed: fewer than 2^30 rows, 65,535 heads at most");
+    TORCH_CHECK(cu.is_contiguous() && head_rows_ok(q) && head_rows_ok(k) && head_rows_ok(v), "attention_packed: the last index must be contiguous");
     sg::PackedAttn p{};
     p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr();
     p.q_ld = q.stride(0); p.k_ld = k.stride(0); p.v_ld = v.stride(0);
@@ -169,13 +171,16 @@ enum { KEEP_COUNT = 0, KEEP_DONE = 1, KEEP_INV = 2, KEEP_MORE = 4 };
 // Returns (loss, xc, keep, d, dx of earlier pieces, dw of earlier pieces).  The gradient products of the last piece are left to the backward
 // pass, which writes them in the final type; of the pieces before it the products are taken here, because their d makes room for the next one's.
 std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w_, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, Tensor err) {
-    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w_.dim() == 2 && t.dim() == 1 && x.size(1) == w_.size(1) && t.size(0) == x.size(0),
-                "linear_cross_entropy: x [rows, D], weight [vocabulary, D], target [rows]");
-    TORCH_CHECK(w_.device() == x.device() && t.device() == x.device(), "linear_cross_entropy: all tensors on one device");
-    TORCH_CHECK(w_.scalar_type() == x.scalar_type() && t.scalar_type() == at::kLong && t.is_contiguous(), "linear_cross_entropy: x and weight of one dtype, int64 targets");
-    TORCH_CHECK(w_.size(0) >= 1 && w_.size(0) < (1 << 22) && x.size(1) >= 1 && x.size(1) < (1 << 22) && x.size(0) < ((int64_t)1 << 30),
-                "linear_cross_entropy: vocabulary and width below 2^22, fewer than 2^30 rows");
-    TORCH_CHECK((x.stride(1) == 1 || x.size(1) == 1) && (w_.stride(1) == 1 || w_.size(1) == 1), "linear_cross_entropy: the last index must be contiguous");
+    TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && w_.dim() == 2 && t.dim() == 1 && x.size(1) == w_.size(1) && t.size(0) == x.size(0),
+                      "linear_cross_entropy: x [..., D], weight [vocabulary, D] and target [...] expected, got ", x.sizes(), ", ", w_.sizes(), ", ", t.sizes());
+    TORCH_CHECK_VALUE(w_.scalar_type() == x.scalar_type() && t.scalar_type() == at::kLong && w_.device() == x.device() && t.device() == x.device(),
+                      "linear_cross_entropy: x and weight need one dtype, target int64, and all tensors one device");
+    TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf || x.scalar_type() == at::kFloat,
+                      "linear_cross_entropy: bf16, fp16 or fp32 on CUDA, got ", x.scalar_type());
+    TORCH_CHECK_VALUE(w_.size(0) >= 1 && w_.size(0) < (1 << 22) && x.size(1) >= 1 && x.size(1) < (1 << 22) && x.size(0) < ((int64_t)1 << 30),
+                      "linear_cross_entropy: vocabulary and width from 1 to below 2^22, fewer than 2^30 rows");
+    TORCH_CHECK(t.is_contiguous() && (x.stride(1) == 1 || x.size(1) == 1) && (w_.stride(1) == 1 || w_.size(1) == 1),
+                "linear_cross_entropy: the last index must be contiguous");
     const bool train = need_x || need_w;
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor w = loadable_rows(w_);
@@ -301,13 +306,26 @@ void register_packed(pybind11::module_& m) {
     m.def("lce_bwd", [](const Tensor& w, const Tensor& xc, const Tensor& keep, const Tensor& u, const Tensor& dx, const Tensor& dw, const Tensor& gout,
                         std::vector<int64_t> x_size, bool need_x, bool need_w, Tensor err) { return lce_bwd(w, xc, keep, u, dx, dw, gout, x_size, need_x, need_w, err); });
     m.def("lce_piece_rows", &lce_piece_rows);
-    m.def("lce_node", [](const Tensor& x, const Tensor& w, const Tensor& t, int64_t ignore_index, bool need_x, bool need_w, const Tensor& err) {
-        return LceNode::apply(x, w, t, ignore_index, need_x, need_w, err);
+    // x [..., D] and target [...] of any strides
+    m.def("lce_node", [](const Tensor& x_, const Tensor& w_, const Tensor& t_, int64_t ignore_index, const Tensor& err) {
+        TORCH_CHECK_VALUE(x_.dim() >= 1 && w_.dim() == 2 && t_.sizes() == x_.sizes().slice(0, x_.dim() - 1),
+                          "linear_cross_entropy: x [..., D], weight [vocabulary, D] and target [...] expected, got ", x_.sizes(), ", ", w_.sizes(), ", ", t_.sizes());
+        const bool grad = at::GradMode::is_enabled();
+        Tensor x = x_.dim() == 2 ? x_ : x_.reshape({t_.numel(), x_.size(-1)}), w = w_, t = t_.dim() == 1 ? t_ : t_.reshape({-1});
+        if (x.stride(1) != 1) x = x.contiguous();
+        if (w.stride(1) != 1) w = w.contiguous();
+        if (!t.is_contiguous()) t = t.contiguous();
+        return LceNode::apply(x, w, t, ignore_index, grad && x.requires_grad(), grad && w.requires_grad(), err);
     });
     m.def("packed_attn_fwd", &packed_attn_fwd);
     m.def("packed_attn_bwd", &packed_attn_bwd);
-    m.def("packed_attn_node", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, bool causal, double scale, bool train, const Tensor& err) {
-        return PackedAttnNode::apply(q, k, v, cu, causal, scale, train, err);
+    m.def("packed_attn_node", [](const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_, bool causal, c10::optional<double> scale, const Tensor& err) {
+        const auto rows = [](const Tensor& t) { return t.dim() != 3 || t.stride(2) == 1 ? t : t.contiguous(); };
+        const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
+        Tensor cu = cu_.scalar_type() == at::kLong ? cu_.to(at::kInt) : cu_;
+        if (!cu.is_contiguous()) cu = cu.contiguous();
+        const bool train = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+        return PackedAttnNode::apply(q, k, v, cu, causal, scale.has_value() ? *scale : (q.dim() == 3 && q.size(2) > 0 ? 1.0 / std::sqrt((double)q.size(2)) : 1.0), train, err);
     });
 }
 }  // namespace sgb

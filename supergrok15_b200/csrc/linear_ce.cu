@@ -141,7 +141,7 @@ __device__ __forceinline__ void last_adds(const LceArgs& a, float* red) {
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
-        is_last = atomicAdd(a.done, 1u) + 1 == gridDim.x;
+        is_last = atomicAdd(a.done, 1u) + 1 == gridDim.x * gridDim.y;
     }
     __syncthreads();
     if (!is_last) return;
@@ -155,13 +155,29 @@ __device__ __forceinline__ void last_adds(const LceArgs& a, float* red) {
     if (threadIdx.x == 0) { *a.out_loss = total * inv; *a.inv_count = inv; }
 }
 
-// Training: one CTA per row: the loss from the tiles' statistics, then u -> d in place (16 bytes per thread and step).
+// Training: the loss of a row from its tiles' statistics, then u -> d in place, two pieces of 16 bytes in flight per thread (4,096 rows of
+// 32,000 columns, one in flight: 110 us, 4.7 TB/s).  A row is cut over gridDim.y CTAs when there are few (13 rows: 11.6 us by one CTA each);
+// every one of them adds up the statistics, which are a hundredth of the row.
+template <typename T>
+__device__ __forceinline__ uint4 rows_vector(uint4 raw, int c, int64_t t, int V, float f, float at_target) {
+    constexpr int PER = 16 / sizeof(T);
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        float d = Cvt<T>::to(e[k]) * f;
+        if (c + k == t) d = at_target;
+        if (c + k >= V) d = 0.f;                                           // columns between V and the pitch meet zeros of w
+        e[k] = Cvt<T>::from(d);
+    }
+    return raw;
+}
 template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int tiles, int tile_cols, bool last) {
     extern __shared__ float fac[];                                        // [tiles] factor of a tile's columns
     __shared__ float red[32];
-    constexpr int PER = 16 / sizeof(T);
+    constexpr int PER = 16 / sizeof(T), STEP = ROW_THREADS * PER;
     const int row = blockIdx.x, rows = lce_active(a);
+    const int slice = (int)((a.ldu / PER + gridDim.y - 1) / gridDim.y) * PER, c0 = blockIdx.y * slice, c1 = min((int64_t)(c0 + slice), a.ldu);
     T* u = (T*)a.u + (int64_t)row * a.ldu;
     if (row < rows) {
         const float2* st = a.stats + (int64_t)row * tiles;
@@ -173,23 +189,16 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int ti
         for (int i = threadIdx.x; i < tiles; i += ROW_THREADS) { fac[i] = expf(fac[i] - top); sum += st[i].y * fac[i]; }
         const float others = block_total(sum, red);                       // without the target's column
         const int64_t t = a.target[row];
-        const float zt = a.z_target[row], et = expf(zt - top), inv = 1.f / (others + et);
-        if (threadIdx.x == 0) a.loss[row] = row_loss(top, others, et, zt);
-        for (int c = threadIdx.x * PER; c < a.ldu; c += ROW_THREADS * PER) {
-            uint4 raw = *reinterpret_cast<const uint4*>(u + c);
-            T* e = reinterpret_cast<T*>(&raw);
-            const float f = fac[c / tile_cols] * inv;                      // PER divides the tile's width
-#pragma unroll
-            for (int k = 0; k < PER; ++k) {
-                float d = Cvt<T>::to(e[k]) * f;
-                if (c + k == t) d = -others * inv * LceUnit<T>::value;
-                if (c + k >= a.V) d = 0.f;                                 // columns between V and the pitch meet zeros of w
-                e[k] = Cvt<T>::from(d);
-            }
-            *reinterpret_cast<uint4*>(u + c) = raw;
+        const float zt = a.z_target[row], et = expf(zt - top), inv = 1.f / (others + et), at_target = -others * inv * LceUnit<T>::value;
+        if (threadIdx.x == 0 && blockIdx.y == 0) a.loss[row] = row_loss(top, others, et, zt);
+        for (int c = c0 + threadIdx.x * PER; c < c1; c += 2 * STEP) {
+            const int c2 = c + STEP;
+            const uint4 x = *reinterpret_cast<const uint4*>(u + c), y = c2 < c1 ? *reinterpret_cast<const uint4*>(u + c2) : make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(u + c) = rows_vector<T>(x, c, t, a.V, fac[c / tile_cols] * inv, at_target);      // PER divides the tile's width
+            if (c2 < c1) *reinterpret_cast<uint4*>(u + c2) = rows_vector<T>(y, c2, t, a.V, fac[c2 / tile_cols] * inv, at_target);
         }
     } else if (row < (rows + 63) / 64 * 64) {                              // the products take rows in steps of 64
-        for (int c = threadIdx.x * PER; c < a.ldu; c += ROW_THREADS * PER) *reinterpret_cast<uint4*>(u + c) = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = c0 + threadIdx.x * PER; c < c1; c += STEP) *reinterpret_cast<uint4*>(u + c) = make_uint4(0u, 0u, 0u, 0u);
     }
     if (last) last_adds(a, red);
 }
@@ -214,7 +223,7 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_row_losses_kernel(LceArgs a, 
 }
 
 // ---- the counted rows
-constexpr int GATHER_ROWS = 32, COUNT_ROWS = 4096, GATHER_DIRECT = 16384;
+constexpr int GATHER_ROWS = 16, COUNT_ROWS = 4096, GATHER_DIRECT = 16384;
 __device__ __forceinline__ bool counted(int64_t t, int64_t ignore_index, int V) { return t != ignore_index && t >= 0 && t < V; }
 
 // blocks[b] = counted rows among [4096 b, 4096 (b + 1))
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(256) lce_count_kernel(const int64_t* __restric
     if (threadIdx.x == 0) { int s = 0; for (int i = 0; i < 8; ++i) s += sh[i]; blocks[blockIdx.x] = s; }
 }
 
-// A CTA moves the counted ones of 32 rows: it counts the rows before its own (all of them up to 16,384 rows, else those of the
+// A CTA moves the counted ones of 16 rows: it counts the rows before its own (all of them up to 16,384 rows, else those of the
 // 4,096-row block it lies in, on top of the blocks' counts), so the order is kept and no CTA waits for another.
 __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restrict__ x, int64_t pitch, const int64_t* __restrict__ target, int64_t ignore_index, int rows,
                                                          int V, int row_bytes, int vec, int* __restrict__ place, uint8_t* __restrict__ xc, int64_t* __restrict__ tc,
@@ -244,6 +253,7 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restri
         from = r0 / COUNT_ROWS * COUNT_ROWS;
         for (int i = threadIdx.x; i < r0 / COUNT_ROWS; i += 256) n += blocks[i];
     }
+#pragma unroll 8
     for (int r = from + threadIdx.x; r < r0; r += 256) n += counted(target[r], ignore_index, V) ? 1 : 0;
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) sh[warp] = n;
@@ -253,11 +263,13 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restri
         for (int i = 0; i < 8; ++i) b += sh[i];
         const int r = r0 + lane;
         const int64_t t = r < rows ? target[r] : -1;
-        const bool on = r < rows && counted(t, ignore_index, V);
+        const bool on = lane < GATHER_ROWS && r < rows && counted(t, ignore_index, V);
         const unsigned m = __ballot_sync(0xffffffffu, on);
         const int p = on ? b + __popc(m & ((1u << lane) - 1)) : -1;
-        to[lane] = p;
-        if (r < rows) place[r] = p;
+        if (lane < GATHER_ROWS) {
+            to[lane] = p;
+            if (r < rows) place[r] = p;
+        }
         if (on) tc[p] = t;
         if (lane == 0) base = b + __popc(m);
     }
@@ -267,8 +279,15 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restri
         if (p < 0) continue;
         const uint8_t* src = x + (int64_t)(r0 + i) * pitch;
         uint8_t* dst = xc + (int64_t)p * row_bytes;
-        if (vec) for (int c = lane * 16; c < row_bytes; c += 512) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-        else for (int c = lane * 2; c < row_bytes; c += 64) *reinterpret_cast<uint16_t*>(dst + c) = *reinterpret_cast<const uint16_t*>(src + c);
+        if (vec) {
+            for (int c = lane * 16; c < row_bytes; c += 8 * 512) {
+                uint4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) if (c + k * 512 < row_bytes) v[k] = *reinterpret_cast<const uint4*>(src + c + k * 512);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) if (c + k * 512 < row_bytes) *reinterpret_cast<uint4*>(dst + c + k * 512) = v[k];
+            }
+        } else for (int c = lane * 2; c < row_bytes; c += 64) *reinterpret_cast<uint16_t*>(dst + c) = *reinterpret_cast<const uint16_t*>(src + c);
     }
     if (blockIdx.x == gridDim.x - 1) {
         const int end = (base + 63) / 64 * 64 < rows ? (base + 63) / 64 * 64 : rows;
@@ -285,40 +304,42 @@ __global__ void __launch_bounds__(256) lce_add_parts_kernel(const float* __restr
     }
 }
 
-// A warp per row, eight columns (or one, where a row is not a whole number of eights) per lane and step
+// A warp per row and 32 x PER columns (PER = 8, or 1 where a row is not a whole number of eights), the parts four at a time
 template <typename T, int PER>
 __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* __restrict__ place, int rows, int D, int first, const float* __restrict__ early,
                                                           const float* __restrict__ part, int parts, int64_t row_pitch, const float* __restrict__ gout,
                                                           const float* __restrict__ inv, T* __restrict__ dx) {
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= rows) return;
+    const int pieces = (D + 32 * PER - 1) / (32 * PER), lane = threadIdx.x & 31;
+    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int row = (int)(item / pieces), c = (int)(item % pieces) * 32 * PER + lane * PER;
+    if (row >= rows || c >= D) return;
     const int p = place[row];
-    const float f = p >= 0 && p < first ? gout[0] * inv[0] / LceUnit<T>::value : 1.f;
-    for (int c = lane * PER; c < D; c += 32 * PER) {
-        float v[PER];
+    float v[PER];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) v[k] = 0.f;
-        if (p >= 0) {
-            const float* src = p < first ? early + (int64_t)p * D + c : part + (int64_t)(p - first) * D + c;
-            const int n = p < first ? 1 : parts;
-            for (int s = 0; s < n; ++s) {
-                const float* q = src + s * row_pitch * D;
-                if constexpr (PER == 8) {
-                    const float4 x = reinterpret_cast<const float4*>(q)[0], y = reinterpret_cast<const float4*>(q)[1];
-                    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-                } else v[0] += q[0];
-            }
+    for (int k = 0; k < PER; ++k) v[k] = 0.f;
+    if (p >= 0) {
+        const float* src = p < first ? early + (int64_t)p * D + c : part + (int64_t)(p - first) * D + c;
+        const int n = p < first ? 1 : parts;
+        const float f = p < first ? gout[0] * inv[0] / LceUnit<T>::value : 1.f;
+#pragma unroll 4
+        for (int s = 0; s < n; ++s) {
+            const float* q = src + s * row_pitch * D;
+            if constexpr (PER == 8) {
+                const float4 x = reinterpret_cast<const float4*>(q)[0], y = reinterpret_cast<const float4*>(q)[1];
+                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+            } else v[0] += q[0];
         }
-        T o[PER];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) o[k] = Cvt<T>::from(v[k] * f);
-        T* dst = dx + (int64_t)row * D + c;
-        if constexpr (PER == 8 && sizeof(T) == 2) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
-        else if constexpr (PER == 8) {
-            reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(o)[0];
-            reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(o)[1];
-        } else dst[0] = o[0];
+        for (int k = 0; k < PER; ++k) v[k] *= f;
     }
+    T o[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) o[k] = Cvt<T>::from(v[k]);
+    T* dst = dx + (int64_t)row * D + c;
+    if constexpr (PER == 8) {
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(T) / 2; ++k) reinterpret_cast<uint4*>(dst)[k] = reinterpret_cast<const uint4*>(o)[k];
+    } else dst[0] = o[0];
 }
 
 template <typename T> int logits(const LceArgs& a, cudaStream_t st) {
@@ -339,7 +360,8 @@ template <typename T> int rows(const LceArgs& a, int tile_cols, bool last, cudaS
     if (!once_per_device(done, current_device(), [] { return cudaFuncSetAttribute(lce_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) == cudaSuccess; }))
         return 2;
     if (smem > 200 * 1024) return 4;
-    lce_rows_kernel<T><<<a.rows, ROW_THREADS, smem, st>>>(a, tiles, tile_cols, last);
+    const int cut = a.rows >= 2 * device_sms() ? 1 : (2 * device_sms() + a.rows - 1) / a.rows;
+    lce_rows_kernel<T><<<dim3(a.rows, cut < 8 ? cut : 8), ROW_THREADS, smem, st>>>(a, tiles, tile_cols, last);
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
@@ -359,7 +381,8 @@ template <typename T>
 int scatter(const int* place, int rows, int D, int first, const float* early, const float* part, int parts, int64_t row_pitch, const float* gout, const float* inv,
             void* dx, cudaStream_t st) {
     count_launch();
-    const unsigned grid = (unsigned)((rows + 7) / 8);
+    const int cols = D % 8 == 0 ? 256 : 32;
+    const unsigned grid = (unsigned)(((int64_t)rows * ((D + cols - 1) / cols) + 7) / 8);
     if (D % 8 == 0) lce_scatter_kernel<T, 8><<<grid, 256, 0, st>>>(place, rows, D, first, early, part, parts, row_pitch, gout, inv, (T*)dx);
     else lce_scatter_kernel<T, 1><<<grid, 256, 0, st>>>(place, rows, D, first, early, part, parts, row_pitch, gout, inv, (T*)dx);
     return cudaGetLastError() == cudaSuccess ? 0 : 3;

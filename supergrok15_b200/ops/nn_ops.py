@@ -354,11 +354,16 @@ def attention_packed_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     return torch.cat(parts + [nothing(done, q.shape[0])]).to(dtype)
 
 
+def _gemm_err_flag(device: torch.device) -> torch.Tensor:
+    """The device word in which a kernel records a wait that ran out (``gemm.check`` raises for it)."""
+    from . import gemm
+    return gemm._err_flag(device)
+
+
 class _AttnPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, causal, scale):
-        from . import gemm as _gemm
-        out, rest, lse = _build.require().packed_attn_fwd(q, k, v, cu, causal, scale, True, _gemm._err_flag(q.device))
+        out, rest, lse = _build.require().packed_attn_fwd(q, k, v, cu, causal, scale, True, _gemm_err_flag(q.device))
         ctx.save_for_backward(q, k, v, cu, out, rest, lse)
         ctx.args = causal, scale
         return out
@@ -367,8 +372,7 @@ class _AttnPacked(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, cu, out, rest, lse = ctx.saved_tensors
-        from . import gemm as _gemm
-        return (*_build.require().packed_attn_bwd(q, k, v, cu, out, rest, lse, dout, *ctx.args, _gemm._err_flag(q.device)), None, None, None)
+        return (*_build.require().packed_attn_bwd(q, k, v, cu, out, rest, lse, dout, *ctx.args, _gemm_err_flag(q.device)), None, None, None)
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, causal: bool = True,
@@ -382,6 +386,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     are neither read nor counted: their output and their gradients are zero.  The offsets stay on the device (no host synchronisation, and a
     captured call follows offsets rewritten in place); offsets that do not ascend give undefined rows.  bf16, fp16 and fp32; head sizes up to
     128 on CUDA.  Sums, softmax statistics and gradient accumulators are fp32 and added in a fixed order."""
+    if q.is_cuda and _cpp_node(q, k, v, cu_seqlens):                     # checks its arguments like the lines below
+        return _build.require().packed_attn_node(q, k, v, cu_seqlens, causal, scale, _gemm_err_flag(q.device))
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"attention_packed: q [rows, heads, hd] and k, v [rows, kv_heads, hd] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
@@ -392,16 +398,9 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError("attention_packed: q, k and v need one dtype, and all tensors one device")
     if not q.is_cuda:
         return attention_packed_reference(q, k, v, cu_seqlens, causal, scale)
-    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32) or not 1 <= q.shape[2] <= 128:
-        raise ValueError(f"attention_packed: bf16, fp16 or fp32 with head sizes up to 128 on CUDA, got {q.dtype} with {q.shape[2]}")
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    cu = cu_seqlens.to(torch.int32).contiguous()
     q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
-    if _cpp_node(q, k, v):
-        train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-        from . import gemm as _gemm
-        return _build.require().packed_attn_node(q, k, v, cu, causal, scale, train, _gemm._err_flag(q.device))
-    return _AttnPacked.apply(q, k, v, cu, causal, scale)
+    return _AttnPacked.apply(q, k, v, cu_seqlens.to(torch.int32).contiguous(), causal, scale)
 
 
 def _native_ok(x: torch.Tensor) -> bool:
@@ -545,9 +544,8 @@ def linear_cross_entropy_reference(x: torch.Tensor, weight: torch.Tensor, target
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index):
-        from . import gemm as _gemm
         need = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        loss, *kept = _build.require().lce_fwd(x, weight, target, ignore_index, *need, _gemm._err_flag(x.device))
+        loss, *kept = _build.require().lce_fwd(x, weight, target, ignore_index, *need, _gemm_err_flag(x.device))
         ctx.save_for_backward(weight, *kept)
         ctx.args = x.shape, *need
         return loss
@@ -555,8 +553,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
-        from . import gemm as _gemm
-        return (*_build.require().lce_bwd(*ctx.saved_tensors, gout, *ctx.args, _gemm._err_flag(gout.device)), None, None)
+        return (*_build.require().lce_bwd(*ctx.saved_tensors, gout, *ctx.args, _gemm_err_flag(gout.device)), None, None)
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
@@ -568,6 +565,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     [rows, vocabulary] values exist at a time, in the type of ``x``; a pass with gradients takes the rows in pieces of that size, and from the
     second piece on holds the weight's gradient in fp32 between forward and backward.  The gradients' products of all pieces but the last
     are formed in the forward pass.  Sums are fp32 and added in a fixed order."""
+    if x.is_cuda and _cpp_node(x, weight, target):                       # checks its arguments like the lines below
+        return _build.require().lce_node(x, weight, target, ignore_index, _gemm_err_flag(x.device))
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or target.shape != x.shape[:-1] or 0 in weight.shape:
         raise ValueError(f"linear_cross_entropy: x [..., D], weight [vocabulary, D] and target [...] expected, got {tuple(x.shape)}, {tuple(weight.shape)}, "
                          f"{tuple(target.shape)}")
@@ -575,12 +574,6 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise ValueError("linear_cross_entropy: x and weight need one dtype, target int64, and all tensors one device")
     if not x.is_cuda:
         return linear_cross_entropy_reference(x, weight, target, ignore_index)
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise ValueError(f"linear_cross_entropy: bf16, fp16 or fp32 on CUDA, got {x.dtype}")
     x2, t = x.reshape(-1, x.shape[-1]), target.reshape(-1).contiguous()
     x2, w = (a if a.stride(1) == 1 else a.contiguous() for a in (x2, weight))
-    if _cpp_node(x2, w, t):
-        from . import gemm as _gemm
-        grad = torch.is_grad_enabled()
-        return _build.require().lce_node(x2, w, t, ignore_index, grad and x2.requires_grad, grad and w.requires_grad, _gemm._err_flag(x.device))
     return _LinearCrossEntropy.apply(x2, w, t, ignore_index)

@@ -196,6 +196,9 @@ def test_refusals():
         nn_ops.linear_cross_entropy(x, w, t.cpu())
     with pytest.raises(ValueError, match="bf16, fp16 or fp32"):
         nn_ops.linear_cross_entropy(x.double(), w.double(), t)
+    for args in ((x, w[0], t), (x, w[:, :8], t), (x, w, t[:9]), (x, w[:0], t), (x, w.double(), t), (x, w, t.int()), (x[None], w, t), (x[0, 0], w, t), (x, w[:, :0], t)):
+        with pytest.raises(ValueError, match="linear_cross_entropy"):
+            nn_ops.linear_cross_entropy(*args)
     loss = nn_ops.linear_cross_entropy(x.requires_grad_(True), w, t)
     with pytest.raises(RuntimeError, match="cannot be differentiated"):
         torch.autograd.grad(loss, x, create_graph=True)

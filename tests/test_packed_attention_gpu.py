@@ -203,6 +203,10 @@ def test_refusals():
         nn_ops.attention_packed(q.repeat(1, 1, 3), k.repeat(1, 1, 3), v.repeat(1, 1, 3), cu)
     with pytest.raises(ValueError, match="bf16, fp16 or fp32"):
         nn_ops.attention_packed(q.double(), k.double(), v.double(), cu)
+    for args in ((q[0], k, k, cu), (q, k, k[:, :1], cu), (q, k[:3], k[:3], cu), (q, k[..., :32], k[..., :32], cu), (q, k.repeat(1, 3, 1)[:, :3], k.repeat(1, 3, 1)[:, :3], cu),
+                 (q, k[:, :0], k[:, :0], cu), (q, k, k, cu[None]), (q, k, k, cu[:0]), (q, k, k, cu.float()), (q, k, k.half(), cu), (q[..., :0], k[..., :0], k[..., :0], cu)):
+        with pytest.raises(ValueError, match="attention_packed"):
+            nn_ops.attention_packed(*args)
     out = nn_ops.attention_packed(q.requires_grad_(True), k, v, cu)
     with pytest.raises(RuntimeError, match="cannot be differentiated"):
         torch.autograd.grad(out.sum(), q, create_graph=True)
