@@ -145,7 +145,7 @@ struct LceShape {
         p.x = (const char*)a.x + r0 * a.D * elem;
         p.target = a.target ? a.target + r0 : nullptr;
         p.loss = a.loss ? a.loss + r0 : nullptr;
-        return p;
+        return p;                                                         // u, stats, z_target and row_scale are those of any piece
     }
     int64_t last() const { return rows == 0 ? 0 : (rows - 1) / piece * piece; }      // first row of the last piece
 };
@@ -164,8 +164,9 @@ LceShape lce_shape(const Tensor& x, const Tensor& w, bool train) {
     return s;
 }
 
-// What a training pass keeps from forward to backward: the counted rows xc, where they came from (keep: [rows] places, then the count, the
-// counter of the row pass and 1 / count as a float), d of the last piece, and with several pieces fp32 dx and dw of the others.
+// What a training pass keeps from forward to backward: the counted rows xc (scaled where lce_scales_rows says so), where they came from (keep:
+// [rows] places, then the count, the counter of the row pass, 1 / count as a float and the last piece's row scales as floats), u or d of the
+// last piece, and with several pieces fp32 dx and dw of the others.
 enum { KEEP_COUNT = 0, KEEP_DONE = 1, KEEP_INV = 2, KEEP_MORE = 4 };
 
 // Returns (loss, xc, keep, d, dx of earlier pieces, dw of earlier pieces).  The gradient products of the last piece are left to the backward
@@ -190,7 +191,7 @@ std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w_, const Tensor& t, 
     const auto xo = x.options().memory_format(at::MemoryFormat::Contiguous);
     const Tensor none = at::empty({0}, fo);
     if (s.rows == 0) return {at::zeros({}, fo), none, none, none, none, none};
-    Tensor loss = at::empty({}, fo), xc = at::empty({s.rows, x.size(1)}, xo), keep = at::empty({s.rows + KEEP_MORE}, fo.dtype(at::kInt));
+    Tensor loss = at::empty({}, fo), xc = at::empty({s.rows, x.size(1)}, xo), keep = at::empty({s.rows + KEEP_MORE + (train ? s.piece : 0)}, fo.dtype(at::kInt));
     Tensor u = train ? at::empty({s.piece, s.a.ldu}, xo) : none, dx = none, dw = none;
     s.a.x = xc.data_ptr();
     const int64_t tiles = (s.a.V + sg::lce_tile_columns(s.dtype, s.a) - 1) / sg::lce_tile_columns(s.dtype, s.a), blocks = sg::lce_gather_blocks((int)s.rows);
@@ -209,6 +210,7 @@ std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w_, const Tensor& t, 
     s.a.out_loss = loss.data_ptr<float>();
     s.a.inv_count = reinterpret_cast<float*>(kept + KEEP_INV);
     s.a.done = reinterpret_cast<unsigned*>(kept + KEEP_DONE);
+    s.a.row_scale = train && sg::lce_scales_rows(s.dtype, s.a) ? reinterpret_cast<float*>(kept + KEEP_MORE) : nullptr;
     int rc = sg::lce_gather(s.dtype, x.data_ptr(), s.ldx, t.data_ptr<int64_t>(), ignore_index, (int)s.rows, s.a.V, s.a.D, keep.data_ptr<int>(), xc.data_ptr(), tc,
                             kept + KEEP_COUNT, s.a.done, reinterpret_cast<int*>(s.a.loss + s.rows), st);
     const int64_t last = s.last();
@@ -253,12 +255,13 @@ std::vector<Tensor> lce_bwd(const Tensor& w_, const Tensor& xc, const Tensor& ke
     if (need_w) dw = at::empty(w.sizes(), xo);
     const int64_t last = s.last();
     TORCH_CHECK(xc.is_contiguous() && xc.size(0) == rows && xc.size(1) == D && u.is_contiguous() && u.dim() == 2 && u.size(0) == s.piece && u.size(1) == s.a.ldu &&
-                u.scalar_type() == w.scalar_type() && keep.numel() == rows + KEEP_MORE && (!need_x || dx32.numel() == last * D) &&
+                u.scalar_type() == w.scalar_type() && keep.numel() == rows + KEEP_MORE + s.piece && (!need_x || dx32.numel() == last * D) &&
                 (!need_w || dw32.numel() == (last > 0 ? w.numel() : 0)), "linear_cross_entropy: not what the forward pass left");
-    const int* kept = keep.data_ptr<int>() + rows;
+    int* kept = keep.data_ptr<int>() + rows;
     s.a.x = xc.data_ptr();
     s.a.u = u.data_ptr();
     s.a.count = kept + KEEP_COUNT;
+    s.a.row_scale = sg::lce_scales_rows(s.dtype, s.a) ? reinterpret_cast<float*>(kept + KEEP_MORE) : nullptr;
     const sg::LceArgs a = s.at(last);
     sg::LceGrads g{};
     Tensor part;

@@ -18,7 +18,9 @@ struct LceArgs {
     int first, rows, V, D;
     void* u;                            // [rows, ldu], the type of x; null: no gradient is wanted
     int64_t ldu;                        // V rounded up to whole 16 bytes
-    float2* stats;                      // [rows][tiles]: maximum m of the row's logits in a tile of columns, sum of exp(z - m) without the target's column
+    float2* stats;                      // [rows][tiles]: reference r of the row's logits in a tile of columns (in powers of two), sum of 2^(z log2 e - r)
+                                        // without the target's column
+    float* row_scale;                   // [rows], bf16 on the tensor cores: what a row of u still has to be multiplied by; else null
     float* z_target;                    // [rows]: the target's logit
     float* loss;                        // [rows]
     // the last piece's row pass adds up: loss_all [all counted rows] -> out_loss = mean, inv_count = 1 / max(count, 1); done: a zero
@@ -44,6 +46,9 @@ struct LceGrads {
     bool f32_dw;                        // dw is fp32, else the type of x
     const float *gout, *inv_count;
 };
+
+// Whether lce_rows leaves u as it is and scales the rows of x instead (see linear_ce.cu): the references of nearly all tiles are equal
+bool lce_scales_rows(int dtype, const LceArgs& a);
 
 // u holds d times this: fp16 has no exponent to spare for probabilities (2^-17 for a flat row of 128,000 columns), bf16 and fp32 have
 template <typename T> struct LceUnit { static constexpr float value = 1.f; };

@@ -1,8 +1,8 @@
 // Products of the linear-head cross-entropy on the 5th-generation tensor cores (tcgen05 / TMEM / TMA), sm_100a only: 16-bit operands,
 // fp32 accumulators.  linear_ce.cu has the mathematics and the pass over the rows that stands between the two kernels.
 //
-//   LOGITS   z = x w^T, a tile of 128 rows x 256 columns at a time; the epilogue leaves maximum, sum and u = exp(z - max) of each row and
-//            half tile: the logits never reach memory
+//   LOGITS   z = x w^T, a tile of 128 rows x 256 columns at a time; the epilogue leaves reference, sum and u of each row and
+//            half tile (see linear_ce.cu): the logits never reach memory
 //   GRADS    dx = d w and dw = d^T x in one launch.  dx has few tiles with a long sum (the vocabulary), dw many with a short one; the long
 //            ones start first and are cut along the sum when one alone would take longer than everything spread over the SMs.  d, w and x are
 //            read where they are, in whichever order their rows run (K-major or MN-major descriptors).
@@ -52,7 +52,7 @@ struct LArgs {
     float* z_target;
     int store_u;
     // GRADS
-    const float* dw_prev;
+    const float *dw_prev, *row_scale;
     const float *gout, *inv;
     int splits, f32_w;                                                    // dx is left as fp32 sums of its splits; f32_w: dw is fp32
     int items_x;                                                          // items below this are dx
@@ -332,12 +332,15 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
 #pragma unroll
                             for (int i = 0; i < 32; ++i) if (n0 + c * 32 + i >= a.V) r[c][i] = __float_as_uint(-INFINITY);
                     }
-                    float mx = -FLT_MAX;
+                    float mx = -1e30f;                                    // finite, so that a row of -inf gives zeros, not NaN
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) mx = max3f(mx, __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
-                    const float mc = -mx * LOG2E;
+                    // the reference: the maximum (fp16), or a multiple of 64 powers of two that most tiles share (bf16)
+                    float ref = mx * LOG2E;
+                    if constexpr (Half2<T>::FMT == 1) ref = fabsf(ref) <= 64.f ? 0.f : 64.f * rintf(ref * (1.f / 64.f));
+                    const float mc = -ref;
                     float sum0 = 0.f, sum1 = 0.f;
                     auto chunk = [&](uint32_t (&rc)[32], int c) {         // 32 columns
                         uint32_t zt = 0u;
@@ -376,12 +379,13 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                         }
                     };
                     chunk(r[0], 0); chunk(r[1], 1); chunk(r[2], 2); chunk(r[3], 3);
-                    if (row < live) a.stats[(int64_t)row * ((a.V + 127) / 128) + n0 / 128] = make_float2(mx, sum0 + sum1);
+                    if (row < live) a.stats[(int64_t)row * ((a.V + 127) / 128) + n0 / 128] = make_float2(ref, sum0 + sum1);
                 }
             } else {
                 const bool is_x = w.kind == 1, f32 = is_x || a.f32_w;
                 const CUtensorMap* map = is_x ? &map_c1 : &map_c2;
                 const int tm = (a.rows + BM - 1) / BM, mrow = w.m0 + q * 32 + (is_x ? w.split * tm * BM : 0);      // partial sums of dx: [split][rows]
+                const float fr = is_x && a.row_scale && row < live ? f * a.row_scale[row] : f;
                 const float* prev = !is_x && a.dw_prev && row < a.V ? a.dw_prev + (int64_t)row * a.D : nullptr;
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                             }
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * fr);
                     if (f32) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k) put(k, make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]));
@@ -490,7 +494,7 @@ template <typename T, bool PAIR> int grads(const LceArgs& a, const LceGrads& g, 
     if (g.dx_part && !make_map(&cx, g.dx_part, g.parts * g.row_pitch, a.D, a.D, 32, 32, false)) return 10;
     if (g.dw && !make_map(&cw, g.dw, a.V, a.D, a.D, 32, g.f32_dw ? 32 : 64, !g.f32_dw)) return 10;
     LArgs k{};
-    k.dw_prev = g.dw_prev; k.splits = g.parts; k.f32_w = g.f32_dw; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err; k.count = a.count; k.first = a.first;
+    k.dw_prev = g.dw_prev; k.row_scale = a.row_scale; k.splits = g.parts; k.f32_w = g.f32_dw; k.rows = a.rows; k.V = a.V; k.D = a.D; k.err = err; k.count = a.count; k.first = a.first;
     k.gout = g.gout; k.inv = g.inv_count;
     k.items_x = g.dx_part ? g.parts * tm * tn : 0;
     const unsigned items = (unsigned)k.items_x + (g.dw ? (unsigned)((a.V + S::BM - 1) / S::BM) * (unsigned)tn : 0u);
