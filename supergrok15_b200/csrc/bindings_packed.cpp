@@ -136,13 +136,13 @@ Tensor loadable_rows(const Tensor& t) {
 struct LceShape {
     sg::LceArgs a{};
     int dtype = 0;
-    int64_t rows = 0, piece = 0, elem = 0, ldx = 0;
+    int64_t rows = 0, piece = 0, elem = 0;
     // the piece of the counted rows from r0 on (sized as if all rows were counted)
     sg::LceArgs at(int64_t r0) const {
         sg::LceArgs p = a;
         p.first = (int)r0;
         p.rows = (int)(rows - r0 < piece ? rows - r0 : piece);
-        p.x = (const char*)a.x + r0 * a.D * elem;
+        p.x = (const char*)a.x + r0 * a.ldx * elem;
         p.target = a.target ? a.target + r0 : nullptr;
         p.loss = a.loss ? a.loss + r0 : nullptr;
         return p;                                                         // u, stats, z_target and row_scale are those of any piece
@@ -150,16 +150,15 @@ struct LceShape {
     int64_t last() const { return rows == 0 ? 0 : (rows - 1) / piece * piece; }      // first row of the last piece
 };
 
-LceShape lce_shape(const Tensor& x, const Tensor& w, bool train) {
+LceShape lce_shape(int64_t rows, const Tensor& w, bool train) {
     LceShape s;
-    s.dtype = dtype_code(x);
-    s.elem = x.element_size();
-    s.rows = x.size(0);
-    s.ldx = x.stride(0);
+    s.dtype = dtype_code(w);
+    s.elem = w.element_size();
+    s.rows = rows;
     s.a.w = w.data_ptr(); s.a.ldw = w.stride(0);
     s.a.V = (int)w.size(0); s.a.D = (int)w.size(1);
-    const int64_t per = 16 / s.elem;
-    s.a.ldu = (w.size(0) + per - 1) / per * per;
+    s.a.ldx = sg::lce_pitch(w.size(1), s.elem);
+    s.a.ldu = sg::lce_pitch(w.size(0), s.elem);
     s.piece = lce_piece_rows(s.rows, s.a.ldu, s.elem, train);
     return s;
 }
@@ -185,13 +184,13 @@ std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w_, const Tensor& t, 
     const bool train = need_x || need_w;
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor w = loadable_rows(w_);
-    LceShape s = lce_shape(x, w, train);
+    LceShape s = lce_shape(x.size(0), w, train);
     auto st = at::cuda::getCurrentCUDAStream();
     const auto fo = x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
     const auto xo = x.options().memory_format(at::MemoryFormat::Contiguous);
     const Tensor none = at::empty({0}, fo);
     if (s.rows == 0) return {at::zeros({}, fo), none, none, none, none, none};
-    Tensor loss = at::empty({}, fo), xc = at::empty({s.rows, x.size(1)}, xo), keep = at::empty({s.rows + KEEP_MORE + (train ? s.piece : 0)}, fo.dtype(at::kInt));
+    Tensor loss = at::empty({}, fo), xc = at::empty({s.rows, s.a.ldx}, xo), keep = at::empty({s.rows + KEEP_MORE + (train ? s.piece : 0)}, fo.dtype(at::kInt));
     Tensor u = train ? at::empty({s.piece, s.a.ldu}, xo) : none, dx = none, dw = none;
     s.a.x = xc.data_ptr();
     const int64_t tiles = (s.a.V + sg::lce_tile_columns(s.dtype, s.a) - 1) / sg::lce_tile_columns(s.dtype, s.a), blocks = sg::lce_gather_blocks((int)s.rows);
@@ -211,7 +210,7 @@ std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w_, const Tensor& t, 
     s.a.inv_count = reinterpret_cast<float*>(kept + KEEP_INV);
     s.a.done = reinterpret_cast<unsigned*>(kept + KEEP_DONE);
     s.a.row_scale = train && sg::lce_scales_rows(s.dtype, s.a) ? reinterpret_cast<float*>(kept + KEEP_MORE) : nullptr;
-    int rc = sg::lce_gather(s.dtype, x.data_ptr(), s.ldx, t.data_ptr<int64_t>(), ignore_index, (int)s.rows, s.a.V, s.a.D, keep.data_ptr<int>(), xc.data_ptr(), tc,
+    int rc = sg::lce_gather(s.dtype, x.data_ptr(), x.stride(0), t.data_ptr<int64_t>(), ignore_index, (int)s.rows, s.a.V, s.a.D, keep.data_ptr<int>(), xc.data_ptr(), tc,
                             kept + KEEP_COUNT, s.a.done, reinterpret_cast<int*>(s.a.loss + s.rows), st);
     const int64_t last = s.last();
     if (train && last > 0 && need_x) dx = at::empty({last, x.size(1)}, fo);
@@ -249,12 +248,12 @@ std::vector<Tensor> lce_bwd(const Tensor& w_, const Tensor& xc, const Tensor& ke
     const int64_t rows = x_size[0], D = w_.size(1);
     if (rows == 0) return {need_x ? at::zeros(x_size, xo) : dx, need_w ? at::zeros(w_.sizes(), xo) : dw};
     const Tensor w = loadable_rows(w_);
-    LceShape s = lce_shape(xc, w, true);
+    LceShape s = lce_shape(rows, w, true);
     Tensor gout = gout_.to(at::kFloat).reshape({1}).contiguous();
     if (need_x) dx = at::empty(x_size, xo);
     if (need_w) dw = at::empty(w.sizes(), xo);
     const int64_t last = s.last();
-    TORCH_CHECK(xc.is_contiguous() && xc.size(0) == rows && xc.size(1) == D && u.is_contiguous() && u.dim() == 2 && u.size(0) == s.piece && u.size(1) == s.a.ldu &&
+    TORCH_CHECK(xc.is_contiguous() && xc.size(0) == rows && xc.size(1) == s.a.ldx && u.is_contiguous() && u.dim() == 2 && u.size(0) == s.piece && u.size(1) == s.a.ldu &&
                 u.scalar_type() == w.scalar_type() && keep.numel() == rows + KEEP_MORE + s.piece && (!need_x || dx32.numel() == last * D) &&
                 (!need_w || dw32.numel() == (last > 0 ? w.numel() : 0)), "linear_cross_entropy: not what the forward pass left");
     int* kept = keep.data_ptr<int>() + rows;

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(CTHREADS) lce_logits_kernel(LceArgs a) {
     const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, rows = lce_active(a);
     if (m0 >= rows) return;
     float s[4][4] = {};
-    tile_product<T, false, false>((const T*)a.x, a.D, (const T*)a.w, a.ldw, rows, a.V, a.D, m0, n0, s);
+    tile_product<T, false, false>((const T*)a.x, a.ldx, (const T*)a.w, a.ldw, rows, a.V, a.D, m0, n0, s);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int row = m0 + ty * 4 + i;
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(CTHREADS) lce_grad_kernel(LceArgs a, const flo
     const int M = AM ? a.V : rows;
     if (m0 >= M) return;
     float s[4][4] = {};
-    if (AM) tile_product<T, true, true>((const T*)a.u, a.ldu, (const T*)a.x, a.D, a.V, a.D, rows, m0, n0, s);
+    if (AM) tile_product<T, true, true>((const T*)a.u, a.ldu, (const T*)a.x, a.ldx, a.V, a.D, rows, m0, n0, s);
     else tile_product<T, false, true>((const T*)a.u, a.ldu, (const T*)a.w, a.ldw, rows, a.D, a.V, m0, n0, s);
     const float f = gout ? gout[0] * inv[0] / LceUnit<T>::value : 1.f;
 #pragma unroll
@@ -170,21 +170,14 @@ __device__ __forceinline__ void last_adds(const LceArgs& a, float* red) {
 // Training: the loss of a row from its tiles' statistics, then u -> d in place, two pieces of 16 bytes in flight per thread (4,096 rows of
 // 32,000 columns, one in flight: 110 us, 4.7 TB/s).  A row is cut over gridDim.y CTAs when there are few (13 rows: 11.6 us by one CTA each);
 // every one of them adds up the statistics, which are a hundredth of the row.
-template <typename T>
-__device__ __forceinline__ uint4 rows_vector(uint4 raw, int c, int64_t t, int V, float f, float at_target) {
-    constexpr int PER = 16 / sizeof(T);
+template <typename T> __device__ __forceinline__ uint4 scaled(uint4 raw, float f) {
     T* e = reinterpret_cast<T*>(&raw);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        float d = Cvt<T>::to(e[k]) * f;
-        if (c + k == t) d = at_target;
-        if (c + k >= V) d = 0.f;                                           // columns between V and the pitch meet zeros of w
-        e[k] = Cvt<T>::from(d);
-    }
+    for (int k = 0; k < 16 / (int)sizeof(T); ++k) e[k] = Cvt<T>::from(Cvt<T>::to(e[k]) * f);
     return raw;
 }
 template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int tiles, int tile_cols, bool last) {
+__global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int tiles, int tile_shift, bool last) {
     extern __shared__ float fac[];                                        // [tiles] factor of a tile's columns
     __shared__ float red[32];
     constexpr int PER = 16 / sizeof(T), STEP = ROW_THREADS * PER;
@@ -200,16 +193,19 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int ti
         float sum = 0.f;
         for (int i = threadIdx.x; i < tiles; i += ROW_THREADS) { fac[i] = exp2f(fac[i] - top); sum += st[i].y * fac[i]; }
         const float others = block_total(sum, red);                       // without the target's column
-        const int64_t t = a.target[row];
+        const int t = (int)a.target[row];
         const RowTerms rt = row_terms(top, others, a.z_target[row]);
         const float inv = 1.f / (others + rt.et), at_target = -others * inv * LceUnit<T>::value;
         if (threadIdx.x == 0 && blockIdx.y == 0) a.loss[row] = rt.loss;
-        for (int c = c0 + threadIdx.x * PER; c < c1; c += 2 * STEP) {
+        for (int c = c0 + threadIdx.x * PER; c < c1; c += 2 * STEP) {     // PER divides a tile's columns
             const int c2 = c + STEP;
             const uint4 x = *reinterpret_cast<const uint4*>(u + c), y = c2 < c1 ? *reinterpret_cast<const uint4*>(u + c2) : make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(u + c) = rows_vector<T>(x, c, t, a.V, fac[c / tile_cols] * inv, at_target);      // PER divides the tile's width
-            if (c2 < c1) *reinterpret_cast<uint4*>(u + c2) = rows_vector<T>(y, c2, t, a.V, fac[c2 / tile_cols] * inv, at_target);
+            *reinterpret_cast<uint4*>(u + c) = scaled<T>(x, fac[min(c >> tile_shift, tiles - 1)] * inv);
+            if (c2 < c1) *reinterpret_cast<uint4*>(u + c2) = scaled<T>(y, fac[min(c2 >> tile_shift, tiles - 1)] * inv);
         }
+        __syncthreads();
+        if (threadIdx.x == 0 && t >= c0 && t < c1) u[t] = Cvt<T>::from(at_target);
+        if (c1 > a.V) for (int c = max(c0, a.V) + (int)threadIdx.x; c < c1; c += ROW_THREADS) u[c] = Cvt<T>::from(0.f);      // columns between V and the pitch meet zeros of w
     } else if (row < (rows + 63) / 64 * 64) {                              // the products take rows in steps of 64
         for (int c = c0 + threadIdx.x * PER; c < c1; c += STEP) *reinterpret_cast<uint4*>(u + c) = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -267,7 +263,7 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_scale_rows_kernel(LceArgs a, 
             a.row_scale[row] = s;
             u[a.target[row]] = __float2bfloat16_rn(-sum);
         }
-        uint4* x = reinterpret_cast<uint4*>((__nv_bfloat16*)a.x + (int64_t)row * a.D);      // D is a multiple of 8 here
+        uint4* x = reinterpret_cast<uint4*>((__nv_bfloat16*)a.x + (int64_t)row * a.ldx);      // D is a multiple of 8 here
         for (int c = lane; c < a.D / 8; c += 32) {
             uint4 v = x[c];
             __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&v);
@@ -300,7 +296,7 @@ __global__ void __launch_bounds__(256) lce_count_kernel(const int64_t* __restric
 // A CTA moves the counted ones of 16 rows: it counts the rows before its own (all of them up to 16,384 rows, else those of the
 // 4,096-row block it lies in, on top of the blocks' counts), so the order is kept and no CTA waits for another.
 __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restrict__ x, int64_t pitch, const int64_t* __restrict__ target, int64_t ignore_index, int rows,
-                                                         int V, int row_bytes, int vec, int* __restrict__ place, uint8_t* __restrict__ xc, int64_t* __restrict__ tc,
+                                                         int V, int row_bytes, int row_pitch, int vec, int* __restrict__ place, uint8_t* __restrict__ xc, int64_t* __restrict__ tc,
                                                          int* __restrict__ count, unsigned* __restrict__ done, const int* __restrict__ blocks) {
     __shared__ int sh[8], base;
     __shared__ int to[GATHER_ROWS];
@@ -335,7 +331,7 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restri
         const int p = to[i];
         if (p < 0) continue;
         const uint8_t* src = x + (int64_t)(r0 + i) * pitch;
-        uint8_t* dst = xc + (int64_t)p * row_bytes;
+        uint8_t* dst = xc + (int64_t)p * row_pitch;
         if (vec) {
             for (int c = lane * 16; c < row_bytes; c += 8 * 512) {
                 uint4 v[8];
@@ -348,7 +344,7 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restri
     }
     if (blockIdx.x == gridDim.x - 1) {
         const int end = (base + 63) / 64 * 64 < rows ? (base + 63) / 64 * 64 : rows;
-        for (int64_t i = (int64_t)base * row_bytes + 2 * threadIdx.x; i < (int64_t)end * row_bytes; i += 512) *reinterpret_cast<uint16_t*>(xc + i) = 0;
+        for (int64_t i = (int64_t)base * row_pitch + 2 * threadIdx.x; i < (int64_t)end * row_pitch; i += 512) *reinterpret_cast<uint16_t*>(xc + i) = 0;
         if (threadIdx.x == 0) { *count = base; *done = 0u; }
     }
 }
@@ -422,7 +418,7 @@ template <typename T> int rows(const LceArgs& a, int tile_cols, bool last, cudaS
         return 2;
     if (smem > 200 * 1024) return 4;
     const int cut = a.rows >= 2 * device_sms() ? 1 : (2 * device_sms() + a.rows - 1) / a.rows;
-    lce_rows_kernel<T><<<dim3(a.rows, cut < 8 ? cut : 8), ROW_THREADS, smem, st>>>(a, tiles, tile_cols, last);
+    lce_rows_kernel<T><<<dim3(a.rows, cut < 8 ? cut : 8), ROW_THREADS, smem, st>>>(a, tiles, tile_cols == 128 ? 7 : 6, last);
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
@@ -469,7 +465,7 @@ int lce_gather(int dtype, const void* x, int64_t ldx, const int64_t* target, int
         lce_count_kernel<<<nb, 256, 0, st>>>(target, ignore_index, rows, V, blocks);
     }
     count_launch();
-    lce_gather_kernel<<<(rows + GATHER_ROWS - 1) / GATHER_ROWS, 256, 0, st>>>((const uint8_t*)x, ldx * es, target, ignore_index, rows, V, D * es, vec, place, (uint8_t*)xc, tc,
+    lce_gather_kernel<<<(rows + GATHER_ROWS - 1) / GATHER_ROWS, 256, 0, st>>>((const uint8_t*)x, ldx * es, target, ignore_index, rows, V, D * es, (int)lce_pitch(D, es) * es, vec, place, (uint8_t*)xc, tc,
                                                                             count, done, nb ? blocks : nullptr);
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }

@@ -12,12 +12,12 @@ namespace sg {
 // u is the only thing of the size [rows, vocabulary], and a piece is cut so that it stays below a fixed size.
 struct LceArgs {
     const void *x, *w;                  // [rows, D], the counted rows of this piece one after the other, and [V, D]; the last index is contiguous
-    int64_t ldw;                        // the rows of x are dense
+    int64_t ldx, ldw;                   // rows of x start on 128 bytes on the tensor cores (lce_pitch), so that a box of 64 columns is whole lines
     const int64_t* target;              // [rows], in [0, V)
     const int* count;                   // counted rows of all pieces; this one holds [first, first + rows) of them
     int first, rows, V, D;
     void* u;                            // [rows, ldu], the type of x; null: no gradient is wanted
-    int64_t ldu;                        // V rounded up to whole 16 bytes
+    int64_t ldu;                        // lce_pitch of V
     float2* stats;                      // [rows][tiles]: reference r of the row's logits in a tile of columns (in powers of two), sum of 2^(z log2 e - r)
                                         // without the target's column
     float* row_scale;                   // [rows], bf16 on the tensor cores: what a row of u still has to be multiplied by; else null
@@ -50,6 +50,9 @@ struct LceGrads {
 // Whether lce_rows leaves u as it is and scales the rows of x instead (see linear_ce.cu): the references of nearly all tiles are equal
 bool lce_scales_rows(int dtype, const LceArgs& a);
 
+// elements from row to row of what the operator lays out itself
+inline int64_t lce_pitch(int64_t n, int64_t elem) { const int64_t per = (elem == 2 ? 128 : 16) / elem; return (n + per - 1) / per * per; }
+
 // u holds d times this: fp16 has no exponent to spare for probabilities (2^-17 for a flat row of 128,000 columns), bf16 and fp32 have
 template <typename T> struct LceUnit { static constexpr float value = 1.f; };
 template <> struct LceUnit<__half> { static constexpr float value = 32768.f; };
@@ -61,7 +64,7 @@ int lce_dx_parts(int dtype, const LceArgs& a, bool with_dw, int64_t* row_pitch);
 
 // Return 0 or the number of the step that failed.
 // The counted rows in order: place[row] = where it went or -1, xc and tc = their rows of x (pitch ldx) and targets, count[0] = how many, done[0] = 0.
-// Rows of xc from the count to the next multiple of 64 are zero.  blocks: scratch of lce_gather_blocks(rows) ints.
+// xc has lce_pitch(D) elements per row; its rows from the count to the next multiple of 64 are zero.  blocks: scratch of lce_gather_blocks(rows) ints.
 int lce_gather_blocks(int rows);
 int lce_gather(int dtype, const void* x, int64_t ldx, const int64_t* target, int64_t ignore_index, int rows, int V, int D, int* place, void* xc, int64_t* tc,
                int* count, unsigned* done, int* blocks, cudaStream_t st);

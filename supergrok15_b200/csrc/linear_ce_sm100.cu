@@ -461,7 +461,7 @@ int launch(unsigned items, const CUtensorMap& a1, const CUtensorMap& b1, const C
 template <typename T, bool PAIR> int logits(const LceArgs& a, int* err, cudaStream_t st) {
     using S = Shape<PAIR>;
     CUtensorMap mx, mw, mu;
-    if (!make_map(&mx, a.x, a.rows, a.D, a.D, 128, BK, true) || !make_map(&mw, a.w, a.V, a.D, a.ldw, S::B_ROWS, BK, true)) return 10;
+    if (!make_map(&mx, a.x, a.rows, a.D, a.ldx, 128, BK, true) || !make_map(&mw, a.w, a.V, a.D, a.ldw, S::B_ROWS, BK, true)) return 10;
     if (a.u && !make_map(&mu, a.u, a.rows, a.ldu, a.ldu, 32, 64, true)) return 10;
     LArgs k{};
     k.target = a.target; k.stats = a.stats; k.z_target = a.z_target; k.count = a.count; k.first = a.first;
@@ -472,13 +472,14 @@ template <typename T, bool PAIR> int logits(const LceArgs& a, int* err, cudaStre
 
 bool in_pairs(int rows) { return rows > 128; }
 
-// Pieces that a tile of dx is cut into along the vocabulary: so many that one takes at most half of what a CTA (or pair) does on average.
-// A tile costs its 64-deep steps and about six more for its epilogue.
+// Pieces that a tile of dx is cut into along the vocabulary: so many that one takes about a quarter of what a CTA (or pair) does on average
+// (a half: 769 x 50,021 x 1,000 in 279 us, some pairs busy twice as long as the average; a quarter: 198).  A tile costs its 64-deep steps
+// and about six more for its epilogue.
 int dx_splits(int rows, int V, int D, bool with_dw) {
     const int64_t bm = in_pairs(rows) ? 256 : 128, teams = device_sms() / (bm / 128);
     const int64_t tn = (D + BN - 1) / BN, tx = (rows + bm - 1) / bm * tn, kx = (V + BK - 1) / BK, tw = with_dw ? (V + bm - 1) / bm * tn : 0, kw = (rows + BK - 1) / BK;
     const int64_t share = (tx * (kx + 6) + tw * (kw + 6)) / (teams > 0 ? teams : 1) + 1;
-    int64_t s = (2 * kx + share - 1) / share;
+    int64_t s = (4 * kx + share / 2) / share;
     if (s > kx / 8) s = kx / 8;                                           // eight steps at least, or the partial sums cost more than the products
     if (s > 64) s = 64;
     return s < 1 ? 1 : (int)s;
@@ -489,7 +490,7 @@ template <typename T, bool PAIR> int grads(const LceArgs& a, const LceGrads& g, 
     CUtensorMap ua, wb, cx, um, xb, cw;
     const int tm = (a.rows + S::BM - 1) / S::BM, tn = (a.D + BN - 1) / BN;
     if (!make_map(&ua, a.u, a.rows, a.V, a.ldu, 128, BK, true) || !make_map(&um, a.u, a.rows, a.V, a.ldu, BK, 64, true) ||
-        !make_map(&wb, a.w, a.V, a.D, a.ldw, BK, 64, true) || !make_map(&xb, a.x, a.rows, a.D, a.D, BK, 64, true)) return 10;
+        !make_map(&wb, a.w, a.V, a.D, a.ldw, BK, 64, true) || !make_map(&xb, a.x, a.rows, a.D, a.ldx, BK, 64, true)) return 10;
     cx = ua; cw = ua;
     if (g.dx_part && !make_map(&cx, g.dx_part, g.parts * g.row_pitch, a.D, a.D, 32, 32, false)) return 10;
     if (g.dw && !make_map(&cw, g.dw, a.V, a.D, a.D, 32, g.f32_dw ? 32 : 64, !g.f32_dw)) return 10;
@@ -505,7 +506,7 @@ template <typename T, bool PAIR> int grads(const LceArgs& a, const LceGrads& g, 
 
 bool lce_sm100_takes(int dtype, const LceArgs& a) {
     const auto ok = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld > 0 && ld % 8 == 0; };
-    return dtype != F32 && a.D % 8 == 0 && ok(a.x, a.D) && ok(a.w, a.ldw);
+    return dtype != F32 && a.D % 8 == 0 && ok(a.x, a.ldx) && ok(a.w, a.ldw);
 }
 int lce_sm100_dx_parts(int rows, int V, int D, bool with_dw, int64_t* row_pitch) {
     const int bm = in_pairs(rows) ? 256 : 128;
