@@ -24,6 +24,10 @@ using namespace tc;
 
 constexpr uint32_t HALF_TILE = 128 * 128;                                // [128 rows x 64 elements of 2 bytes] = 16 KB
 constexpr int STAGE_PITCH = 80;                                          // 64 bytes of a row and a pad: conflict-free 16-byte accesses
+template <uint32_t V> struct Const { static constexpr uint32_t v = V; };
+// descriptor step of the kk-th 16 columns of a K-major tile: 32 bytes inside a box of 64 columns, then the next box
+__device__ __forceinline__ constexpr uint32_t KSTEP(int kk) { return (uint32_t)(kk / 4) * (HALF_TILE >> 4) + 2u * (kk % 4); }
+
 // What the scheduling warp tells the others about an item.
 struct Item {
     int lo, hi, row0, head, kind;                                        // kind: 0 end of the work, 1 rows of a sequence, 2 rows of none
@@ -89,7 +93,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 9);
             mbar_init(&b->k_full[i], 1); mbar_init(&b->k_empty[i], 1); mbar_init(&b->v_full[i], 1); mbar_init(&b->v_empty[i], 1);
-            mbar_init(&b->s_full[i], 1); mbar_init(&b->p_full[i], 128); mbar_init(&b->o_done[i], 1); mbar_init(&b->o_empty[i], 128);
+            mbar_init(&b->s_full[i], 1); mbar_init(&b->p_full[i], 4); mbar_init(&b->o_done[i], 1); mbar_init(&b->o_empty[i], 4);
         }
         mbar_init(&b->clc, 1); mbar_init(&b->q_full, 1); mbar_init(&b->q_empty, 1); mbar_init(&b->v_tail, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -188,7 +192,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                 }
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&b->p_full[t]);
+                warp_arrive(&b->p_full[t]);
                 l = l * alpha + (sum0 + sum1);
             }
             if (!ok) break;
@@ -240,7 +244,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                 }
                 if (a.lse && lane < live) a.lse[(int64_t)w.head * a.seqs.total + row0 + lane] = n > 0 ? m_ref * a.scale + logf(l) : 0.f;
             }
-            if (n > 0) { tc_fence_before(); mbar_arrive(&b->o_empty[t]); }
+            if (n > 0) { tc_fence_before(); warp_arrive(&b->o_empty[t]); }
         }
     } else {
         reg_dec<REGS_OTHERS>();
@@ -310,52 +314,69 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                 mbar_arrive(&b->item_full[n_item & 1]);
             }
         } else if (warp == 9) {
-            if (lane == 0) {
+            {
                 const uint32_t idesc_qk = idesc_f16(Half2<T>::FMT, 128, 128, 0), idesc_pv = idesc_f16(Half2<T>::FMT, 128, (a.hd + 15) / 16 * 16, 1);
                 const int ksteps = (a.hd + 15) / 16;
+                const Desc dq = desc_of(make_desc_sw128(smem_u32(sQ))), dk = desc_of(make_desc_sw128(smem_u32(sK))),
+                           dv = desc_of(make_desc_sw128_mn(smem_u32(sV), HALF_TILE, 1024));
                 uint32_t n_item = 0, n_q = 0, n_k = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};
                 bool ok = true;
                 while (ok) {
                     const uint32_t si = n_item & 1;
-                    if (!mbar_wait(&b->item_full[si], (n_item >> 1) & 1)) { atomicExch(a.err, 67); break; }
+                    if (!warp_wait(&b->item_full[si], (n_item >> 1) & 1)) { if (lane == 0) atomicExch(a.err, 67); break; }
                     const Item w = b->item[si];
-                    mbar_arrive(&b->item_empty[si]);
+                    warp_arrive(&b->item_empty[si]);
                     ++n_item;
                     if (w.kind == 0) break;
                     if (w.kind == 2) continue;
                     const int nA = blocks(w, 0), nB = blocks(w, 1), n = nB > 0 ? nB : nA, lastt = nB > 0 ? 1 : 0;
-                    if (!mbar_wait(&b->q_full, n_q & 1)) { atomicExch(a.err, 68); ok = false; break; }
+                    if (!warp_wait(&b->q_full, n_q & 1)) { if (lane == 0) atomicExch(a.err, 68); ok = false; break; }
                     ++n_q;
-                    auto issue_qk = [&](int t, int j) {
-                        const uint32_t r = (n_k + j) & 1, q0 = smem_u32(sQ + t * TILE), k0 = smem_u32(sK + r * TILE);
-                        for (int kk = 0; kk < ksteps; ++kk)
-                            tc_mma_bf16(tmem + t * 128, make_desc_sw128(q0 + (kk / 4) * HALF_TILE) + 2 * (kk % 4), make_desc_sw128(k0 + (kk / 4) * HALF_TILE) + 2 * (kk % 4),
-                                        idesc_qk, kk > 0 ? 1u : 0u);
+                    // a product of 128 rows by 128 keys, issued by one lane; the ring slot is a constant in each of the two copies
+                auto qk = [&](int t, auto slot) {
+                    const uint32_t qa = dq.lo + t * (TILE >> 4), kb = dk.lo + slot.v * (TILE >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk)
+                        if (kk < ksteps) tc_mma_ss(tmem + t * 128, qa + KSTEP(kk), dq.hi, kb + KSTEP(kk), dk.hi, idesc_qk, kk > 0 ? 1u : 0u);
+                };
+                auto pv = [&](int t, auto slot, bool add) {
+                    const uint32_t vb = dv.lo + slot.v * (TILE >> 4), o = tmem + 256 + t * 128, pa = tmem + t * 128;
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) tc_mma_ts(o, pa + kk * 8, vb + kk * (2048 >> 4), dv.hi, idesc_pv, (kk > 0 || add) ? 1u : 0u);
+                };
+                auto issue_qk = [&](int t, int j) {
+                    const uint32_t r = (n_k + j) & 1;
+                    if (elect_one()) {
+                        if (t == 0) { if (r == 0) qk(0, Const<0>{}); else qk(0, Const<1>{}); }
+                        else { if (r == 0) qk(1, Const<0>{}); else qk(1, Const<1>{}); }
                         if (t == lastt) { tc_commit(&b->k_empty[r]); if (j + 1 == n) tc_commit(&b->q_empty); }
                         tc_commit(&b->s_full[t]);
-                    };
-                    auto issue_pv = [&](int t, int j, int nt) {
-                        const uint32_t r = (n_k + j) & 1, v0 = smem_u32(sV + r * TILE);
-    #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk)
-                            tc_mma_bf16_ta(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, make_desc_sw128_mn(v0 + kk * 2048, HALF_TILE, 1024), idesc_pv,
-                                           (j > 0 || kk > 0) ? 1u : 0u);
+                    }
+                    __syncwarp();
+                };
+                auto issue_pv = [&](int t, int j, int nt) {
+                    const uint32_t r = (n_k + j) & 1;
+                    if (elect_one()) {
+                        if (t == 0) { if (r == 0) pv(0, Const<0>{}, j > 0); else pv(0, Const<1>{}, j > 0); }
+                        else { if (r == 0) pv(1, Const<0>{}, j > 0); else pv(1, Const<1>{}, j > 0); }
                         if (t == lastt) tc_commit(&b->v_empty[r]);
                         if (j + 1 == nt) tc_commit(&b->o_done[t]);
-                    };
-                    if (!mbar_wait(&b->k_full[n_k & 1], (n_k >> 1) & 1)) { atomicExch(a.err, 69); ok = false; break; }
+                    }
+                    __syncwarp();
+                };
+                if (!warp_wait(&b->k_full[n_k & 1], (n_k >> 1) & 1)) { if (lane == 0) atomicExch(a.err, 69); ok = false; break; }
                     tc_fence_after();
                     issue_qk(0, 0);
                     if (nB > 0) issue_qk(1, 0);
                     for (int j = 0; j < n && ok; ++j) {
                         const uint32_t g = n_k + j;
-                        if (!mbar_wait(&b->v_full[g & 1], (g >> 1) & 1)) { atomicExch(a.err, 70); ok = false; break; }
-                        if (j + 1 < n && !mbar_wait(&b->k_full[(g + 1) & 1], ((g + 1) >> 1) & 1)) { atomicExch(a.err, 71); ok = false; break; }
+                        if (!warp_wait(&b->v_full[g & 1], (g >> 1) & 1)) { if (lane == 0) atomicExch(a.err, 70); ok = false; break; }
+                        if (j + 1 < n && !warp_wait(&b->k_full[(g + 1) & 1], ((g + 1) >> 1) & 1)) { if (lane == 0) atomicExch(a.err, 71); ok = false; break; }
                         for (int t = 0; t < 2 && ok; ++t) {
                             const int nt = t == 0 ? nA : nB;
                             if (j >= nt) continue;
-                            if (j == 0 && n_o[t] > 0 && !mbar_wait(&b->o_empty[t], (n_o[t] - 1) & 1)) { atomicExch(a.err, 72); ok = false; break; }
-                            if (!mbar_wait(&b->p_full[t], n_p[t] & 1)) { atomicExch(a.err, 73); ok = false; break; }
+                            if (j == 0 && n_o[t] > 0 && !warp_wait(&b->o_empty[t], (n_o[t] - 1) & 1)) { if (lane == 0) atomicExch(a.err, 72); ok = false; break; }
+                            if (!warp_wait(&b->p_full[t], n_p[t] & 1)) { if (lane == 0) atomicExch(a.err, 73); ok = false; break; }
                             ++n_p[t];
                             tc_fence_after();
                             issue_pv(t, j, nt);
@@ -385,11 +406,15 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
 //   KV = false: an item is 128 queries of a head (R = Q, dO); over its key tiles (T = K, V)
 //               X = S, Y = dP,  dQ += dS K
 // with P = exp(scale S - lse), dS = P (dP - delta); the factor scale of dS is applied once at the end.  The second operand of every
-// accumulating product is the tile that served as K-major operand of the first, read again through an MN-major descriptor.  Two groups of
-// 128 threads share a tile, a thread has one row and 64 columns; P and dS go back to tensor memory as 16-bit A operands.  The next tile's
-// X is issued as soon as this tile's scores have been taken out, its Y as soon as dS is stored, so the tensor cores work on dV and X
-// while the threads form dS, on dK and Y while they form the next P.
+// accumulating product is the tile that served as K-major operand of the first, read again through an MN-major descriptor.  Four groups of
+// 128 threads share a tile, a thread has one row and 32 columns; P and dS go back to tensor memory as 16-bit A operands, each group's into
+// columns that it alone has read.  The next tile's X is issued as soon as this tile's scores have been taken out, its Y as soon as dS is
+// stored, so the tensor cores work on dV and X while the threads form dS, on dK and Y while they form the next P.
+// Bound by the latency of that hand-over: with two groups (two warps per scheduler, 64 columns per thread) the tensor pipe was 46 % busy.
 // P and dS are rounded to 16 bits to be operands (half a step of each value); everything they come from and are added to is fp32.
+constexpr int BWD_THREADS = 640;
+constexpr int BWD_REGS = 104, BWD_REGS_OTHERS = 56;                       // 512 x 104 + 128 x 56 <= 640 x 96, the registers of the launch
+constexpr int BWD_PITCH = 48;                                             // 32 bytes of a row and a pad
 struct BwdBars {
     uint64_t item_full[2], item_empty[2], clc, res_full, res_empty, ring_full[2], ring_empty[2], tail, a_full, b_full, pa_full, pb_full, vec_full, done;
     uint4 answer;
@@ -407,7 +432,7 @@ struct BwdArgs {
 };
 
 template <typename T, int HD, bool KV>
-__global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                                                                           const __grid_constant__ BwdArgs a) {
     constexpr int HALVES = HD / 64;
@@ -421,19 +446,19 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
     float* s_lse = reinterpret_cast<float*>(sT1 + 2 * TILE);              // [2][128]  -lse * log2(e)
     float* s_del = s_lse + 256;                                           // [2][128]
     uint8_t* s_stage = reinterpret_cast<uint8_t*>(s_del + 256);
-    BwdBars* b = reinterpret_cast<BwdBars*>(s_stage + 8 * 32 * STAGE_PITCH);
+    BwdBars* b = reinterpret_cast<BwdBars*>(s_stage + 16 * 32 * BWD_PITCH);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n_heads = KV ? a.heads / a.group : a.heads;                 // heads of the items
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 9); mbar_init(&b->ring_full[i], 1); mbar_init(&b->ring_empty[i], 1);
+            mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 17); mbar_init(&b->ring_full[i], 1); mbar_init(&b->ring_empty[i], 1);
         }
         mbar_init(&b->clc, 1); mbar_init(&b->res_full, 1); mbar_init(&b->res_empty, 1); mbar_init(&b->tail, 1); mbar_init(&b->a_full, 1); mbar_init(&b->b_full, 1);
-        mbar_init(&b->pa_full, 256); mbar_init(&b->pb_full, 256); mbar_init(&b->vec_full, 256); mbar_init(&b->done, 1);
+        mbar_init(&b->pa_full, 16); mbar_init(&b->pb_full, 16); mbar_init(&b->vec_full, 8); mbar_init(&b->done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&b->tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -449,13 +474,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         return (w.hi - w.lo + 127) / 128 - first_tile(w);
     };
 
-    if (warp < 8) {
-        reg_inc<REGS_SOFTMAX>();
+    if (warp < 16) {
+        reg_inc<BWD_REGS>();
         const int q = warp & 3, g = warp >> 2, row = q * 32 + lane, tl = (int)threadIdx.x;
         const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
-        const uint32_t my_x = tm_x + lane_addr + g * 64, my_y = tm_y + lane_addr + g * 64;
+        const uint32_t my_x = tm_x + lane_addr + g * 32, my_y = tm_y + lane_addr + g * 32;
         const float c2 = a.scale * LOG2E;
-        uint8_t* stg = s_stage + warp * 32 * STAGE_PITCH;
+        uint8_t* stg = s_stage + warp * 32 * BWD_PITCH;
         uint32_t n_item = 0, n = 0, n_done = 0;
         bool ok = true;
         auto take = [&](Item& w) {
@@ -469,6 +494,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         };
         // KV: the per-query vectors of a tile, one value per thread (threads 0..127 -lse log2 e, 128..255 delta); queries past the end get
         // probability zero.  Else: both values of the thread's own query.
+        const bool carries = KV && tl < 256;
         auto fetch = [&](const Item& w, int h, int i) {
             const int r = w.lo + i * 128 + (tl & 127);
             if (r >= w.hi) return tl < 128 ? -INFINITY : 0.f;
@@ -478,7 +504,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         float v0 = 0.f, v1 = 0.f;
         auto fetch_first = [&](const Item& w) {
             if (w.kind != 1) return;
-            if (KV) v0 = fetch(w, w.head * a.group, first_tile(w));
+            if (KV) { if (carries) v0 = fetch(w, w.head * a.group, first_tile(w)); }
             else if (w.row0 + row < w.hi) {
                 const int64_t at = (int64_t)w.head * a.seqs.total + w.row0 + row;
                 v0 = a.lse[at]; v1 = a.delta[at];
@@ -490,9 +516,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         while (ok && w.kind != 0) {
             const int per_head = w.kind == 1 ? tiles(w) : 0, n_it = KV ? per_head * a.group : per_head;
             const float lse_row = v0 * LOG2E, del_row = v1;
-            if (KV && n_it > 0) {
+            if (carries && n_it > 0) {
                 (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = v0;    // buffer n & 1: every thread has left iteration n - 2
-                mbar_arrive(&b->vec_full);
+                warp_arrive(&b->vec_full);
             }
             int h = KV ? w.head * a.group : w.head, i = first_tile(w);
             const int i0 = i, i1 = i + per_head;
@@ -503,68 +529,63 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 const bool diag = a.causal && i == (KV ? i0 : i1 - 1);
                 const int see = KV ? 128 : w.hi - (w.lo + i * 128);      // keys of this tile that exist
                 if (++i == i1 && KV) { i = i0; ++h; }
-                if (KV && it + 1 < n_it) nx = fetch(w, h, i);
+                if (carries && it + 1 < n_it) nx = fetch(w, h, i);
                 if (KV && !warp_wait(&b->vec_full, n & 1)) { atomicExch(a.err, 82); ok = false; break; }
                 if (!warp_wait(&b->a_full, n & 1)) { atomicExch(a.err, 83); ok = false; break; }
                 tc_fence_after();
-                uint32_t r[2][32];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) tc_ld32(my_x + c * 32, r[c]);
+                uint32_t r[32];
+                tc_ld32(my_x, r);
                 tc_wait_ld();
-                if (!KV) { tc_fence_before(); mbar_arrive(&b->pa_full); }         // P stays in registers: X is free
+                if (!KV) { tc_fence_before(); warp_arrive(&b->pa_full); }         // P stays in registers: X is free
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int k = 0; k < 32; k += 4) {
-                        float4 nl = make_float4(-lse_row, -lse_row, -lse_row, -lse_row);
-                        if (KV) nl = *reinterpret_cast<const float4*>(s_lse + bs * 128 + g * 64 + c * 32 + k);
-                        float e0, e1, e2, e3;
-                        fma2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1]), c2, c2, nl.x, nl.y, e0, e1);
-                        fma2(__uint_as_float(r[c][k + 2]), __uint_as_float(r[c][k + 3]), c2, c2, nl.z, nl.w, e2, e3);
-                        r[c][k] = __float_as_uint(ex2f(e0)); r[c][k + 1] = __float_as_uint(ex2f(e1));
-                        r[c][k + 2] = __float_as_uint(ex2f(e2)); r[c][k + 3] = __float_as_uint(ex2f(e3));
-                    }
+                for (int k = 0; k < 32; k += 4) {
+                    float4 nl = make_float4(-lse_row, -lse_row, -lse_row, -lse_row);
+                    if (KV) nl = *reinterpret_cast<const float4*>(s_lse + bs * 128 + g * 32 + k);
+                    float e0, e1, e2, e3;
+                    fma2(__uint_as_float(r[k]), __uint_as_float(r[k + 1]), c2, c2, nl.x, nl.y, e0, e1);
+                    fma2(__uint_as_float(r[k + 2]), __uint_as_float(r[k + 3]), c2, c2, nl.z, nl.w, e2, e3);
+                    r[k] = __float_as_uint(ex2f(e0)); r[k + 1] = __float_as_uint(ex2f(e1));
+                    r[k + 2] = __float_as_uint(ex2f(e2)); r[k + 3] = __float_as_uint(ex2f(e3));
+                }
                 if (diag || see < 128) {
                     // KV: key `row` is seen by the queries (columns) from the diagonal on; else query `row` sees the keys up to it, and those
                     // that exist
-                    const int from = KV ? row - g * 64 : 0, to = KV ? 64 : (diag ? row + 1 : see) - g * 64;
+                    const int from = KV ? row - g * 32 : 0, to = KV ? 32 : (diag ? row + 1 : see) - g * 32;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) if (c * 32 + k < from || c * 32 + k >= to) r[c][k] = 0u;
+                    for (int k = 0; k < 32; ++k) if (k < from || k >= to) r[k] = 0u;
                 }
-                uint32_t d[2][32];                                       // dP; d[0] also takes the packed operands, in place
+                uint32_t d[32];                                          // dP; its first half also takes the packed operands, in place
                 if (KV) {
+                    uint32_t pk[16];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) d[0][k] = Half2<T>::pack(__uint_as_float(r[k >> 4][(2 * k) & 31]), __uint_as_float(r[k >> 4][(2 * k + 1) & 31]));
-                    tc_st32(my_x, d[0]);
+                    for (int k = 0; k < 16; ++k) pk[k] = Half2<T>::pack(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1]));
+                    tc_st16(my_x, pk);
                     tc_wait_st();
                     tc_fence_before();
-                    mbar_arrive(&b->pa_full);
+                    warp_arrive(&b->pa_full);
                 }
                 if (!warp_wait(&b->b_full, n & 1)) { atomicExch(a.err, 84); ok = false; break; }
                 tc_fence_after();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) tc_ld32(my_y + c * 32, d[c]);
+                tc_ld32(my_y, d);
                 tc_wait_ld();
+                uint32_t pk[16];
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {                         // columns 2k .. 2k+3 of this group
+                for (int k = 0; k < 32; k += 4) {
                     float4 de = make_float4(del_row, del_row, del_row, del_row);
-                    if (KV) de = *reinterpret_cast<const float4*>(s_del + bs * 128 + g * 64 + 2 * k);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int c = k >> 4, k0 = (2 * k + 2 * u) & 31;
-                        float t0, t1, s0, s1;
-                        fma2(u ? de.z : de.x, u ? de.w : de.y, -1.f, -1.f, __uint_as_float(d[c][k0]), __uint_as_float(d[c][k0 + 1]), t0, t1);   // dP - delta
-                        fma2(__uint_as_float(r[c][k0]), __uint_as_float(r[c][k0 + 1]), t0, t1, 0.f, 0.f, s0, s1);
-                        d[0][k + u] = Half2<T>::pack(s0, s1);             // its own columns or ones already used
-                    }
+                    if (KV) de = *reinterpret_cast<const float4*>(s_del + bs * 128 + g * 32 + k);
+                    float t0, t1, t2, t3;
+                    fma2(de.x, de.y, -1.f, -1.f, __uint_as_float(d[k]), __uint_as_float(d[k + 1]), t0, t1);               // dP - delta
+                    fma2(de.z, de.w, -1.f, -1.f, __uint_as_float(d[k + 2]), __uint_as_float(d[k + 3]), t2, t3);
+                    fma2(__uint_as_float(r[k]), __uint_as_float(r[k + 1]), t0, t1, 0.f, 0.f, t0, t1);
+                    fma2(__uint_as_float(r[k + 2]), __uint_as_float(r[k + 3]), t2, t3, 0.f, 0.f, t2, t3);
+                    pk[k / 2] = Half2<T>::pack(t0, t1);
+                    pk[k / 2 + 1] = Half2<T>::pack(t2, t3);
                 }
-                tc_st32(my_y, d[0]);                                      // this group alone has read these columns
+                tc_st16(my_y, pk);                                        // this group alone has read these columns
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&b->pb_full);
-                if (KV && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = nx; mbar_arrive(&b->vec_full); }
+                warp_arrive(&b->pb_full);
+                if (carries && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = nx; warp_arrive(&b->vec_full); }
             }
             if (!ok) break;
             const Item cur = w;
@@ -576,14 +597,16 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 ++n_done;
                 tc_fence_after();
             }
-            // KV: group 0 writes dV, group 1 dK; else each group writes half of the columns of dQ.  Rows of no sequence: zeros
+            // KV: groups 0 and 1 write dV, 2 and 3 dK, each half of the columns; else each group writes a quarter of dQ (HD = 64: two of them
+            // half).  Rows of no sequence: zeros
             const int row0 = cur.row0 + q * 32, live = cur.hi - row0;
             if (live > 0) {
                 const int64_t ld = (int64_t)n_heads * a.hd;
-                T* base = (T*)(KV && g == 1 ? a.out1 : a.out0) + (int64_t)row0 * ld + (int64_t)cur.head * a.hd;
-                const float f = KV && g == 0 ? 1.f : a.scale;
-                const uint32_t acc = (KV && g == 1 ? tm_acc1 : tm_acc0) + lane_addr;
-                const int c0 = KV ? 0 : g * (HD / 64), c1 = KV ? HD / 32 : c0 + HD / 64;
+                const bool second = KV && g >= 2;
+                T* base = (T*)(second ? a.out1 : a.out0) + (int64_t)row0 * ld + (int64_t)cur.head * a.hd;
+                const float f = KV && !second ? 1.f : a.scale;
+                const uint32_t acc = (second ? tm_acc1 : tm_acc0) + lane_addr;
+                const int c0 = KV ? (g & 1) * (HD / 64) : g, c1 = KV ? c0 + HD / 64 : (g < HD / 32 ? g + 1 : g);
 #pragma unroll 1
                 for (int c = c0; c < c1; ++c) {
                     uint32_t t[32];
@@ -595,27 +618,30 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                         for (int k = 0; k < 32; ++k) t[k] = 0u;
                     }
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        uint32_t pk[4];
+                    for (int half = 0; half < 2; ++half) {                // 16 columns at a time, two lanes store 32 consecutive bytes of a row
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) pk[e] = Half2<T>::pack(__uint_as_float(t[8 * u + 2 * e]) * f, __uint_as_float(t[8 * u + 2 * e + 1]) * f);
-                        *reinterpret_cast<uint4*>(stg + lane * STAGE_PITCH + u * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                    }
-                    __syncwarp();
+                        for (int u = 2 * half; u < 2 * half + 2; ++u) {
+                            uint32_t pk[4];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int rr = u * 8 + (lane >> 2), piece = lane & 3;
-                        if (rr < live && c * 32 + piece * 8 < a.hd)
-                            *reinterpret_cast<uint4*>(base + rr * ld + c * 32 + piece * 8) = *reinterpret_cast<const uint4*>(stg + rr * STAGE_PITCH + piece * 16);
+                            for (int e = 0; e < 4; ++e) pk[e] = Half2<T>::pack(__uint_as_float(t[8 * u + 2 * e]) * f, __uint_as_float(t[8 * u + 2 * e + 1]) * f);
+                            *reinterpret_cast<uint4*>(stg + lane * BWD_PITCH + (u & 1) * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int rr = u * 16 + (lane >> 1), col = c * 32 + half * 16 + (lane & 1) * 8;
+                            if (rr < live && col < a.hd)
+                                *reinterpret_cast<uint4*>(base + rr * ld + col) = *reinterpret_cast<const uint4*>(stg + rr * BWD_PITCH + (lane & 1) * 16);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
             tc_fence_before();                                            // the accumulators have been read: the next item's products wait for this
         }                                                                 // group's pa_full / pb_full
     } else {
-        reg_dec<REGS_OTHERS>();
-        if (warp == 8) {
+        reg_dec<BWD_REGS_OTHERS>();
+        if (warp == 16) {
             int item = (int)blockIdx.x;
             uint32_t n_item = 0, n_clc = 0, n_res = 0, n = 0, n_tail = 0;
             bool ok = true, more = true;
@@ -684,39 +710,49 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 b->item[n_item & 1].kind = 0;
                 mbar_arrive(&b->item_full[n_item & 1]);
             }
-        } else if (warp == 9 && lane == 0) {
+        } else if (warp == 17) {
             const uint32_t idesc_first = idesc_f16(Half2<T>::FMT, 128, 128, 0), idesc_acc = idesc_f16(Half2<T>::FMT, 128, (a.hd + 15) / 16 * 16, 1);
             const int ksteps = (a.hd + 15) / 16;
             uint32_t n_item = 0, n_res = 0;
             // iterations of the next item; 0 at the end of the work, -1 when a wait ran out, -2 for rows of no sequence
             auto take = [&]() {
                 const uint32_t si = n_item & 1;
-                if (!mbar_wait(&b->item_full[si], (n_item >> 1) & 1)) { atomicExch(a.err, 91); return -1; }
+                if (!warp_wait(&b->item_full[si], (n_item >> 1) & 1)) { if (lane == 0) atomicExch(a.err, 91); return -1; }
                 const Item w = b->item[si];
-                mbar_arrive(&b->item_empty[si]);
+                warp_arrive(&b->item_empty[si]);
                 ++n_item;
                 if (w.kind != 1) return w.kind == 0 ? 0 : -2;
                 return KV ? tiles(w) * a.group : tiles(w);
             };
-            auto first_product = [&](uint32_t tm, const uint8_t* res, const uint8_t* ring) {
-                const uint32_t r0 = smem_u32(res), t0 = smem_u32(ring);
-                for (int kk = 0; kk < ksteps; ++kk)
-                    tc_mma_bf16(tm, make_desc_sw128(r0 + (kk / 4) * HALF_TILE) + 2 * (kk % 4), make_desc_sw128(t0 + (kk / 4) * HALF_TILE) + 2 * (kk % 4), idesc_first,
-                                kk > 0 ? 1u : 0u);
+            const Desc r0 = desc_of(make_desc_sw128(smem_u32(sR0))), r1 = desc_of(make_desc_sw128(smem_u32(sR1))), t0 = desc_of(make_desc_sw128(smem_u32(sT0))),
+                       t1 = desc_of(make_desc_sw128(smem_u32(sT1))), m0 = desc_of(make_desc_sw128_mn(smem_u32(sT0), HALF_TILE, 1024)),
+                       m1 = desc_of(make_desc_sw128_mn(smem_u32(sT1), HALF_TILE, 1024));
+            // X or Y = R T^T of ring slot `slot` (a constant in each of its two copies)
+            auto first_copy = [&](uint32_t tm, const Desc& res, const Desc& ring, auto slot) {
+                const uint32_t rb = ring.lo + slot.v * (TILE >> 4);
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk)
+                    if (kk < ksteps) tc_mma_ss(tm, res.lo + KSTEP(kk), res.hi, rb + KSTEP(kk), ring.hi, idesc_first, kk > 0 ? 1u : 0u);
             };
-            // acc += A T, A the 16-bit operand in the columns of X or Y (its second half starts at column 64), T a ring tile read MN-major
-            auto acc_product = [&](uint32_t acc, uint32_t tm, const uint8_t* ring, bool add) {
-                const uint32_t t0 = smem_u32(ring);
+            auto first_product = [&](uint32_t tm, const Desc& res, const Desc& ring, uint32_t slot) {
+                if (slot == 0) first_copy(tm, res, ring, Const<0>{}); else first_copy(tm, res, ring, Const<1>{});
+            };
+            // acc += A T, A the 16-bit operand in the columns of X or Y (32 of its columns in the first half of 32), T a ring tile read MN-major
+            auto acc_copy = [&](uint32_t acc, uint32_t tm, const Desc& ring, auto slot, bool add) {
+                const uint32_t rb = ring.lo + slot.v * (TILE >> 4);
 #pragma unroll
                 for (int kk = 0; kk < 8; ++kk)
-                    tc_mma_bf16_ta(acc, tm + (kk >> 2) * 64 + (kk & 3) * 8, make_desc_sw128_mn(t0 + kk * 2048, HALF_TILE, 1024), idesc_acc, (add || kk > 0) ? 1u : 0u);
+                    tc_mma_ts(acc, tm + (kk >> 1) * 32 + (kk & 1) * 8, rb + kk * (2048 >> 4), ring.hi, idesc_acc, (kk > 0 || add) ? 1u : 0u);
+            };
+            auto acc_product = [&](uint32_t acc, uint32_t tm, const Desc& ring, uint32_t slot, bool add) {
+                if (slot == 0) acc_copy(acc, tm, ring, Const<0>{}, add); else acc_copy(acc, tm, ring, Const<1>{}, add);
             };
             auto tiles_ready = [&](uint32_t n, bool first_it) {
                 if (first_it) {
-                    if (!mbar_wait(&b->res_full, n_res & 1)) { atomicExch(a.err, 92); return false; }
+                    if (!warp_wait(&b->res_full, n_res & 1)) { if (lane == 0) atomicExch(a.err, 92); return false; }
                     ++n_res;
                 }
-                if (!mbar_wait(&b->ring_full[n & 1], (n >> 1) & 1)) { atomicExch(a.err, 93); return false; }
+                if (!warp_wait(&b->ring_full[n & 1], (n >> 1) & 1)) { if (lane == 0) atomicExch(a.err, 93); return false; }
                 tc_fence_after();
                 return true;
             };
@@ -727,11 +763,14 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                     do n_it = take(); while (n_it == -2);
                     if (n_it <= 0) break;
                     if (!tiles_ready(n, true)) break;
-                    first_product(tm_x, sR0, sT0 + (n & 1) * TILE);
-                    tc_commit(&b->a_full);
-                    first_product(tm_y, sR1, sT1 + (n & 1) * TILE);
-                    tc_commit(&b->b_full);
-                    if (n_it == 1) tc_commit(&b->res_empty);
+                    if (elect_one()) {
+                        first_product(tm_x, r0, t0, n & 1);
+                        tc_commit(&b->a_full);
+                        first_product(tm_y, r1, t1, n & 1);
+                        tc_commit(&b->b_full);
+                        if (n_it == 1) tc_commit(&b->res_empty);
+                    }
+                    __syncwarp();
                 }
                 int n_next = 0;
                 for (int it = 0; it < n_it; ++it, ++n) {
@@ -740,24 +779,31 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                     // one item ahead, no further: the other warps take the item behind it only when this one is done
                     if (last) { n_next = take(); if (n_next == -1) { ok = false; break; } }
                     const bool next = !last || n_next > 0;
-                    if (!mbar_wait(&b->pa_full, n & 1)) { atomicExch(a.err, 94); ok = false; break; }
+                    if (!warp_wait(&b->pa_full, n & 1)) { if (lane == 0) atomicExch(a.err, 94); ok = false; break; }
                     tc_fence_after();
-                    if (KV) acc_product(tm_acc0, tm_x, sT1 + s * TILE, it > 0);                          // dV += P^T dO
+                    if (KV && elect_one()) acc_product(tm_acc0, tm_x, m1, s, it > 0);                    // dV += P^T dO
+                    __syncwarp();
                     if (next) {
                         if (!tiles_ready(n + 1, last)) { ok = false; break; }
-                        first_product(tm_x, sR0, sT0 + ns * TILE);
-                        tc_commit(&b->a_full);
+                        if (elect_one()) {
+                            first_product(tm_x, r0, t0, ns);
+                            tc_commit(&b->a_full);
+                        }
+                        __syncwarp();
                     }
-                    if (!mbar_wait(&b->pb_full, n & 1)) { atomicExch(a.err, 95); ok = false; break; }
+                    if (!warp_wait(&b->pb_full, n & 1)) { if (lane == 0) atomicExch(a.err, 95); ok = false; break; }
                     tc_fence_after();
-                    acc_product(KV ? tm_acc1 : tm_acc0, tm_y, sT0 + s * TILE, it > 0);                   // dK += dS^T Q / dQ += dS K
-                    tc_commit(&b->ring_empty[s]);
-                    if (last) tc_commit(&b->done);
-                    if (next) {
-                        first_product(tm_y, sR1, sT1 + ns * TILE);
-                        tc_commit(&b->b_full);
-                        if (last ? n_next == 1 : it + 2 == n_it) tc_commit(&b->res_empty);               // the last first products of their item
+                    if (elect_one()) {
+                        acc_product(KV ? tm_acc1 : tm_acc0, tm_y, m0, s, it > 0);                        // dK += dS^T Q / dQ += dS K
+                        tc_commit(&b->ring_empty[s]);
+                        if (last) tc_commit(&b->done);
+                        if (next) {
+                            first_product(tm_y, r1, t1, ns);
+                            tc_commit(&b->b_full);
+                            if (last ? n_next == 1 : it + 2 == n_it) tc_commit(&b->res_empty);           // the last first products of their item
+                        }
                     }
+                    __syncwarp();
                 }
                 n_it = n_next;
             }
@@ -765,7 +811,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_bwd_sm100_kernel(const 
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 17) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
@@ -818,7 +864,7 @@ template <typename T, int HD> int bwd(const PackedAttn& p, int* err, cudaStream_
     const int hk = p.heads / p.group;
     if (!head_map(&mq, p.q, p, p.heads, p.q_ld, p.q_hs) || !head_map(&mk, p.k, p, hk, p.k_ld, p.k_hs) || !head_map(&mv, p.v, p, hk, p.v_ld, p.v_hs) ||
         !head_map(&md, p.dout, p, p.heads, (int64_t)p.heads * p.hd, p.hd)) return 10;
-    constexpr size_t smem = 6 * (HD / 64) * HALF_TILE + 2048 + 8 * 32 * STAGE_PITCH + sizeof(BwdBars) + 1024;
+    constexpr size_t smem = 6 * (HD / 64) * HALF_TILE + 2048 + 16 * 32 * BWD_PITCH + sizeof(BwdBars) + 1024;
     static std::atomic<uint64_t> done{0};
     if (!once_per_device(done, current_device(), [&] {
             return cudaFuncSetAttribute(packed_bwd_sm100_kernel<T, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
@@ -829,9 +875,9 @@ template <typename T, int HD> int bwd(const PackedAttn& p, int* err, cudaStream_
     BwdArgs a{p.lse, p.delta, p.dv, p.dk, p.seqs, p.heads, p.group, p.hd, p.causal, slots, p.scale, err};
     count_launch(3);
     packed_delta_sm100_kernel<T, LANES><<<(unsigned)(((int64_t)p.seqs.total * p.heads * LANES + 255) / 256), 256, 0, st>>>(p);
-    packed_bwd_sm100_kernel<T, HD, true><<<(unsigned)slots * (unsigned)hk, FWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
+    packed_bwd_sm100_kernel<T, HD, true><<<(unsigned)slots * (unsigned)hk, BWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
     a.out0 = p.dq; a.out1 = nullptr;
-    packed_bwd_sm100_kernel<T, HD, false><<<(unsigned)slots * (unsigned)p.heads, FWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
+    packed_bwd_sm100_kernel<T, HD, false><<<(unsigned)slots * (unsigned)p.heads, BWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
     return cudaGetLastError() == cudaSuccess ? 0 : 12;
 }
 
