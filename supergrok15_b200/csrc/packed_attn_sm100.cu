@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = b->tmem_slot;                                   // tile t: S / P at 128 t, O at 256 + 128 t
+    // all 512 columns are allocated, so they start at 0: a constant keeps address arithmetic out of the loops.  Tile t: S / P at 128 t, O at 256 + 128 t
+    constexpr uint32_t tmem = 0;
 
     // key tiles that tile t of an item meets
     auto blocks = [&](const Item& w, int t) {
@@ -335,9 +336,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                     // a product of 128 rows by 128 keys, issued by one lane; the ring slot is a constant in each of the two copies
                 auto qk = [&](int t, auto slot) {
                     const uint32_t qa = dq.lo + t * (TILE >> 4), kb = dk.lo + slot.v * (TILE >> 4);
+                    if (ksteps == HD / 16) {
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk)
-                        if (kk < ksteps) tc_mma_ss(tmem + t * 128, qa + KSTEP(kk), dq.hi, kb + KSTEP(kk), dk.hi, idesc_qk, kk > 0 ? 1u : 0u);
+                        for (int kk = 0; kk < HD / 16; ++kk) tc_mma_ss(tmem + t * 128, qa + KSTEP(kk), dq.hi, kb + KSTEP(kk), dk.hi, idesc_qk, kk > 0 ? 1u : 0u);
+                    } else
+#pragma unroll 1
+                        for (int kk = 0; kk < ksteps; ++kk) tc_mma_ss(tmem + t * 128, qa + KSTEP(kk), dq.hi, kb + KSTEP(kk), dk.hi, idesc_qk, kk > 0 ? 1u : 0u);
                 };
                 auto pv = [&](int t, auto slot, bool add) {
                     const uint32_t vb = dv.lo + slot.v * (TILE >> 4), o = tmem + 256 + t * 128, pa = tmem + t * 128;
@@ -465,7 +469,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = b->tmem_slot, tm_x = tmem, tm_y = tmem + 128, tm_acc0 = tmem + 256, tm_acc1 = tmem + 384;
+    constexpr uint32_t tmem = 0, tm_x = 0, tm_y = 128, tm_acc0 = 256, tm_acc1 = 384;       // all 512 columns are allocated, so they start at 0
 
     // tiles of the other axis that one head of an item meets: [first, first + count) in tiles of 128 rows from the sequence's begin
     auto first_tile = [&](const Item& w) { return KV && a.causal ? (w.row0 - w.lo) / 128 : 0; };
@@ -730,9 +734,12 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             // X or Y = R T^T of ring slot `slot` (a constant in each of its two copies)
             auto first_copy = [&](uint32_t tm, const Desc& res, const Desc& ring, auto slot) {
                 const uint32_t rb = ring.lo + slot.v * (TILE >> 4);
+                if (ksteps == HD / 16) {
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk)
-                    if (kk < ksteps) tc_mma_ss(tm, res.lo + KSTEP(kk), res.hi, rb + KSTEP(kk), ring.hi, idesc_first, kk > 0 ? 1u : 0u);
+                    for (int kk = 0; kk < HD / 16; ++kk) tc_mma_ss(tm, res.lo + KSTEP(kk), res.hi, rb + KSTEP(kk), ring.hi, idesc_first, kk > 0 ? 1u : 0u);
+                } else
+#pragma unroll 1
+                    for (int kk = 0; kk < ksteps; ++kk) tc_mma_ss(tm, res.lo + KSTEP(kk), res.hi, rb + KSTEP(kk), ring.hi, idesc_first, kk > 0 ? 1u : 0u);
             };
             auto first_product = [&](uint32_t tm, const Desc& res, const Desc& ring, uint32_t slot) {
                 if (slot == 0) first_copy(tm, res, ring, Const<0>{}); else first_copy(tm, res, ring, Const<1>{});
