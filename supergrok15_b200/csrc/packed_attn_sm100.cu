@@ -154,11 +154,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                             for (int i = 0; i < 32; ++i) if (c * 32 + i >= see) r[c][i] = __float_as_uint(-INFINITY);
                     }
                 }
-                float mx = -FLT_MAX;                                       // finite, so that a tile of -inf scores gives zeros, not NaN
+                float top[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};  // finite, so that a tile of -inf scores gives zeros, not NaN; four chains
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int i = 0; i < 32; i += 2)
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) mx = max3f(mx, __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+                    for (int c = 0; c < 4; ++c) top[c] = max3f(top[c], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+                const float mx = fmaxf(max3f(top[0], top[1], top[2]), top[3]);
                 float alpha = 1.f;
                 bool move = false;
                 if (j == 0) m_ref = mx;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                     }
                 }
                 const float mc = -m_ref * c2;
-                float sum0 = 0.f, sum1 = 0.f;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t pk[32];
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                         float e0, e1;
                         fma2(__uint_as_float(r[k0 >> 5][k0 & 31]), __uint_as_float(r[(k0 + 1) >> 5][(k0 + 1) & 31]), c2, c2, mc, mc, e0, e1);
                         const float p0 = ex2f(e0), p1 = ex2f(e1);
-                        sum0 += p0; sum1 += p1;
+                        sum[2 * (i & 1)] += p0; sum[2 * (i & 1) + 1] += p1;
                         pk[i] = Half2<T>::pack(p0, p1);
                     }
                     tc_st32(ts + c * 32, pk);
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                 tc_wait_st();
                 tc_fence_before();
                 warp_arrive(&b->p_full[t]);
-                l = l * alpha + (sum0 + sum1);
+                l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
             }
             if (!ok) break;
             float inv = 0.f;
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
 // Bound by the latency of that hand-over: with two groups (two warps per scheduler, 64 columns per thread) the tensor pipe was 46 % busy.
 // P and dS are rounded to 16 bits to be operands (half a step of each value); everything they come from and are added to is fp32.
 constexpr int BWD_THREADS = 640;
-constexpr int BWD_REGS = 104, BWD_REGS_OTHERS = 56;                       // 512 x 104 + 128 x 56 <= 640 x 96, the registers of the launch
+constexpr int BWD_REGS = 104, BWD_REGS_OTHERS = 64;                       // 512 x 104 + 128 x 64 = 640 x 96, the registers of the launch
 constexpr int BWD_PITCH = 48;                                             // 32 bytes of a row and a pad
 struct BwdBars {
     uint64_t item_full[2], item_empty[2], clc, res_full, res_empty, ring_full[2], ring_empty[2], tail, a_full, b_full, pa_full, pb_full, vec_full, done;
