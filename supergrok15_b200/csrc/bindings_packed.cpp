@@ -90,6 +90,11 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& q_, const Tensor& k_, const Te
     p.dq = dq.data_ptr(); p.dk = dk.data_ptr(); p.dv = dv.data_ptr();
     const int dt = dtype_code(q);
     auto st = at::cuda::getCurrentCUDAStream();
+    Tensor parts;
+    if (sg::packed_attn_sm100_takes(dt, p)) {
+        const int split = sg::packed_attn_sm100_split(p);
+        if (split > 1) { parts = at::empty({2 * split * k.numel()}, lse.options()); p.kv_parts = parts.data_ptr<float>(); }
+    }
     const int rc = sg::packed_attn_sm100_takes(dt, p) ? sg::packed_attn_sm100_bwd(dt, p, err.data_ptr<int>(), st) : sg::packed_attn_bwd(dt, p, st);
     TORCH_CHECK(rc == 0, "attention_packed: launch of the backward pass failed (code ", rc, ")");
     return {dq, dk, dv};

@@ -432,6 +432,7 @@ struct BwdArgs {
     void *out0, *out1;                                                    // dV, dK, or dQ
     PackedSeqs seqs;
     int heads, group, hd, causal, slots;
+    int split;                                                            // KV: parts of a group of heads, each an item of its own with fp32 results
     float scale;
     int* err;
 };
@@ -454,7 +455,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
     BwdBars* b = reinterpret_cast<BwdBars*>(s_stage + 16 * 32 * BWD_PITCH);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n_heads = KV ? a.heads / a.group : a.heads;                 // heads of the items
+    const int n_heads = KV ? a.heads / a.group : a.heads, n_parts = KV ? n_heads * a.split : n_heads;      // heads, and items of a tile
+    const int group = KV ? a.group / a.split : a.group;                   // KV: query heads of an item (item `head` is key head * split + part)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 17); mbar_init(&b->ring_full[i], 1); mbar_init(&b->ring_empty[i], 1);
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         float v0 = 0.f, v1 = 0.f;
         auto fetch_first = [&](const Item& w) {
             if (w.kind != 1) return;
-            if (KV) { if (carries) v0 = fetch(w, w.head * a.group, first_tile(w)); }
+            if (KV) { if (carries) v0 = fetch(w, w.head * group, first_tile(w)); }
             else if (w.row0 + row < w.hi) {
                 const int64_t at = (int64_t)w.head * a.seqs.total + w.row0 + row;
                 v0 = a.lse[at]; v1 = a.delta[at];
@@ -519,13 +521,13 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         ok = take(w);
         if (ok) fetch_first(w);
         while (ok && w.kind != 0) {
-            const int per_head = w.kind == 1 ? tiles(w) : 0, n_it = KV ? per_head * a.group : per_head;
+            const int per_head = w.kind == 1 ? tiles(w) : 0, n_it = KV ? per_head * group : per_head;
             const float lse_row = v0 * LOG2E, del_row = v1;
             if (carries && n_it > 0) {
                 (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = v0;    // buffer n & 1: every thread has left iteration n - 2
                 warp_arrive(&b->vec_full);
             }
-            int h = KV ? w.head * a.group : w.head, i = first_tile(w);
+            int h = KV ? w.head * group : w.head, i = first_tile(w);
             const int i0 = i, i1 = i + per_head;
             for (int it = 0; it < n_it; ++it, ++n) {
                 const int bs = n & 1;
@@ -608,7 +610,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             if (live > 0) {
                 const int64_t ld = (int64_t)n_heads * a.hd;
                 const bool second = KV && g >= 2;
-                T* base = (T*)(second ? a.out1 : a.out0) + (int64_t)row0 * ld + (int64_t)cur.head * a.hd;
+                const int head = KV ? cur.head / a.split : cur.head;
+                const int64_t at = (int64_t)row0 * ld + (int64_t)head * a.hd;
+                T* base = (T*)(second ? a.out1 : a.out0) + at;
+                float* part = KV && a.split > 1 ? (float*)(second ? a.out1 : a.out0) + (int64_t)(cur.head % a.split) * a.seqs.total * ld + at + lane * ld : nullptr;
                 const float f = KV && !second ? 1.f : a.scale;
                 const uint32_t acc = (second ? tm_acc1 : tm_acc0) + lane_addr;
                 const int c0 = KV ? (g & 1) * (HD / 64) : g, c1 = KV ? c0 + HD / 64 : (g < HD / 32 ? g + 1 : g);
@@ -621,6 +626,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                     } else {
 #pragma unroll
                         for (int k = 0; k < 32; ++k) t[k] = 0u;
+                    }
+                    if (KV && part) {                                     // a part of a sum: fp32, added up by packed_join_kernel
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            if (lane < live && c * 32 + k < a.hd)
+                                *reinterpret_cast<float4*>(part + c * 32 + k) = make_float4(__uint_as_float(t[k]) * f, __uint_as_float(t[k + 1]) * f,
+                                                                                           __uint_as_float(t[k + 2]) * f, __uint_as_float(t[k + 3]) * f);
+                        continue;
                     }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {                // 16 columns at a time, two lanes store 32 consecutive bytes of a row
@@ -656,18 +669,18 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                     clc_ask(&b->answer, &b->clc);
                 }
                 // the tiles with the most work start first: early keys are seen by most queries, late queries see most keys
-                const int ord = item / n_heads;
+                const int ord = item / n_parts;
                 const PackedTile t = packed_tile<128>(a.seqs, KV ? ord : a.slots - 1 - ord);
                 if (t.live) {
-                    const Item w{t.lo, t.hi, t.row0, item % n_heads, t.pad ? 2 : 1};
+                    const Item w{t.lo, t.hi, t.row0, item % n_parts, t.pad ? 2 : 1};
                     const uint32_t s = n_item & 1;
                     if (n_item >= 2) ok = warp_wait(&b->item_empty[s], ((n_item >> 1) & 1) ^ 1);
                     if (!ok) { if (lane == 0) atomicExch(a.err, 86); break; }
                     if (lane == 0) { b->item[s] = w; mbar_arrive(&b->item_full[s]); }
                     ++n_item;
-                    const int per_head = t.pad ? 0 : tiles(w), n_it = KV ? per_head * a.group : per_head, i0 = first_tile(w);
-                    const int hk = KV ? w.head : w.head / a.group;
-                    int h = KV ? w.head * a.group : w.head, i = i0;
+                    const int per_head = t.pad ? 0 : tiles(w), n_it = KV ? per_head * group : per_head, i0 = first_tile(w);
+                    const int hk = KV ? w.head / a.split : w.head / a.group;
+                    int h = KV ? w.head * group : w.head, i = i0;
                     for (int it = 0; it < n_it; ++it, ++n) {
                         const uint32_t r = n & 1;
                         const int row = t.lo + i * 128, have = t.hi - row;
@@ -688,8 +701,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                             if (lane == 0) {
                                 mbar_expect_tx(&b->res_full, 2 * TILE);
                                 for (int hf = 0; hf < HALVES; ++hf) {
-                                    tma_load_3d(sR0 + hf * HALF_TILE, KV ? &map_k : &map_q, hf * 64, w.head, t.row0, &b->res_full);
-                                    tma_load_3d(sR1 + hf * HALF_TILE, KV ? &map_v : &map_do, hf * 64, w.head, t.row0, &b->res_full);
+                                    tma_load_3d(sR0 + hf * HALF_TILE, KV ? &map_k : &map_q, hf * 64, KV ? hk : w.head, t.row0, &b->res_full);
+                                    tma_load_3d(sR1 + hf * HALF_TILE, KV ? &map_v : &map_do, hf * 64, KV ? hk : w.head, t.row0, &b->res_full);
                                 }
                             }
                         }
@@ -727,7 +740,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 warp_arrive(&b->item_empty[si]);
                 ++n_item;
                 if (w.kind != 1) return w.kind == 0 ? 0 : -2;
-                return KV ? tiles(w) * a.group : tiles(w);
+                return KV ? tiles(w) * group : tiles(w);
             };
             const Desc r0 = desc_of(make_desc_sw128(smem_u32(sR0))), r1 = desc_of(make_desc_sw128(smem_u32(sR1))), t0 = desc_of(make_desc_sw128(smem_u32(sT0))),
                        t1 = desc_of(make_desc_sw128(smem_u32(sT1))), m0 = desc_of(make_desc_sw128_mn(smem_u32(sT0), HALF_TILE, 1024)),
@@ -825,6 +838,21 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
     }
 }
 
+// out0 / out1 = the sums of their parts, in order, n elements each (a multiple of 8)
+template <typename T>
+__global__ void __launch_bounds__(256) packed_join_kernel(const float* __restrict__ p0, const float* __restrict__ p1, int split, int64_t n, T* __restrict__ o0, T* __restrict__ o1) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= n) return;
+    const float* p = (blockIdx.y ? p1 : p0) + i;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < split; ++s) {
+        const float4 x = *reinterpret_cast<const float4*>(p + s * n), y = *reinterpret_cast<const float4*>(p + s * n + 4);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+    *reinterpret_cast<uint4*>((blockIdx.y ? o1 : o0) + i) = make_uint4(Half2<T>::pack(v[0], v[1]), Half2<T>::pack(v[2], v[3]), Half2<T>::pack(v[4], v[5]), Half2<T>::pack(v[6], v[7]));
+}
+
 // delta[head][row] = dO . (O + rest): 16 bytes of each per lane, 8 or 16 lanes per (row, head)
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) packed_delta_sm100_kernel(PackedAttn p) {
@@ -880,10 +908,15 @@ template <typename T, int HD> int bwd(const PackedAttn& p, int* err, cudaStream_
         })) return 11;
     constexpr int LANES = HD / 8;
     const int slots = packed_slots(p.seqs.n, p.seqs.total, 128);
-    BwdArgs a{p.lse, p.delta, p.dv, p.dk, p.seqs, p.heads, p.group, p.hd, p.causal, slots, p.scale, err};
-    count_launch(3);
+    const int split = p.kv_parts ? packed_attn_sm100_split(p) : 1;
+    const int64_t n_kv = (int64_t)p.seqs.total * hk * p.hd;
+    BwdArgs a{p.lse, p.delta, split > 1 ? (void*)p.kv_parts : p.dv, split > 1 ? (void*)(p.kv_parts + split * n_kv) : p.dk, p.seqs, p.heads, p.group, p.hd, p.causal, slots,
+              split, p.scale, err};
+    count_launch(split > 1 ? 4 : 3);
     packed_delta_sm100_kernel<T, LANES><<<(unsigned)(((int64_t)p.seqs.total * p.heads * LANES + 255) / 256), 256, 0, st>>>(p);
-    packed_bwd_sm100_kernel<T, HD, true><<<(unsigned)slots * (unsigned)hk, BWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
+    packed_bwd_sm100_kernel<T, HD, true><<<(unsigned)slots * (unsigned)(hk * split), BWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
+    if (split > 1)
+        packed_join_kernel<T><<<dim3((unsigned)((n_kv / 8 + 255) / 256), 2), 256, 0, st>>>(p.kv_parts, p.kv_parts + split * n_kv, split, n_kv, (T*)p.dv, (T*)p.dk);
     a.out0 = p.dq; a.out1 = nullptr;
     packed_bwd_sm100_kernel<T, HD, false><<<(unsigned)slots * (unsigned)p.heads, BWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
     return cudaGetLastError() == cudaSuccess ? 0 : 12;
@@ -899,6 +932,17 @@ bool packed_attn_sm100_takes(int dtype, const PackedAttn& p) {
            (int64_t)packed_slots(p.seqs.n, p.seqs.total, 128) * p.heads < ((int64_t)1 << 31);
 }
 
+// Parts that the query heads of a key head are cut into for dK and dV.  An item of that kernel visits every query tile of all its heads; with
+// few key heads the longest ones (the first keys of a long causal sequence) then take longer than the average SM is busy.  Cut until one
+// takes at most half of that, were the rows one sequence of their average length; below 1,024 rows a sequence items are short anyway.
+// Two key heads, 14,354 + 2,030 tokens: 2,030 us whole, 1,480 and 24 for the sums in four parts.
+int packed_attn_sm100_split(const PackedAttn& p) {
+    const int64_t hk = p.heads / p.group, tiles = p.seqs.total / 128, each = p.seqs.n > 0 ? p.seqs.total / p.seqs.n : 0;
+    if (p.group == 1 || each < 1024) return 1;
+    const int64_t want = (4 * (int64_t)device_sms() + hk * tiles - 1) / (hk * tiles);
+    for (int s = 1; s < p.group; ++s) if (p.group % s == 0 && s >= want) return s;
+    return want > 1 ? p.group : 1;
+}
 int packed_attn_sm100_fwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st) {
     if (p.hd > 64) return dtype == BF16 ? fwd<__nv_bfloat16, 128>(p, err, st) : fwd<__half, 128>(p, err, st);
     return dtype == BF16 ? fwd<__nv_bfloat16, 64>(p, err, st) : fwd<__half, 64>(p, err, st);
