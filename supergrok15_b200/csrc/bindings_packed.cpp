@@ -198,7 +198,7 @@ std::vector<Tensor> lce_fwd(const Tensor& x, const Tensor& w_, const Tensor& t, 
     Tensor loss = at::empty({}, fo), xc = at::empty({s.rows, s.a.ldx}, xo), keep = at::empty({s.rows + KEEP_MORE + (train ? s.piece : 0)}, fo.dtype(at::kInt));
     Tensor u = train ? at::empty({s.piece, s.a.ldu}, xo) : none, dx = none, dw = none;
     s.a.x = xc.data_ptr();
-    const int64_t tiles = (s.a.V + sg::lce_tile_columns(s.dtype, s.a) - 1) / sg::lce_tile_columns(s.dtype, s.a), blocks = sg::lce_gather_blocks((int)s.rows);
+    const int64_t tiles = (s.a.V + sg::LCE_COLUMNS - 1) / sg::LCE_COLUMNS, blocks = sg::lce_gather_blocks((int)s.rows);
     // scratch of this pass: targets [rows] (8 bytes each), statistics [piece][tiles] (8), target logits [piece], losses [rows], block counts
     Tensor scratch = at::empty({2 * s.rows + 2 * s.piece * tiles + s.piece + s.rows + blocks}, fo);
     float* f = scratch.data_ptr<float>();

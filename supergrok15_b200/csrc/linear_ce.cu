@@ -23,7 +23,8 @@
 // reading and writing u once more.
 //
 // This file: the passes over the rows, and products on the CUDA cores for fp32 operands and for 16-bit ones that TMA cannot address.  Their
-// 64 x 64 tiles take 4 x 4 outputs per thread from shared memory in steps of 16, bound by the FMA pipe and its operand loads.
+// 128 x 128 tiles take 8 x 8 outputs per thread in steps of 16, the next step's operands on their way to registers under this one's
+// products; two fused multiply-adds per instruction (packed pairs), four 16-byte loads from shared memory for 64 of them.
 #include "sg_native.h"
 #include "optim_math.cuh"
 #include "linear_ce.h"
@@ -33,62 +34,122 @@
 namespace sg {
 namespace {
 
-constexpr int CT = 64, CK = 16, CTHREADS = 256;
+constexpr int CT = 128, CK = 16, CTHREADS = 256;
+using Pair = unsigned long long;                                          // two fp32 values
 
-// s[i][j] += sum_k A(m0 + ty*4 + i, k) B(n0 + tx*4 + j, k).  AM / BN: the operand's m / n index is the contiguous one, else its k index.
-template <typename T, bool AM, bool BN>
-__device__ __forceinline__ void tile_product(const T* A, int64_t lda, const T* B, int64_t ldb, int M, int N, int K, int m0, int n0, float (&s)[4][4]) {
-    __shared__ __align__(16) float sa[CK][CT + 4], sb[CK][CT + 4];
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    for (int k0 = 0; k0 < K; k0 += CK) {
-        __syncthreads();
+__device__ __forceinline__ Pair twice(float a) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "f"(a));
+    return p;
+}
+__device__ __forceinline__ float2 both(Pair p) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void fma_pair(Pair& acc, Pair a, Pair b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b)); }
+
+// A step's operand, 128 indices x 16 of k: two vectors of four per thread, from memory in which the index (IM) or k is contiguous
+template <typename T, bool IM> struct StepLoad {
+    float v[2][4];
+    // vec: rows start on 16 bytes and the contiguous extent is whole fours (fp32)
+    __device__ __forceinline__ void load(const T* p, int64_t ld, bool vec, int i0, int I, int k0, int K) {
 #pragma unroll
-        for (int i = threadIdx.x; i < CT * CK; i += CTHREADS) {
-            const int ma = AM ? i % CT : i / CK, ka = AM ? i / CT : i % CK;
-            sa[ka][ma] = m0 + ma < M && k0 + ka < K ? Cvt<T>::to(AM ? A[(int64_t)(k0 + ka) * lda + m0 + ma] : A[(int64_t)(m0 + ma) * lda + k0 + ka]) : 0.f;
-            const int nb = BN ? i % CT : i / CK, kb = BN ? i / CT : i % CK;
-            sb[kb][nb] = n0 + nb < N && k0 + kb < K ? Cvt<T>::to(BN ? B[(int64_t)(k0 + kb) * ldb + n0 + nb] : B[(int64_t)(n0 + nb) * ldb + k0 + kb]) : 0.f;
-        }
-        __syncthreads();
+        for (int u = 0; u < 2; ++u) {
+            const int q = threadIdx.x + u * CTHREADS;
+            const int i = i0 + (IM ? (q & 31) * 4 : q >> 2), k = k0 + (IM ? q >> 5 : (q & 3) * 4);
+            const T* src = IM ? p + (int64_t)k * ld + i : p + (int64_t)i * ld + k;
+            const bool row = IM ? k < K : i < I;
+            if (sizeof(T) == 4 && vec) {
+                const float4 f = row && (IM ? i < I : k < K) ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[u][0] = f.x; v[u][1] = f.y; v[u][2] = f.z; v[u][3] = f.w;
+            } else {
 #pragma unroll
-        for (int k = 0; k < CK; ++k) {
-            const float4 a = *reinterpret_cast<const float4*>(&sa[k][ty * 4]), b = *reinterpret_cast<const float4*>(&sb[k][tx * 4]);
-            const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[i][j] = fmaf(av[i], bv[j], s[i][j]);
+                for (int e = 0; e < 4; ++e) v[u][e] = row && (IM ? i + e < I : k + e < K) ? Cvt<T>::to(src[e]) : 0.f;
+            }
         }
     }
+    __device__ __forceinline__ void store(float (*s)[CT + 4]) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int q = threadIdx.x + u * CTHREADS;
+            if (IM) *reinterpret_cast<float4*>(&s[q >> 5][(q & 31) * 4]) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[(q & 3) * 4 + e][q >> 2] = v[u][e];
+        }
+    }
+};
+
+// Whether an operand's rows can be read four at a time; n: its contiguous extent
+__device__ __forceinline__ bool fours(const void* p, int64_t ld, int n) { return ((reinterpret_cast<uintptr_t>(p) & 15) | (ld & 3) | (n & 3)) == 0; }
+
+// M, KA: extents of A (u is zero from V to its pitch, so that its rows can be read to whole fours); N: of B, whose k ends with k1.
+// acc[i][j] += sum over [k0, k1) of A(m, k) B(n, k), m = m0 + row(i), n = n0 + 4 tx + 64 (j / 2) + 2 (j % 2) and the next; row(i) = 4 ty + i % 4 + 64 (i / 4)
+template <typename T, bool AM, bool BN>
+__device__ __forceinline__ void tile_product(const T* A, int64_t lda, const T* B, int64_t ldb, int M, int KA, int N, int k0, int k1, int m0, int n0, Pair (&acc)[8][4]) {
+    __shared__ __align__(16) float sa[2][CK][CT + 4], sb[2][CK][CT + 4];
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const bool va = fours(A, lda, AM ? M : KA), vb = fours(B, ldb, BN ? N : k1);
+    StepLoad<T, AM> la;
+    StepLoad<T, BN> lb;
+    la.load(A, lda, va, m0, M, k0, KA); lb.load(B, ldb, vb, n0, N, k0, k1);
+    la.store(sa[0]); lb.store(sb[0]);
+    __syncthreads();
+    int cur = 0;
+    for (int k = k0; k < k1; k += CK, cur ^= 1) {
+        const bool more = k + CK < k1;
+        if (more) { la.load(A, lda, va, m0, M, k + CK, KA); lb.load(B, ldb, vb, n0, N, k + CK, k1); }
+#pragma unroll
+        for (int kk = 0; kk < CK; ++kk) {
+            const float4 a0 = *reinterpret_cast<const float4*>(&sa[cur][kk][ty * 4]), a1 = *reinterpret_cast<const float4*>(&sa[cur][kk][64 + ty * 4]);
+            const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(&sb[cur][kk][tx * 4]), b1 = *reinterpret_cast<const ulonglong2*>(&sb[cur][kk][64 + tx * 4]);
+            const float av[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const Pair aa = twice(av[i]);
+                fma_pair(acc[i][0], aa, b0.x); fma_pair(acc[i][1], aa, b0.y); fma_pair(acc[i][2], aa, b1.x); fma_pair(acc[i][3], aa, b1.y);
+            }
+        }
+        if (more) { la.store(sa[cur ^ 1]); lb.store(sb[cur ^ 1]); }
+        __syncthreads();
+    }
+}
+__device__ __forceinline__ int tile_row(int i) { return (int)(threadIdx.x >> 4) * 4 + (i & 3) + 64 * (i >> 2); }
+__device__ __forceinline__ int tile_col(int j) { return (int)(threadIdx.x & 15) * 4 + (j & 3) + 64 * (j >> 2); }
+__device__ __forceinline__ void row_of(const Pair (&acc)[4], float (&s)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { const float2 v = both(acc[j]); s[2 * j] = v.x; s[2 * j + 1] = v.y; }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(CTHREADS) lce_logits_kernel(LceArgs a) {
-    const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, rows = lce_active(a);
+__global__ void __launch_bounds__(CTHREADS, 2) lce_logits_kernel(LceArgs a) {
+    const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, tx = threadIdx.x & 15, rows = lce_active(a);
     if (m0 >= rows) return;
-    float s[4][4] = {};
-    tile_product<T, false, false>((const T*)a.x, a.ldx, (const T*)a.w, a.ldw, rows, a.V, a.D, m0, n0, s);
+    Pair acc[8][4] = {};
+    tile_product<T, false, false>((const T*)a.x, a.ldx, (const T*)a.w, a.ldw, rows, a.D, a.V, 0, a.D, m0, n0, acc);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = m0 + ty * 4 + i;
+    for (int i = 0; i < 8; ++i) {
+        const int row = m0 + tile_row(i);
         const int64_t t = row < rows ? a.target[row] : -1;
-        float mx = -INFINITY;
+        float s[8], mx = -INFINITY;
+        row_of(acc[i], s);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int v = n0 + tx * 4 + j;
-            if (v >= a.V) s[i][j] = -INFINITY;
-            else if (v == t) a.z_target[row] = s[i][j];
-            s[i][j] *= 1.4426950408889634f;                               // from here on in powers of two
-            mx = fmaxf(mx, s[i][j]);
+        for (int j = 0; j < 8; ++j) {
+            const int v = n0 + tile_col(j);
+            if (v >= a.V) s[j] = -INFINITY;
+            else if (v == t) a.z_target[row] = s[j];
+            s[j] *= 1.4426950408889634f;                                  // from here on in powers of two
+            mx = fmaxf(mx, s[j]);
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const float ref = mx == -INFINITY ? 0.f : mx;
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int v = n0 + tx * 4 + j;
-            const float e = exp2f(s[i][j] - ref);
+        for (int j = 0; j < 8; ++j) {
+            const int v = n0 + tile_col(j);
+            const float e = exp2f(s[j] - ref);
             if (v != t) sum += e;
             if (a.u && row < rows && v < a.V) ((T*)a.u)[(int64_t)row * a.ldu + v] = Cvt<T>::from(e * LceUnit<T>::value);
         }
@@ -98,23 +159,31 @@ __global__ void __launch_bounds__(CTHREADS) lce_logits_kernel(LceArgs a) {
     }
 }
 
-// dx (AM = false: d [rows, V] times w [V, D]) or dw (AM = true: d^T times x [rows, D])
+// dx (AM = false: d [rows, V] times w [V, D], part blockIdx.z of the sum) or dw (AM = true: d^T times x [rows, D])
 template <typename T, typename TO, bool AM>
-__global__ void __launch_bounds__(CTHREADS) lce_grad_kernel(LceArgs a, const float* prev, TO* out, const float* gout, const float* inv) {
-    const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, rows = lce_active(a);
+__global__ void __launch_bounds__(CTHREADS, 2) lce_grad_kernel(LceArgs a, const float* prev, TO* out, int64_t row_pitch, const float* gout, const float* inv) {
+    const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, rows = lce_active(a);
     const int M = AM ? a.V : rows;
     if (m0 >= M) return;
-    float s[4][4] = {};
-    if (AM) tile_product<T, true, true>((const T*)a.u, a.ldu, (const T*)a.x, a.ldx, a.V, a.D, rows, m0, n0, s);
-    else tile_product<T, false, true>((const T*)a.u, a.ldu, (const T*)a.w, a.ldw, rows, a.D, a.V, m0, n0, s);
+    Pair acc[8][4] = {};
+    if (AM) tile_product<T, true, true>((const T*)a.u, a.ldu, (const T*)a.x, a.ldx, (int)a.ldu, rows, a.D, 0, rows, m0, n0, acc);
+    else {
+        const int per = ((a.V + (int)gridDim.z - 1) / (int)gridDim.z + CK - 1) / CK * CK, k0 = per * (int)blockIdx.z;
+        out += (int64_t)blockIdx.z * row_pitch * a.D;
+        if (k0 < a.V) tile_product<T, false, true>((const T*)a.u, a.ldu, (const T*)a.w, a.ldw, rows, min(k0 + per, (int)a.ldu), a.D, k0, min(k0 + per, a.V), m0, n0, acc);
+    }
     const float f = gout ? gout[0] * inv[0] / LceUnit<T>::value : 1.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i) {
+        const int m = m0 + tile_row(i);
+        float s[8];
+        row_of(acc[i], s);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m < M && n < a.D) out[(int64_t)m * a.D + n] = Cvt<TO>::from(f * (prev ? s[i][j] + prev[(int64_t)m * a.D + n] : s[i][j]));
+        for (int j = 0; j < 8; ++j) {
+            const int n = n0 + tile_col(j);
+            if (m < M && n < a.D) out[(int64_t)m * a.D + n] = Cvt<TO>::from(f * (prev ? s[j] + prev[(int64_t)m * a.D + n] : s[j]));
         }
+    }
 }
 
 constexpr int ROW_THREADS = 256;
@@ -177,7 +246,7 @@ template <typename T> __device__ __forceinline__ uint4 scaled(uint4 raw, float f
     return raw;
 }
 template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int tiles, int tile_shift, bool last) {
+__global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int tiles, bool last) {
     extern __shared__ float fac[];                                        // [tiles] factor of a tile's columns
     __shared__ float red[32];
     constexpr int PER = 16 / sizeof(T), STEP = ROW_THREADS * PER;
@@ -200,8 +269,8 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int ti
         for (int c = c0 + threadIdx.x * PER; c < c1; c += 2 * STEP) {     // PER divides a tile's columns
             const int c2 = c + STEP;
             const uint4 x = *reinterpret_cast<const uint4*>(u + c), y = c2 < c1 ? *reinterpret_cast<const uint4*>(u + c2) : make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(u + c) = scaled<T>(x, fac[min(c >> tile_shift, tiles - 1)] * inv);
-            if (c2 < c1) *reinterpret_cast<uint4*>(u + c2) = scaled<T>(y, fac[min(c2 >> tile_shift, tiles - 1)] * inv);
+            *reinterpret_cast<uint4*>(u + c) = scaled<T>(x, fac[min(c / LCE_COLUMNS, tiles - 1)] * inv);
+            if (c2 < c1) *reinterpret_cast<uint4*>(u + c2) = scaled<T>(y, fac[min(c2 / LCE_COLUMNS, tiles - 1)] * inv);
         }
         __syncthreads();
         if (threadIdx.x == 0 && t >= c0 && t < c1) u[t] = Cvt<T>::from(at_target);
@@ -233,7 +302,7 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_row_losses_kernel(LceArgs a, 
 
 // Training in bf16: a warp per row.  The loss and the row's scale; the target's entry of u; the tiles with another reference than the row's;
 // the row of x times the scale, in place (nothing else reads it any more).
-__global__ void __launch_bounds__(ROW_THREADS) lce_scale_rows_kernel(LceArgs a, int tiles, int tile_cols, bool last) {
+__global__ void __launch_bounds__(ROW_THREADS) lce_scale_rows_kernel(LceArgs a, int tiles, bool last) {
     __shared__ float red[32];
     const int row = blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row < lce_active(a)) {
@@ -255,7 +324,7 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_scale_rows_kernel(LceArgs a, 
                 const float r = st[i].x;
                 if (r == mx) continue;
                 const float f = exp2f(r - mx);
-                for (int c = i * tile_cols + lane; c < (i + 1) * tile_cols && c < a.V; c += 32) u[c] = __float2bfloat16_rn(__bfloat162float(u[c]) * f);
+                for (int c = i * LCE_COLUMNS + lane; c < (i + 1) * LCE_COLUMNS && c < a.V; c += 32) u[c] = __float2bfloat16_rn(__bfloat162float(u[c]) * f);
             }
         __syncwarp();
         if (lane == 0) {
@@ -401,15 +470,15 @@ template <typename T> int logits(const LceArgs& a, cudaStream_t st) {
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
-template <typename T> int rows(const LceArgs& a, int tile_cols, bool last, cudaStream_t st) {
-    const int tiles = (a.V + tile_cols - 1) / tile_cols;
+template <typename T> int rows(const LceArgs& a, bool last, cudaStream_t st) {
+    const int tiles = (a.V + LCE_COLUMNS - 1) / LCE_COLUMNS;
     count_launch();
     if (!a.u) {
         lce_row_losses_kernel<<<(a.rows + 7) / 8, ROW_THREADS, 0, st>>>(a, tiles, last);
         return cudaGetLastError() == cudaSuccess ? 0 : 3;
     }
     if (a.row_scale) {
-        lce_scale_rows_kernel<<<(a.rows + 7) / 8, ROW_THREADS, 0, st>>>(a, tiles, tile_cols, last);
+        lce_scale_rows_kernel<<<(a.rows + 7) / 8, ROW_THREADS, 0, st>>>(a, tiles, last);
         return cudaGetLastError() == cudaSuccess ? 0 : 3;
     }
     const size_t smem = tiles * sizeof(float);
@@ -418,18 +487,19 @@ template <typename T> int rows(const LceArgs& a, int tile_cols, bool last, cudaS
         return 2;
     if (smem > 200 * 1024) return 4;
     const int cut = a.rows >= 2 * device_sms() ? 1 : (2 * device_sms() + a.rows - 1) / a.rows;
-    lce_rows_kernel<T><<<dim3(a.rows, cut < 8 ? cut : 8), ROW_THREADS, smem, st>>>(a, tiles, tile_cols == 128 ? 7 : 6, last);
+    lce_rows_kernel<T><<<dim3(a.rows, cut < 8 ? cut : 8), ROW_THREADS, smem, st>>>(a, tiles, last);
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
 template <typename T, typename TO> int grads(const LceArgs& a, const LceGrads& g, cudaStream_t st) {
     if (g.dx_part) {
         count_launch();
-        lce_grad_kernel<T, float, false><<<dim3((a.D + CT - 1) / CT, (a.rows + CT - 1) / CT), CTHREADS, 0, st>>>(a, nullptr, g.dx_part, g.gout, g.inv_count);
+        lce_grad_kernel<T, float, false><<<dim3((a.D + CT - 1) / CT, (a.rows + CT - 1) / CT, g.parts), CTHREADS, 0, st>>>(a, nullptr, g.dx_part, g.row_pitch, g.gout,
+                                                                                                                      g.inv_count);
     }
     if (g.dw) {
         count_launch();
-        lce_grad_kernel<T, TO, true><<<dim3((a.D + CT - 1) / CT, (a.V + CT - 1) / CT), CTHREADS, 0, st>>>(a, g.dw_prev, (TO*)g.dw, g.gout, g.inv_count);
+        lce_grad_kernel<T, TO, true><<<dim3((a.D + CT - 1) / CT, (a.V + CT - 1) / CT), CTHREADS, 0, st>>>(a, g.dw_prev, (TO*)g.dw, 0, g.gout, g.inv_count);
     }
     return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
@@ -448,12 +518,15 @@ int scatter(const int* place, int rows, int D, int first, const float* early, co
 }  // namespace
 
 #define SG_LCE_GO(fn, ...) { if (dtype == F32) return fn<float>(__VA_ARGS__); if (dtype == BF16) return fn<__nv_bfloat16>(__VA_ARGS__); return fn<__half>(__VA_ARGS__); }
-int lce_tile_columns(int dtype, const LceArgs& a) { return lce_sm100_takes(dtype, a) ? LCE_SM100_COLUMNS : CT; }
+static_assert(CT == LCE_COLUMNS, "a tile of the logits is a tile of the statistics");
 bool lce_scales_rows(int dtype, const LceArgs& a) { return dtype == BF16 && lce_sm100_takes(dtype, a); }
 int lce_dx_parts(int dtype, const LceArgs& a, bool with_dw, int64_t* row_pitch) {
     if (lce_sm100_takes(dtype, a)) return lce_sm100_dx_parts(a.rows, a.V, a.D, with_dw, row_pitch);
+    // two tiles per SM at a time: as many parts as fill them, each at least 256 columns of the vocabulary
     *row_pitch = a.rows;
-    return 1;
+    const int64_t tiles = (int64_t)((a.rows + CT - 1) / CT) * ((a.D + CT - 1) / CT), fill = (2 * device_sms() + tiles - 1) / tiles, most = a.V / 256;
+    const int64_t n = fill < most ? fill : most;
+    return n < 1 ? 1 : (n < 64 ? (int)n : 64);
 }
 int lce_gather_blocks(int rows) { return rows > GATHER_DIRECT ? (rows + COUNT_ROWS - 1) / COUNT_ROWS : 0; }
 int lce_gather(int dtype, const void* x, int64_t ldx, const int64_t* target, int64_t ignore_index, int rows, int V, int D, int* place, void* xc, int64_t* tc,
@@ -473,7 +546,7 @@ int lce_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st) {
     if (lce_sm100_takes(dtype, a)) return lce_sm100_logits(dtype, a, err, st);
     SG_LCE_GO(logits, a, st)
 }
-int lce_rows(int dtype, const LceArgs& a, bool last, cudaStream_t st) SG_LCE_GO(rows, a, lce_tile_columns(dtype, a), last, st)
+int lce_rows(int dtype, const LceArgs& a, bool last, cudaStream_t st) SG_LCE_GO(rows, a, last, st)
 int lce_grads(int dtype, const LceArgs& a, const LceGrads& g, int* err, cudaStream_t st) {
     if (lce_sm100_takes(dtype, a)) return lce_sm100_grads(dtype, a, g, err, st);
     if (dtype == F32) return grads<float, float>(a, g, st);

@@ -57,8 +57,7 @@ inline int64_t lce_pitch(int64_t n, int64_t elem) { const int64_t per = (elem ==
 template <typename T> struct LceUnit { static constexpr float value = 1.f; };
 template <> struct LceUnit<__half> { static constexpr float value = 32768.f; };
 
-// columns per statistics tile of the kernels that will run
-int lce_tile_columns(int dtype, const LceArgs& a);
+constexpr int LCE_COLUMNS = 128;        // columns per statistics tile
 // parts that dx is summed in, and rows from one part to the next
 int lce_dx_parts(int dtype, const LceArgs& a, bool with_dw, int64_t* row_pitch);
 
@@ -79,7 +78,6 @@ int lce_scatter(int dtype, const int* place, int rows, int D, int first, const f
                 const float* inv_count, void* dx, cudaStream_t st);
 
 // The tensor-core kernels; `err` (a device word) becomes non-zero when a wait inside a kernel ran out.
-constexpr int LCE_SM100_COLUMNS = 128;
 bool lce_sm100_takes(int dtype, const LceArgs& a);
 int lce_sm100_dx_parts(int rows, int V, int D, bool with_dw, int64_t* row_pitch);
 int lce_sm100_logits(int dtype, const LceArgs& a, int* err, cudaStream_t st);

@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
                         }
                     };
                     chunk(r[0], 0); chunk(r[1], 1); chunk(r[2], 2); chunk(r[3], 3);
-                    if (row < live) a.stats[(int64_t)row * ((a.V + 127) / 128) + n0 / 128] = make_float2(ref, sum0 + sum1);
+                    if (row < live) a.stats[(int64_t)row * ((a.V + LCE_COLUMNS - 1) / LCE_COLUMNS) + n0 / LCE_COLUMNS] = make_float2(ref, sum0 + sum1);
                 }
             } else {
                 const bool is_x = w.kind == 1, f32 = is_x || a.f32_w;
