@@ -25,23 +25,40 @@ namespace {
 
 constexpr int PT = 64, PTHREADS = 256;
 
-// rows [row0, row0 + 64) of head `h`, zero where row >= hi or column >= hd
+// rows [row0, row0 + 64) of a head, zero where row >= hi or column >= hd: four columns of DP / 16 rows per thread, all loads in flight at once
 template <typename T, int DP>
 __device__ __forceinline__ void load_tile(float* dst, const T* base, int64_t ld, int row0, int hi, int hd) {
-    for (int i = threadIdx.x; i < PT * DP; i += PTHREADS) {
-        const int r = i / DP, c = i % DP, row = row0 + r;
-        dst[r * (DP + 4) + c] = (row < hi && c < hd) ? Cvt<T>::to(base[(int64_t)row * ld + c]) : 0.f;
-    }
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const bool vec = sizeof(T) == 4 && ((reinterpret_cast<uintptr_t>(base) & 15) | (ld & 3) | (hd & 3)) == 0;
+    float4 v[4][DP / 64];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int m = 0; m < DP / 64; ++m) {
+            const int row = row0 + ty + 16 * i, c = 4 * (tx + 16 * m);
+            const T* src = base + (int64_t)row * ld + c;
+            if (vec) v[i][m] = row < hi && c < hd ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+            else {
+                float e[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) e[u] = row < hi && c + u < hd ? Cvt<T>::to(src[u]) : 0.f;
+                v[i][m] = make_float4(e[0], e[1], e[2], e[3]);
+            }
+        }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int m = 0; m < DP / 64; ++m) *reinterpret_cast<float4*>(dst + (ty + 16 * i) * (DP + 4) + 4 * (tx + 16 * m)) = v[i][m];
 }
 
 // s[i][j] = a[ty + 16 i] . b[tx + 16 j]
-template <int DP> __device__ __forceinline__ void dot4x4(const float* a, const float* b, int ty, int tx, float (&s)[4][4]) {
+template <int DP> __device__ __forceinline__ void dot4x4(const float* a, const float* b, int hd, int ty, int tx, float (&s)[4][4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
 #pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
+    for (int d = 0; d < hd; d += 4) {
         float4 x[4], y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -144,7 +161,7 @@ __global__ void __launch_bounds__(PTHREADS) packed_fwd_kernel(PackedAttn p) {
         load_tile<T, DP>(sV, (const T*)p.v + hk * p.v_hs, p.v_ld, k0, t.hi, p.hd);
         __syncthreads();
         float s[4][4];
-        dot4x4<DP>(sQ, sK, ty, tx, s);
+        dot4x4<DP>(sQ, sK, p.hd, ty, tx, s);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = t.row0 + ty + 16 * i;
@@ -192,8 +209,8 @@ template <int DP>
 __device__ __forceinline__ void bwd_scores(const PackedAttn& p, const float* sQ, const float* sK, const float* sDO, const float* sV, float* sP, float* sS, int h,
                                            int q0, int k0, int hi, int ty, int tx) {
     float s[4][4], d[4][4];
-    dot4x4<DP>(sQ, sK, ty, tx, s);
-    dot4x4<DP>(sDO, sV, ty, tx, d);
+    dot4x4<DP>(sQ, sK, p.hd, ty, tx, s);
+    dot4x4<DP>(sDO, sV, p.hd, ty, tx, d);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int row = q0 + ty + 16 * i;
