@@ -2,6 +2,8 @@
 
     python -m supergrok15_b200.ops.bench_nn --what flash            # tcgen05 flash attention fwd / bwd vs F.scaled_dot_product_attention
     python -m supergrok15_b200.ops.bench_nn --what ce               # fused cross-entropy fwd / bwd vs F.cross_entropy
+    python -m supergrok15_b200.ops.bench_nn --what packed           # attention over packed sequences, fwd / bwd, against a padded batch through SDPA
+    python -m supergrok15_b200.ops.bench_nn --what head             # linear_cross_entropy fwd / bwd vs F.linear + the fused cross-entropy
     python -m supergrok15_b200.ops.bench_nn --what norm             # RMSNorm with fused residual vs F.rms_norm(x + r)
     python -m supergrok15_b200.ops.bench_nn --what linear           # tcgen05 Linear (forward, dgrad, wgrad) vs cuBLAS on the flagship's layer shapes
     python -m supergrok15_b200.ops.bench_nn --what small_ops        # GELU, bias-gradient column sums, small-table embedding gradient, LayerNorm backward
@@ -72,6 +74,47 @@ def bench_ce(small: bool, it: int):
     t_o, t_r = timed(own, it), timed(ref, it)
     by = rows * V * 2 * 3                                       # logits read twice, gradient written once
     print(json.dumps({"kernel": "cross_entropy_fwd_bwd", "rows": rows, "V": V, "ms": t_o, "GBps": by / t_o / 1e6, "torch_ms": t_r}), flush=True)
+
+
+def bench_packed(small: bool, it: int):
+    from . import gemm, nn_ops
+    dev = torch.device("cuda:0")
+    docs = [700, 90, 1258] if small else [42, 120, 77, 464, 33, 56, 409, 783, 2309, 36, 1897, 272, 1676, 18]
+    for H, K, HD in [(16, 16, 128), (16, 4, 128), (16, 4, 64)]:
+        T, B, S = sum(docs), len(docs), max(docs)
+        cu = torch.tensor([0] + docs, device=dev).cumsum(0).to(torch.int32)
+        q, k, v = (torch.randn(T, h, HD, device=dev).to(torch.bfloat16).requires_grad_(True) for h in (H, K, K))
+        do = torch.randn(T, H, HD, device=dev).to(torch.bfloat16)
+        o = nn_ops.attention_packed(q, k, v, cu)
+        t_f = timed(lambda: nn_ops.attention_packed(q, k, v, cu), it)
+        t_b = timed(lambda: torch.autograd.grad(o, (q, k, v), do, retain_graph=True), it)
+        gemm.check(dev)
+        pq, pk, pv, pdo = (torch.randn(B, S, h, HD, device=dev).to(torch.bfloat16).requires_grad_(True) for h in (H, H, H, H))
+        po = nn_ops.attention_reference(pq, pk, pv, True)
+        t_pf = timed(lambda: nn_ops.attention_reference(pq, pk, pv, True), it)
+        t_pb = timed(lambda: torch.autograd.grad(po, (pq, pk, pv), pdo, retain_graph=True), it)
+        fl = 2.0 * H * HD * sum(n * (n + 1) for n in docs)          # causal forward FLOPs; backward = 2.5x
+        print(json.dumps({"kernel": "attention_packed_causal", "tokens": T, "docs": B, "H": H, "kv": K, "hd": HD, "fwd_ms": t_f, "fwd_tflops": fl / t_f / 1e9,
+                          "bwd_ms": t_b, "bwd_tflops": 2.5 * fl / t_b / 1e9, "padded_sdpa_fwd_ms": t_pf, "padded_sdpa_bwd_ms": t_pb}), flush=True)
+
+
+def bench_head(small: bool, it: int):
+    from . import gemm, nn_ops
+    dev = torch.device("cuda:0")
+    for N, V, D in [(2048, 8000, 512)] if small else [(8188, 32000, 2048), (4096, 50021, 1024)]:
+        x = torch.randn(N, D, device=dev).to(torch.bfloat16).requires_grad_(True)
+        w = (torch.randn(V, D, device=dev) * D ** -0.5).to(torch.bfloat16).requires_grad_(True)
+        t = torch.randint(0, V, (N,), device=dev)
+
+        def own():
+            return torch.autograd.grad(nn_ops.linear_cross_entropy(x, w, t), (x, w))
+
+        def ref():
+            return torch.autograd.grad(nn_ops.cross_entropy(F.linear(x, w), t), (x, w))
+        t_o, t_r = timed(own, it), timed(ref, it)
+        gemm.check(dev)
+        print(json.dumps({"kernel": "linear_cross_entropy_fwd_bwd", "rows": N, "V": V, "D": D, "ms": t_o, "tflops": 6.0 * N * V * D / t_o / 1e9, "stored_logits_ms": t_r}),
+              flush=True)
 
 
 def bench_norm(small: bool, it: int):
@@ -195,13 +238,13 @@ def main():
     global KERNELS
     ap = argparse.ArgumentParser()
     ap.add_argument("--kernels", action="store_true", help="linear: also list the device time of every kernel of one autograd call (torch.profiler)")
-    ap.add_argument("--what", default="flash", choices=["flash", "ce", "norm", "linear", "small_ops", "all"])
+    ap.add_argument("--what", default="flash", choices=["flash", "ce", "packed", "head", "norm", "linear", "small_ops", "all"])
     ap.add_argument("--small", action="store_true")
     ap.add_argument("--iters", type=int, default=None)
     a = ap.parse_args()
     KERNELS = a.kernels
     it = a.iters or (2 if a.small else 20)
-    for name, fn in (("flash", bench_flash), ("ce", bench_ce), ("norm", bench_norm), ("linear", bench_linear), ("small_ops", bench_small_ops)):
+    for name, fn in (("flash", bench_flash), ("ce", bench_ce), ("packed", bench_packed), ("head", bench_head), ("norm", bench_norm), ("linear", bench_linear), ("small_ops", bench_small_ops)):
         if a.what in (name, "all"):
             fn(a.small, it)
 

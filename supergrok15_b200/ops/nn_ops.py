@@ -8,6 +8,7 @@
 ``swiglu(gate, up)``                silu(gate) * up in one pass; ``gelu(x)`` exact GELU.
 ``attention_packed(q, k, v, cu)``   attention inside each of several sequences of different lengths that share one row axis, with
                                     grouped key / value heads; the gradients of a key head are summed over its query heads.
+``packed_positions(cu, rows)``      the position of every packed row in its sequence (for the rotary tables).
 ``embedding(ids, weight)``          row gather; the gradient is a deterministic sorted segment sum (no atomics).
 ``cross_entropy(logits, target)``   mean softmax cross-entropy with ``ignore_index``; forward reads the logits once.
 ``linear_cross_entropy(x, w, target)``  the mean cross-entropy of ``x @ w.T`` without keeping the logits, with the gradients of both.
@@ -328,6 +329,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
             return _build.require().flash_node(q, k, v, causal, _gemm._err_flag(q.device))
         return _FlashAttention.apply(q, k, v, causal)
     return attention_reference(q, k, v, causal)
+
+
+def packed_positions(cu_seqlens: torch.Tensor, rows: int) -> torch.Tensor:
+    """Position of each of ``rows`` packed rows in its own sequence (int64; rows behind the last sequence count on from its end)."""
+    row = torch.arange(rows, device=cu_seqlens.device)
+    seq = torch.searchsorted(cu_seqlens, row.to(cu_seqlens.dtype), right=True) - 1
+    return torch.where(seq < 0, row, row - cu_seqlens[seq.clamp(min=0)])
 
 
 def attention_packed_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, causal: bool = True,

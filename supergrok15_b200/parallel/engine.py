@@ -60,7 +60,7 @@ class ZeroEngine:
     def __init__(self, model: torch.nn.Module, optimizer: str = "supergrok2", opt_kwargs: Optional[dict] = None,
                  comm: Optional[str] = None, param_dtype: torch.dtype = torch.bfloat16, group=None,
                  timeout_s: float = 20.0, criterion=None, graph: Optional[bool] = None, graph_warmup: int = 3,
-                 overlap: bool = False, bucket_numel: int = 1 << 24, heartbeat=None, gather: str = "push"):
+                 overlap: bool = False, bucket_numel: int = 1 << 24, heartbeat=None, gather: str = "push", model_loss: bool = False):
         self.comm = comm or os.environ.get("GROK_COMM", "p2p")
         assert self.comm in ("p2p", "nvls", "nccl")
         self.rank, self.world = symm.world_info(group)
@@ -69,6 +69,11 @@ class ZeroEngine:
         self.opt_kwargs = dict(opt_kwargs or {})
         self.timeout_s = timeout_s
         self.criterion = criterion                                       # None: the fused softmax cross-entropy kernel
+        # the model's own ``loss(x, y)`` (Llama: cross-entropy of the head without stored logits) instead of logits and a criterion
+        self.model_loss = model_loss
+        if model_loss and (criterion is not None or gather == "gemm" or not callable(getattr(model, "loss", None))):
+            raise ValueError("model_loss: the model needs a loss(x, y) of its own, no criterion, and gather='push' (its head's weight is not "
+                             "read through the Linear that would gather it)")
         # forward + backward of a step are captured into a CUDA graph per batch shape (after `graph_warmup` eager steps): the
         # small models of the grokking tasks launch hundreds of short kernels per step and are bound by the host otherwise
         self.use_graph = (os.environ.get("SG_GRAPH", "1") != "0") if graph is None else bool(graph)
@@ -677,13 +682,16 @@ class ZeroEngine:
             for k, (xb, yb) in enumerate(chunks):
                 if self.overlap and k == len(chunks) - 1:
                     self._arm()                                       # the gradients of this backward pass complete the step
-                logits = self.model(xb)
-                if logits.dim() == 3:                                 # language modelling: one target per position
-                    logits, yb = logits.reshape(-1, logits.shape[-1]), yb.reshape(-1)
-                if self.criterion is None:                            # reads the low-precision logits directly (fp32 arithmetic inside)
-                    loss = nn_ops.cross_entropy(logits, yb)
+                if self.model_loss:
+                    loss = self.model.loss(xb, yb)
                 else:
-                    loss = self.criterion(logits.float(), yb)
+                    logits = self.model(xb)
+                    if logits.dim() == 3:                             # language modelling: one target per position
+                        logits, yb = logits.reshape(-1, logits.shape[-1]), yb.reshape(-1)
+                    if self.criterion is None:                        # reads the low-precision logits directly (fp32 arithmetic inside)
+                        loss = nn_ops.cross_entropy(logits, yb)
+                    else:
+                        loss = self.criterion(logits.float(), yb)
                 if micro_batches > 1:
                     loss = loss / micro_batches
                 loss.backward()
