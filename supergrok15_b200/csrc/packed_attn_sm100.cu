@@ -933,15 +933,15 @@ bool packed_attn_sm100_takes(int dtype, const PackedAttn& p) {
 }
 
 // Parts that the query heads of a key head are cut into for dK and dV.  An item of that kernel visits every query tile of all its heads; with
-// few key heads the longest ones (the first keys of a long causal sequence) then take longer than the average SM is busy.  Cut until one
-// takes at most half of that, were the rows one sequence of their average length; below 1,024 rows a sequence items are short anyway.
-// Two key heads, 14,354 + 2,030 tokens: 2,030 us whole, 1,480 and 24 for the sums in four parts.
+// few key heads there are few items, and the longest of them (the first keys of a long causal sequence) take longer than the average SM is
+// busy.  Cut until there are six items for each SM; below 256 rows a sequence all items are short.  Two key heads, 14,354 + 2,030 tokens:
+// 2,030 us whole, 1,480 and 24 for the sums in four parts.
 int packed_attn_sm100_split(const PackedAttn& p) {
     const int64_t hk = p.heads / p.group, tiles = p.seqs.total / 128, each = p.seqs.n > 0 ? p.seqs.total / p.seqs.n : 0;
-    if (p.group == 1 || each < 1024) return 1;
-    const int64_t want = (4 * (int64_t)device_sms() + hk * tiles - 1) / (hk * tiles);
+    if (p.group == 1 || each < 256 || tiles == 0) return 1;
+    const int64_t want = (6 * (int64_t)device_sms() + hk * tiles - 1) / (hk * tiles);
     for (int s = 1; s < p.group; ++s) if (p.group % s == 0 && s >= want) return s;
-    return want > 1 ? p.group : 1;
+    return p.group;
 }
 int packed_attn_sm100_fwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st) {
     if (p.hd > 64) return dtype == BF16 ? fwd<__nv_bfloat16, 128>(p, err, st) : fwd<__half, 128>(p, err, st);
