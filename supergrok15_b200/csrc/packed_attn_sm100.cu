@@ -504,10 +504,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         const bool carries = KV && tl < 256;
         auto fetch = [&](const Item& w, int h, int i) {
             const int r = w.lo + i * 128 + (tl & 127);
-            if (r >= w.hi) return tl < 128 ? -INFINITY : 0.f;
-            const int64_t at = (int64_t)h * a.seqs.total + r;
-            return tl < 128 ? -LOG2E * a.lse[at] : a.delta[at];
+            if (r >= w.hi) return tl < 128 ? INFINITY : 0.f;
+            return (tl < 128 ? a.lse : a.delta)[(int64_t)h * a.seqs.total + r];      // scaled when it is parked: nothing here waits for the load
         };
+        const float vmul = tl < 128 ? -LOG2E : 1.f;
         float v0 = 0.f, v1 = 0.f;
         auto fetch_first = [&](const Item& w) {
             if (w.kind != 1) return;
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             const int per_head = w.kind == 1 ? tiles(w) : 0, n_it = KV ? per_head * group : per_head;
             const float lse_row = v0 * LOG2E, del_row = v1;
             if (carries && n_it > 0) {
-                (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = v0;    // buffer n & 1: every thread has left iteration n - 2
+                (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = v0 * vmul;    // buffer n & 1: every thread has left iteration n - 2
                 warp_arrive(&b->vec_full);
             }
             int h = KV ? w.head * group : w.head, i = first_tile(w);
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 tc_wait_st();
                 tc_fence_before();
                 warp_arrive(&b->pb_full);
-                if (carries && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = nx; warp_arrive(&b->vec_full); }
+                if (carries && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = nx * vmul; warp_arrive(&b->vec_full); }
             }
             if (!ok) break;
             const Item cur = w;
