@@ -56,6 +56,9 @@ template <int HALVES> __device__ __forceinline__ void zero_rows(uint8_t* tile, i
 //   warp 8           takes items, loads Q and the rings of two K and two V tiles      warp 9   issues the products
 // A row of 128 scores is held in registers: the softmax warpgroups take 208 per thread and leave 88 to the third (256 x 208 + 128 x 88 =
 // 384 x 168, the registers of the launch).
+// Bound by the chain S -> softmax -> P V of the two tiles: 8,192 rows, 16 heads of 128, causal, bf16: 276 us, tensor pipe 51 % busy, 34 % of
+// the issue slots, 0.19 GB of DRAM traffic.  Key halves of 64 (349 us against 291 at that step), twice the softmax warps (398), P handed over
+// in halves (295 against 278) and exponentials by polynomial (295 against 279) were all slower.
 constexpr int FWD_THREADS = 384;
 constexpr int REGS_SOFTMAX = 208, REGS_OTHERS = 88;
 struct FwdBars {
@@ -415,7 +418,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
 // 128 threads share a tile, a thread has one row and 32 columns; P and dS go back to tensor memory as 16-bit A operands, each group's into
 // columns that it alone has read.  The next tile's X is issued as soon as this tile's scores have been taken out, its Y as soon as dS is
 // stored, so the tensor cores work on dV and X while the threads form dS, on dK and Y while they form the next P.
-// Bound by the latency of that hand-over: with two groups (two warps per scheduler, 64 columns per thread) the tensor pipe was 46 % busy.
+// Bound by the chain X -> P -> dS -> product of each tile, which the look-ahead hides in part, and by the rate at which one thread issues
+// products (tc_half.cuh).  8,192 rows, 16 heads of 128, causal, bf16: dK/dV 505 us with the tensor pipe 57 % busy, dQ 407 us and 52 %,
+// delta 19 us (bandwidth).
 // P and dS are rounded to 16 bits to be operands (half a step of each value); everything they come from and are added to is fp32.
 constexpr int BWD_THREADS = 640;
 constexpr int BWD_REGS = 104, BWD_REGS_OTHERS = 64;                       // 512 x 104 + 128 x 64 = 640 x 96, the registers of the launch
