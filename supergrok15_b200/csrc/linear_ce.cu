@@ -303,10 +303,15 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_row_losses_kernel(LceArgs a, 
 // Training in bf16: a warp per row.  The loss and the row's scale; the target's entry of u; the tiles with another reference than the row's;
 // the row of x times the scale, in place (nothing else reads it any more).
 __global__ void __launch_bounds__(ROW_THREADS) lce_scale_rows_kernel(LceArgs a, int tiles, bool last) {
+    constexpr int XV = 4;
     __shared__ float red[32];
     const int row = blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row < lce_active(a)) {
         const float2* st = a.stats + (int64_t)row * tiles;
+        uint4* x = reinterpret_cast<uint4*>((__nv_bfloat16*)a.x + (int64_t)row * a.ldx);      // D is a multiple of 8 here
+        uint4 v[XV];                                                      // the first pieces are on their way while the scale is found
+#pragma unroll
+        for (int k = 0; k < XV; ++k) if (lane + 32 * k < a.D / 8) v[k] = x[lane + 32 * k];
         float mx = -INFINITY, mn = INFINITY, sum = 0.f;
 #pragma unroll 4
         for (int i = lane; i < tiles; i += 32) { const float r = st[i].x; mx = fmaxf(mx, r); mn = fminf(mn, r); }
@@ -332,13 +337,13 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_scale_rows_kernel(LceArgs a, 
             a.row_scale[row] = s;
             u[a.target[row]] = __float2bfloat16_rn(-sum);
         }
-        uint4* x = reinterpret_cast<uint4*>((__nv_bfloat16*)a.x + (int64_t)row * a.ldx);      // D is a multiple of 8 here
-        for (int c = lane; c < a.D / 8; c += 32) {
-            uint4 v = x[c];
-            __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&v);
+#pragma unroll 1
+        for (int c = lane; c < a.D / 8; c += 32 * XV) {
+            if (c != lane)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) e[k] = __float2bfloat16_rn(__bfloat162float(e[k]) * s);
-            x[c] = v;
+                for (int k = 0; k < XV; ++k) if (c + 32 * k < a.D / 8) v[k] = x[c + 32 * k];
+#pragma unroll
+            for (int k = 0; k < XV; ++k) if (c + 32 * k < a.D / 8) x[c + 32 * k] = scaled<__nv_bfloat16>(v[k], s);
         }
     }
     if (last) last_adds(a, red);
@@ -426,7 +431,7 @@ __global__ void __launch_bounds__(256) lce_add_parts_kernel(const float* __restr
     }
 }
 
-// A warp per row and 32 x PER columns (PER = 8, or 1 where a row is not a whole number of eights), the parts four at a time
+// A warp per row and 32 x PER columns (PER = 8, or 1 where a row is not a whole number of eights), the parts eight at a time
 template <typename T, int PER>
 __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* __restrict__ place, int rows, int D, int first, const float* __restrict__ early,
                                                           const float* __restrict__ part, int parts, int64_t row_pitch, const float* __restrict__ gout,
@@ -443,7 +448,7 @@ __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* __restrict_
         const float* src = p < first ? early + (int64_t)p * D + c : part + (int64_t)(p - first) * D + c;
         const int n = p < first ? 1 : parts;
         const float f = p < first ? gout[0] * inv[0] / LceUnit<T>::value : 1.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int s = 0; s < n; ++s) {
             const float* q = src + s * row_pitch * D;
             if constexpr (PER == 8) {
