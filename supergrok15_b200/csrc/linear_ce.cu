@@ -22,6 +22,9 @@
 // Against a pass that recomputes z for the gradient this saves a fourth of all products (6 N V D operations instead of 8) and costs
 // reading and writing u once more.
 //
+// Every kernel behind lce_gather is launched early; the passes over rows let the next one in at once, the product kernels, which leave no room
+// for another CTA, when they end (13 rows x 32,000 x 2,048: 108 -> 100 us).
+//
 // This file: the passes over the rows, and products on the CUDA cores for fp32 operands and for 16-bit ones that TMA cannot address.  Their
 // 128 x 128 tiles take 8 x 8 outputs per thread in steps of 16, the next step's operands on their way to registers under this one's
 // products; two fused multiply-adds per instruction (packed pairs), four 16-byte loads from shared memory for 64 of them.
@@ -29,6 +32,7 @@
 #include "optim_math.cuh"
 #include "linear_ce.h"
 #include "per_device.h"
+#include "launch_early.cuh"
 #include <cfloat>
 
 namespace sg {
@@ -124,6 +128,7 @@ __device__ __forceinline__ void row_of(const Pair (&acc)[4], float (&s)[8]) {
 
 template <typename T>
 __global__ void __launch_bounds__(CTHREADS, 2) lce_logits_kernel(LceArgs a) {
+    after_previous();
     const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, tx = threadIdx.x & 15, rows = lce_active(a);
     if (m0 >= rows) return;
     Pair acc[8][4] = {};
@@ -162,6 +167,7 @@ __global__ void __launch_bounds__(CTHREADS, 2) lce_logits_kernel(LceArgs a) {
 // dx (AM = false: d [rows, V] times w [V, D], part blockIdx.z of the sum) or dw (AM = true: d^T times x [rows, D])
 template <typename T, typename TO, bool AM>
 __global__ void __launch_bounds__(CTHREADS, 2) lce_grad_kernel(LceArgs a, const float* prev, TO* out, int64_t row_pitch, const float* gout, const float* inv) {
+    after_previous();
     const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, rows = lce_active(a);
     const int M = AM ? a.V : rows;
     if (m0 >= M) return;
@@ -247,6 +253,8 @@ template <typename T> __device__ __forceinline__ uint4 scaled(uint4 raw, float f
 }
 template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int tiles, bool last) {
+    let_next_start();
+    after_previous();
     extern __shared__ float fac[];                                        // [tiles] factor of a tile's columns
     __shared__ float red[32];
     constexpr int PER = 16 / sizeof(T), STEP = ROW_THREADS * PER;
@@ -283,6 +291,8 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_rows_kernel(LceArgs a, int ti
 
 // Evaluation: a warp per row.
 __global__ void __launch_bounds__(ROW_THREADS) lce_row_losses_kernel(LceArgs a, int tiles, bool last) {
+    let_next_start();
+    after_previous();
     __shared__ float red[32];
     const int row = blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row < lce_active(a)) {
@@ -303,6 +313,8 @@ __global__ void __launch_bounds__(ROW_THREADS) lce_row_losses_kernel(LceArgs a, 
 // Training in bf16: a warp per row.  The loss and the row's scale; the target's entry of u; the tiles with another reference than the row's;
 // the row of x times the scale, in place (nothing else reads it any more).
 __global__ void __launch_bounds__(ROW_THREADS) lce_scale_rows_kernel(LceArgs a, int tiles, bool last) {
+    let_next_start();
+    after_previous();
     constexpr int XV = 4;
     __shared__ float red[32];
     const int row = blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -372,6 +384,7 @@ __global__ void __launch_bounds__(256) lce_count_kernel(const int64_t* __restric
 __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restrict__ x, int64_t pitch, const int64_t* __restrict__ target, int64_t ignore_index, int rows,
                                                          int V, int row_bytes, int row_pitch, int vec, int* __restrict__ place, uint8_t* __restrict__ xc, int64_t* __restrict__ tc,
                                                          int* __restrict__ count, unsigned* __restrict__ done, const int* __restrict__ blocks) {
+    let_next_start();
     __shared__ int sh[8], base;
     __shared__ int to[GATHER_ROWS];
     const int r0 = blockIdx.x * GATHER_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -423,7 +436,9 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const uint8_t* __restri
     }
 }
 
-__global__ void __launch_bounds__(256) lce_add_parts_kernel(const float* __restrict__ part, int parts, int64_t pitch, int64_t n, float* __restrict__ out) {
+__global__ void __launch_bounds__(256) lce_add_parts_kernel(const float* part, int parts, int64_t pitch, int64_t n, float* out) {
+    let_next_start();
+    after_previous();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         float s = 0.f;
         for (int k = 0; k < parts; ++k) s += part[k * pitch + i];
@@ -433,9 +448,9 @@ __global__ void __launch_bounds__(256) lce_add_parts_kernel(const float* __restr
 
 // A warp per row and 32 x PER columns (PER = 8, or 1 where a row is not a whole number of eights), the parts eight at a time
 template <typename T, int PER>
-__global__ void __launch_bounds__(256) lce_scatter_kernel(const int* __restrict__ place, int rows, int D, int first, const float* __restrict__ early,
-                                                          const float* __restrict__ part, int parts, int64_t row_pitch, const float* __restrict__ gout,
-                                                          const float* __restrict__ inv, T* __restrict__ dx) {
+__global__ void __launch_bounds__(256) lce_scatter_kernel(const int* place, int rows, int D, int first, const float* early, const float* part, int parts, int64_t row_pitch,
+                                                          const float* gout, const float* inv, T* dx) {
+    after_previous();
     const int pieces = (D + 32 * PER - 1) / (32 * PER), lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int row = (int)(item / pieces), c = (int)(item % pieces) * 32 * PER + lane * PER;
@@ -471,20 +486,17 @@ __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* __restrict_
 
 template <typename T> int logits(const LceArgs& a, cudaStream_t st) {
     count_launch();
-    lce_logits_kernel<T><<<dim3((a.V + CT - 1) / CT, (a.rows + CT - 1) / CT), CTHREADS, 0, st>>>(a);
-    return cudaGetLastError() == cudaSuccess ? 0 : 3;
+    return launch_early(lce_logits_kernel<T>, dim3((a.V + CT - 1) / CT, (a.rows + CT - 1) / CT), CTHREADS, 0, st, a) == cudaSuccess ? 0 : 3;
 }
 
 template <typename T> int rows(const LceArgs& a, bool last, cudaStream_t st) {
     const int tiles = (a.V + LCE_COLUMNS - 1) / LCE_COLUMNS;
     count_launch();
     if (!a.u) {
-        lce_row_losses_kernel<<<(a.rows + 7) / 8, ROW_THREADS, 0, st>>>(a, tiles, last);
-        return cudaGetLastError() == cudaSuccess ? 0 : 3;
+        return launch_early(lce_row_losses_kernel, dim3((a.rows + 7) / 8), ROW_THREADS, 0, st, a, tiles, last) == cudaSuccess ? 0 : 3;
     }
     if (a.row_scale) {
-        lce_scale_rows_kernel<<<(a.rows + 7) / 8, ROW_THREADS, 0, st>>>(a, tiles, last);
-        return cudaGetLastError() == cudaSuccess ? 0 : 3;
+        return launch_early(lce_scale_rows_kernel, dim3((a.rows + 7) / 8), ROW_THREADS, 0, st, a, tiles, last) == cudaSuccess ? 0 : 3;
     }
     const size_t smem = tiles * sizeof(float);
     static std::atomic<uint64_t> done{0};
@@ -492,21 +504,21 @@ template <typename T> int rows(const LceArgs& a, bool last, cudaStream_t st) {
         return 2;
     if (smem > 200 * 1024) return 4;
     const int cut = a.rows >= 2 * device_sms() ? 1 : (2 * device_sms() + a.rows - 1) / a.rows;
-    lce_rows_kernel<T><<<dim3(a.rows, cut < 8 ? cut : 8), ROW_THREADS, smem, st>>>(a, tiles, last);
-    return cudaGetLastError() == cudaSuccess ? 0 : 3;
+    return launch_early(lce_rows_kernel<T>, dim3(a.rows, cut < 8 ? cut : 8), ROW_THREADS, smem, st, a, tiles, last) == cudaSuccess ? 0 : 3;
 }
 
 template <typename T, typename TO> int grads(const LceArgs& a, const LceGrads& g, cudaStream_t st) {
     if (g.dx_part) {
         count_launch();
-        lce_grad_kernel<T, float, false><<<dim3((a.D + CT - 1) / CT, (a.rows + CT - 1) / CT, g.parts), CTHREADS, 0, st>>>(a, nullptr, g.dx_part, g.row_pitch, g.gout,
-                                                                                                                      g.inv_count);
+        if (launch_early(lce_grad_kernel<T, float, false>, dim3((a.D + CT - 1) / CT, (a.rows + CT - 1) / CT, g.parts), CTHREADS, 0, st, a, nullptr, g.dx_part, g.row_pitch,
+                         g.gout, g.inv_count) != cudaSuccess) return 3;
     }
     if (g.dw) {
         count_launch();
-        lce_grad_kernel<T, TO, true><<<dim3((a.D + CT - 1) / CT, (a.V + CT - 1) / CT), CTHREADS, 0, st>>>(a, g.dw_prev, (TO*)g.dw, 0, g.gout, g.inv_count);
+        if (launch_early(lce_grad_kernel<T, TO, true>, dim3((a.D + CT - 1) / CT, (a.V + CT - 1) / CT), CTHREADS, 0, st, a, g.dw_prev, (TO*)g.dw, 0, g.gout, g.inv_count) !=
+            cudaSuccess) return 3;
     }
-    return cudaGetLastError() == cudaSuccess ? 0 : 3;
+    return 0;
 }
 
 template <typename T>
@@ -515,9 +527,8 @@ int scatter(const int* place, int rows, int D, int first, const float* early, co
     count_launch();
     const int cols = D % 8 == 0 ? 256 : 32;
     const unsigned grid = (unsigned)(((int64_t)rows * ((D + cols - 1) / cols) + 7) / 8);
-    if (D % 8 == 0) lce_scatter_kernel<T, 8><<<grid, 256, 0, st>>>(place, rows, D, first, early, part, parts, row_pitch, gout, inv, (T*)dx);
-    else lce_scatter_kernel<T, 1><<<grid, 256, 0, st>>>(place, rows, D, first, early, part, parts, row_pitch, gout, inv, (T*)dx);
-    return cudaGetLastError() == cudaSuccess ? 0 : 3;
+    return launch_early(D % 8 == 0 ? lce_scatter_kernel<T, 8> : lce_scatter_kernel<T, 1>, dim3(grid), 256, 0, st, place, rows, D, first, early, part, parts, row_pitch, gout, inv,
+                        (T*)dx) == cudaSuccess ? 0 : 3;
 }
 
 }  // namespace
@@ -560,8 +571,7 @@ int lce_grads(int dtype, const LceArgs& a, const LceGrads& g, int* err, cudaStre
 }
 int lce_add_parts(const float* part, int parts, int64_t pitch, int64_t n, float* out, cudaStream_t st) {
     count_launch();
-    lce_add_parts_kernel<<<(unsigned)((n + 255) / 256 < 148 * 8 ? (n + 255) / 256 : 148 * 8), 256, 0, st>>>(part, parts, pitch, n, out);
-    return cudaGetLastError() == cudaSuccess ? 0 : 3;
+    return launch_early(lce_add_parts_kernel, dim3((unsigned)((n + 255) / 256 < 148 * 8 ? (n + 255) / 256 : 148 * 8)), 256, 0, st, part, parts, pitch, n, out) == cudaSuccess ? 0 : 3;
 }
 int lce_scatter(int dtype, const int* place, int rows, int D, int first, const float* early, const float* part, int parts, int64_t row_pitch, const float* gout,
                 const float* inv_count, void* dx, cudaStream_t st) SG_LCE_GO(scatter, place, rows, D, first, early, part, parts, row_pitch, gout, inv_count, dx, st)

@@ -18,6 +18,7 @@
 #include "sg_native.h"
 #include "tc_half.cuh"
 #include "per_device.h"
+#include "launch_early.cuh"
 #include "linear_ce.h"
 #include <cfloat>
 
@@ -151,7 +152,8 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
     if (PAIR) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = b->tmem_slot;
-    const int live = min(max(__ldg(a.count) - a.first, 0), a.rows);       // rows of this piece
+    after_previous();
+    const int live = min(max(*a.count - a.first, 0), a.rows);       // rows of this piece
     // the item that every warp of both CTAs works on next
     auto take = [&](uint32_t n, LItem& w) {
         const uint32_t s = n & 1;
@@ -449,11 +451,13 @@ int launch(unsigned items, const CUtensorMap& a1, const CUtensorMap& b1, const C
     if (!once_per_device(done, current_device(), [&] {
             return cudaFuncSetAttribute(lce_sm100_kernel<T, GRADS, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess;
         })) return 11;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = S::CTAS; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = S::CTAS; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(items * S::CTAS); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = &at; cfg.numAttrs = 1;
+    cfg.gridDim = dim3(items * S::CTAS); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 2;
     count_launch();
     return cudaLaunchKernelEx(&cfg, lce_sm100_kernel<T, GRADS, PAIR>, a1, b1, c1, a2, b2, c2, k) == cudaSuccess ? 0 : 12;
 }
