@@ -15,6 +15,7 @@
 #include "sg_native.h"
 #include "tc_half.cuh"
 #include "per_device.h"
+#include "launch_early.cuh"
 #include "packed_attn.h"
 #include <cfloat>
 
@@ -421,6 +422,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
 // Bound by the chain X -> P -> dS -> product of each tile, which the look-ahead hides in part, and by the rate at which one thread issues
 // products (tc_half.cuh).  8,192 rows, 16 heads of 128, causal, bf16: dK/dV 505 us with the tensor pipe 57 % busy, dQ 407 us and 52 %,
 // delta 19 us (bandwidth).
+// The two kernels do not depend on each other: dQ's CTAs start as those of dK/dV leave their SMs, knowing that delta is complete because every
+// CTA of dK/dV has seen that, and wait for the whole of dK/dV at their end, for what comes behind both (14 documents in 8,192 rows, 16 heads of 128,
+// forward and backward: 409 -> 395 us).
 // P and dS are rounded to 16 bits to be operands (half a step of each value); everything they come from and are added to is fp32.
 constexpr int BWD_THREADS = 640;
 constexpr int BWD_REGS = 104, BWD_REGS_OTHERS = 64;                       // 512 x 104 + 128 x 64 = 640 x 96, the registers of the launch
@@ -478,6 +482,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
     __syncthreads();
     tc_fence_after();
     constexpr uint32_t tmem = 0, tm_x = 0, tm_y = 128, tm_acc0 = 256, tm_acc1 = 384;       // all 512 columns are allocated, so they start at 0
+    if (KV) {
+        after_previous();
+        let_next_start();
+    }
 
     // tiles of the other axis that one head of an item meets: [first, first + count) in tiles of 128 rows from the sequence's begin
     auto first_tile = [&](const Item& w) { return KV && a.causal ? (w.row0 - w.lo) / 128 : 0; };
@@ -510,7 +518,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         auto fetch = [&](const Item& w, int h, int i) {
             const int r = w.lo + i * 128 + (tl & 127);
             if (r >= w.hi) return tl < 128 ? INFINITY : 0.f;
-            return (tl < 128 ? a.lse : a.delta)[(int64_t)h * a.seqs.total + r];      // scaled when it is parked: nothing here waits for the load
+            return __ldcg((tl < 128 ? a.lse : a.delta) + (int64_t)h * a.seqs.total + r);      // scaled when it is parked: nothing here waits for the load
         };
         const float vmul = tl < 128 ? -LOG2E : 1.f;
         float v0 = 0.f, v1 = 0.f;
@@ -519,7 +527,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             if (KV) { if (carries) v0 = fetch(w, w.head * group, first_tile(w)); }
             else if (w.row0 + row < w.hi) {
                 const int64_t at = (int64_t)w.head * a.seqs.total + w.row0 + row;
-                v0 = a.lse[at]; v1 = a.delta[at];
+                v0 = __ldcg(a.lse + at); v1 = __ldcg(a.delta + at);
             }
         };
         Item w;
@@ -841,11 +849,13 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
+    if (!KV) after_previous();
 }
 
 // out0 / out1 = the sums of their parts, in order, n elements each (a multiple of 8)
 template <typename T>
-__global__ void __launch_bounds__(256) packed_join_kernel(const float* __restrict__ p0, const float* __restrict__ p1, int split, int64_t n, T* __restrict__ o0, T* __restrict__ o1) {
+__global__ void __launch_bounds__(256) packed_join_kernel(const float* p0, const float* p1, int split, int64_t n, T* o0, T* o1) {
+    after_previous();
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (i >= n) return;
     const float* p = (blockIdx.y ? p1 : p0) + i;
@@ -861,6 +871,7 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const float* __restric
 // delta[head][row] = dO . (O + rest): 16 bytes of each per lane, 8 or 16 lanes per (row, head)
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) packed_delta_sm100_kernel(PackedAttn p) {
+    let_next_start();
     const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
     const int part = (int)(threadIdx.x % LANES);
     const bool live = item < (int64_t)p.seqs.total * p.heads;
@@ -919,12 +930,13 @@ template <typename T, int HD> int bwd(const PackedAttn& p, int* err, cudaStream_
               split, p.scale, err};
     count_launch(split > 1 ? 4 : 3);
     packed_delta_sm100_kernel<T, LANES><<<(unsigned)(((int64_t)p.seqs.total * p.heads * LANES + 255) / 256), 256, 0, st>>>(p);
-    packed_bwd_sm100_kernel<T, HD, true><<<(unsigned)slots * (unsigned)(hk * split), BWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
-    if (split > 1)
-        packed_join_kernel<T><<<dim3((unsigned)((n_kv / 8 + 255) / 256), 2), 256, 0, st>>>(p.kv_parts, p.kv_parts + split * n_kv, split, n_kv, (T*)p.dv, (T*)p.dk);
+    if (cudaGetLastError() != cudaSuccess ||
+        launch_early(packed_bwd_sm100_kernel<T, HD, true>, dim3((unsigned)slots * (unsigned)(hk * split)), BWD_THREADS, smem, st, mq, mk, mv, md, a) != cudaSuccess) return 12;
     a.out0 = p.dq; a.out1 = nullptr;
-    packed_bwd_sm100_kernel<T, HD, false><<<(unsigned)slots * (unsigned)p.heads, BWD_THREADS, smem, st>>>(mq, mk, mv, md, a);
-    return cudaGetLastError() == cudaSuccess ? 0 : 12;
+    if (launch_early(packed_bwd_sm100_kernel<T, HD, false>, dim3((unsigned)slots * (unsigned)p.heads), BWD_THREADS, smem, st, mq, mk, mv, md, a) != cudaSuccess) return 12;
+    if (split > 1 && launch_early(packed_join_kernel<T>, dim3((unsigned)((n_kv / 8 + 255) / 256), 2), 256, 0, st, p.kv_parts, p.kv_parts + split * n_kv, split, n_kv, (T*)p.dv,
+                                  (T*)p.dk) != cudaSuccess) return 12;
+    return 0;
 }
 
 }  // namespace
