@@ -65,11 +65,11 @@ template <typename T, bool IM> struct StepLoad {
             const T* src = IM ? p + (int64_t)k * ld + i : p + (int64_t)i * ld + k;
             const bool row = IM ? k < K : i < I;
             if (sizeof(T) == 4 && vec) {
-                const float4 f = row && (IM ? i < I : k < K) ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 f = row && (IM ? i < I : k < K) ? __ldcg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 v[u][0] = f.x; v[u][1] = f.y; v[u][2] = f.z; v[u][3] = f.w;
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[u][e] = row && (IM ? i + e < I : k + e < K) ? Cvt<T>::to(src[e]) : 0.f;
+                for (int e = 0; e < 4; ++e) v[u][e] = row && (IM ? i + e < I : k + e < K) ? Cvt<T>::to(__ldcg(src + e)) : 0.f;
             }
         }
     }
@@ -164,13 +164,16 @@ __global__ void __launch_bounds__(CTHREADS, 2) lce_logits_kernel(LceArgs a) {
     }
 }
 
-// dx (AM = false: d [rows, V] times w [V, D], part blockIdx.z of the sum) or dw (AM = true: d^T times x [rows, D])
+// dx (AM = false: d [rows, V] times w [V, D], part blockIdx.z of the sum) or dw (AM = true: d^T times x [rows, D]).  Behind dx, dw starts as dx's
+// CTAs leave their SMs: every one of them has seen the end of the row pass, and what that wrote is read from L2.  It waits for the whole of dx
+// at its end, for what comes behind both.
 template <typename T, typename TO, bool AM>
-__global__ void __launch_bounds__(CTHREADS, 2) lce_grad_kernel(LceArgs a, const float* prev, TO* out, int64_t row_pitch, const float* gout, const float* inv) {
-    after_previous();
+__global__ void __launch_bounds__(CTHREADS, 2) lce_grad_kernel(LceArgs a, const float* prev, TO* out, int64_t row_pitch, const float* gout, const float* inv, bool behind_dx) {
+    if (!behind_dx) after_previous();
+    if (!AM) let_next_start();
     const int m0 = blockIdx.y * CT, n0 = blockIdx.x * CT, rows = lce_active(a);
     const int M = AM ? a.V : rows;
-    if (m0 >= M) return;
+    if (m0 >= M) return;                                                  // never all CTAs of dw
     Pair acc[8][4] = {};
     if (AM) tile_product<T, true, true>((const T*)a.u, a.ldu, (const T*)a.x, a.ldx, (int)a.ldu, rows, a.D, 0, rows, m0, n0, acc);
     else {
@@ -190,6 +193,7 @@ __global__ void __launch_bounds__(CTHREADS, 2) lce_grad_kernel(LceArgs a, const 
             if (m < M && n < a.D) out[(int64_t)m * a.D + n] = Cvt<TO>::from(f * (prev ? s[j] + prev[(int64_t)m * a.D + n] : s[j]));
         }
     }
+    if (behind_dx) after_previous();
 }
 
 constexpr int ROW_THREADS = 256;
@@ -511,11 +515,12 @@ template <typename T, typename TO> int grads(const LceArgs& a, const LceGrads& g
     if (g.dx_part) {
         count_launch();
         if (launch_early(lce_grad_kernel<T, float, false>, dim3((a.D + CT - 1) / CT, (a.rows + CT - 1) / CT, g.parts), CTHREADS, 0, st, a, nullptr, g.dx_part, g.row_pitch,
-                         g.gout, g.inv_count) != cudaSuccess) return 3;
+                         g.gout, g.inv_count, false) != cudaSuccess) return 3;
     }
     if (g.dw) {
         count_launch();
-        if (launch_early(lce_grad_kernel<T, TO, true>, dim3((a.D + CT - 1) / CT, (a.V + CT - 1) / CT), CTHREADS, 0, st, a, g.dw_prev, (TO*)g.dw, 0, g.gout, g.inv_count) !=
+        if (launch_early(lce_grad_kernel<T, TO, true>, dim3((a.D + CT - 1) / CT, (a.V + CT - 1) / CT), CTHREADS, 0, st, a, g.dw_prev, (TO*)g.dw, 0, g.gout, g.inv_count,
+                         g.dx_part != nullptr) !=
             cudaSuccess) return 3;
     }
     return 0;
@@ -538,11 +543,17 @@ static_assert(CT == LCE_COLUMNS, "a tile of the logits is a tile of the statisti
 bool lce_scales_rows(int dtype, const LceArgs& a) { return dtype == BF16 && lce_sm100_takes(dtype, a); }
 int lce_dx_parts(int dtype, const LceArgs& a, bool with_dw, int64_t* row_pitch) {
     if (lce_sm100_takes(dtype, a)) return lce_sm100_dx_parts(a.rows, a.V, a.D, with_dw, row_pitch);
-    // two tiles per SM at a time: as many parts as fill them, each at least 256 columns of the vocabulary
+    // Two tiles per SM at a time: the parts (each at least 256 columns of the vocabulary) that give the shortest rounds, a tile's start and
+    // end counted as 128 columns (28 tiles x 5,003 columns: eleven parts are a round and twelve tiles more, ten are one round)
     *row_pitch = a.rows;
-    const int64_t tiles = (int64_t)((a.rows + CT - 1) / CT) * ((a.D + CT - 1) / CT), fill = (2 * device_sms() + tiles - 1) / tiles, most = a.V / 256;
-    const int64_t n = fill < most ? fill : most;
-    return n < 1 ? 1 : (n < 64 ? (int)n : 64);
+    const int64_t tiles = (int64_t)((a.rows + CT - 1) / CT) * ((a.D + CT - 1) / CT), most = a.V / 256 < 64 ? a.V / 256 : 64;
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int64_t n = 1; n <= (most < 1 ? 1 : most); ++n) {
+        const int64_t cost = (tiles * n + 2 * device_sms() - 1) / (2 * device_sms()) * ((a.V + n - 1) / n + 128);
+        if (cost < least) { least = cost; best = (int)n; }
+    }
+    return best;
 }
 int lce_gather_blocks(int rows) { return rows > GATHER_DIRECT ? (rows + COUNT_ROWS - 1) / COUNT_ROWS : 0; }
 int lce_gather(int dtype, const void* x, int64_t ldx, const int64_t* target, int64_t ignore_index, int rows, int V, int D, int* place, void* xc, int64_t* tc,

@@ -30,7 +30,7 @@ struct LceArgs {
 };
 #ifdef __CUDACC__
 __device__ __forceinline__ int lce_active(const LceArgs& a) {
-    const int n = *a.count - a.first;
+    const int n = __ldcg(a.count) - a.first;
     return n < 0 ? 0 : (n < a.rows ? n : a.rows);
 }
 #endif
