@@ -430,7 +430,10 @@ constexpr int BWD_THREADS = 640;
 constexpr int BWD_REGS = 104, BWD_REGS_OTHERS = 64;                       // 512 x 104 + 128 x 64 = 640 x 96, the registers of the launch
 constexpr int BWD_PITCH = 48;                                             // 32 bytes of a row and a pad
 struct BwdBars {
-    uint64_t item_full[2], item_empty[2], clc, res_full, res_empty, ring_full[2], ring_empty[2], tail, a_full, b_full, pa_full, pb_full, vec_full, done;
+    uint64_t item_full[2], item_empty[2], clc, res_full, res_empty, ring_full[2], ring_empty[2], tail, a_full, b_full, pa_full, pb_full, done;
+    // Two, because a warp that has parked the values of tile n + 1 can be done with tile n before another warp has looked whether those of tile n
+    // are there: on one barrier that warp would miss its phase and wait for good.  Those of tile n + 2 need every warp's part of tile n.
+    uint64_t vec_full[2];
     uint4 answer;
     Item item[2];
     uint32_t tmem_slot;
@@ -469,9 +472,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 17); mbar_init(&b->ring_full[i], 1); mbar_init(&b->ring_empty[i], 1);
+            mbar_init(&b->vec_full[i], 8);
         }
         mbar_init(&b->clc, 1); mbar_init(&b->res_full, 1); mbar_init(&b->res_empty, 1); mbar_init(&b->tail, 1); mbar_init(&b->a_full, 1); mbar_init(&b->b_full, 1);
-        mbar_init(&b->pa_full, 16); mbar_init(&b->pb_full, 16); mbar_init(&b->vec_full, 8); mbar_init(&b->done, 1);
+        mbar_init(&b->pa_full, 16); mbar_init(&b->pb_full, 16); mbar_init(&b->done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 17) {
@@ -538,7 +542,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             const float lse_row = v0 * LOG2E, del_row = v1;
             if (carries && n_it > 0) {
                 (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = v0 * vmul;    // buffer n & 1: every thread has left iteration n - 2
-                warp_arrive(&b->vec_full);
+                warp_arrive(&b->vec_full[n & 1]);
             }
             int h = KV ? w.head * group : w.head, i = first_tile(w);
             const int i0 = i, i1 = i + per_head;
@@ -550,7 +554,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 const int see = KV ? 128 : w.hi - (w.lo + i * 128);      // keys of this tile that exist
                 if (++i == i1 && KV) { i = i0; ++h; }
                 if (carries && it + 1 < n_it) nx = fetch(w, h, i);
-                if (KV && !warp_wait(&b->vec_full, n & 1)) { atomicExch(a.err, 82); ok = false; break; }
+                if (KV && !warp_wait(&b->vec_full[bs], (n >> 1) & 1)) { atomicExch(a.err, 82); ok = false; break; }
                 if (!warp_wait(&b->a_full, n & 1)) { atomicExch(a.err, 83); ok = false; break; }
                 tc_fence_after();
                 uint32_t r[32];
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 tc_wait_st();
                 tc_fence_before();
                 warp_arrive(&b->pb_full);
-                if (carries && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = nx * vmul; warp_arrive(&b->vec_full); }
+                if (carries && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = nx * vmul; warp_arrive(&b->vec_full[bs ^ 1]); }
             }
             if (!ok) break;
             const Item cur = w;
