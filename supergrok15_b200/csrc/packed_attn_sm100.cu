@@ -954,13 +954,14 @@ bool packed_attn_sm100_takes(int dtype, const PackedAttn& p) {
 }
 
 // Parts that the query heads of a key head are cut into for dK and dV.  An item of that kernel visits every query tile of all its heads; with
-// few key heads there are few items, and the longest of them (the first keys of a long causal sequence) take longer than the average SM is
-// busy.  Cut until there are six items for each SM; below 256 rows a sequence all items are short.  Two key heads, 14,354 + 2,030 tokens:
-// 2,030 us whole, 1,480 and 24 for the sums in four parts.
+// few key heads there are few items and SMs stay without one, but parts are fp32 sums to be written and added up, and what long items leave
+// idle at the end, dQ fills.  So: an item for each SM, two where a head has up to 64 columns (half the sums); below 256 rows a sequence all
+// items are short.  Backward pass of 16 query heads, us whole / in two / four / eight parts: 14 documents in 8,192 rows, 4 key heads of 128 295 /
+// 294 / 334, 2 key heads 336 / 312 / 293 / 332, 4 key heads of 64 264 / 220 / 242; 14,354 + 2,030 rows, 2 key heads of 128 2,512 / 2,542 / 2,577.
 int packed_attn_sm100_split(const PackedAttn& p) {
     const int64_t hk = p.heads / p.group, tiles = p.seqs.total / 128, each = p.seqs.n > 0 ? p.seqs.total / p.seqs.n : 0;
     if (p.group == 1 || each < 256 || tiles == 0) return 1;
-    const int64_t want = (6 * (int64_t)device_sms() + hk * tiles - 1) / (hk * tiles);
+    const int64_t want = ((p.hd > 64 ? 1 : 2) * (int64_t)device_sms() + hk * tiles - 1) / (hk * tiles);
     for (int s = 1; s < p.group; ++s) if (p.group % s == 0 && s >= want) return s;
     return p.group;
 }
