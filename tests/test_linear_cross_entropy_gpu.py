@@ -190,6 +190,37 @@ def test_captured_step_and_streams(dtype):
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+@pytest.mark.parametrize("rows,dtype", [(140, torch.bfloat16), (140, torch.float32), (13, torch.float16)])
+def test_captured_backward_behind_a_copy_and_a_joined_stream(rows, dtype):
+    """The backward pass's first kernel has something else than one kernel ahead of it."""
+    x, w, t = inputs(rows, 900, 128, dtype)
+    x.requires_grad_(True), w.requires_grad_(True)
+    seed, side = torch.full((), 3.0, device="cuda"), torch.cuda.Stream()
+
+    def step(join):
+        loss = nn_ops.linear_cross_entropy(x, w, t)
+        go = torch.zeros((), device="cuda")
+        go.copy_(seed)
+        if join:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                other = seed * 2
+            torch.cuda.current_stream().wait_stream(side)
+        res = [loss.detach(), *torch.autograd.grad(loss, (x, w), go)]
+        return res + [other] if join else res
+    for join in (False, True):
+        step(join)                                                        # what a first call sets up
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = step(join)
+        for value in (1.0, 5.0):
+            seed.fill_(value)
+            g.replay()
+            for a, b in zip(step(join), got):
+                assert torch.equal(a, b)
+    gemm.check(x.device)
+
+
 def test_refusals():
     x, w, t = inputs(10, 30, 16, torch.float32)
     with pytest.raises(ValueError, match="one device"):
