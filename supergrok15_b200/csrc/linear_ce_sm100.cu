@@ -13,8 +13,9 @@
 // read accumulators (two per 32 rows, 128 columns each), one loads.  The accumulator is double-buffered in tensor memory, so an epilogue
 // runs under the next tile's products; a running pair takes over the tiles of pairs that have not started (cluster launch control), so
 // long and short tiles balance without a counter in memory.  Up to 128 rows a CTA works alone (PAIR = false, 128 x 256): the pair's second
-// half of A would be empty, and what counts is how fast w streams in (13 rows x 32,000 x 2,048, both products 83 us in pairs, 59 alone).
-// 4,096 rows, logits and both products: 387 and 734 us in pairs, 367 and 837 alone.
+// half of A would be empty (13 rows x 32,000 x 2,048: a pass without gradients 54 us in pairs, 50 alone, the gradients' products 71 and 67).
+// 4,096 rows, without gradients 334 and 364 us, the products 748 and 848.  The products are issued by one lane of a warp that stays together,
+// from descriptors in two words: with a lane that runs by itself and 64-bit descriptors the pass without gradients took 357 us.
 #include "sg_native.h"
 #include "tc_half.cuh"
 #include "per_device.h"
@@ -100,11 +101,13 @@ template <bool PAIR> __device__ __forceinline__ void tile_load(void* dst, const 
         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                      ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
 }
-template <bool PAIR> __device__ __forceinline__ void tile_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+template <bool PAIR>
+__device__ __forceinline__ void tile_mma(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
     if constexpr (PAIR)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
-    else tc_mma_bf16(d, da, db, idesc, accumulate);
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}"
+                     ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
+    else tc_mma_ss(d, a_lo, a_hi, b_lo, b_hi, idesc, accumulate);
 }
 // arrives at the barrier (of both CTAs) when the products issued so far are done
 template <bool PAIR> __device__ __forceinline__ void tile_commit(uint64_t* bar) {
@@ -257,33 +260,41 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
             }
         }
     } else if (warp == 9) {
-        if (rank == 0 && lane == 0) {
+        if (rank == 0) {
             uint32_t n_item = 0, it = 0;
             bool ok = true;
+            const uint32_t ring = smem_u32(smem);
             while (ok) {
                 LItem w;
-                if (!take(n_item, w)) { atomicExch(a.err, 104); break; }
-                release(n_item);
+                if (!__all_sync(0xffffffffu, take(n_item, w))) { if (lane == 0) atomicExch(a.err, 104); break; }
+                __syncwarp();
+                if (lane == 0) release(n_item);
                 if (w.kind == 0) break;
                 const uint32_t s = n_item & 1;
-                if (n_item >= 2 && !mbar_wait(&b->acc_empty[s], ((n_item >> 1) & 1) ^ 1)) { atomicExch(a.err, 105); break; }
+                if (n_item >= 2 && !warp_wait(&b->acc_empty[s], ((n_item >> 1) & 1) ^ 1)) { if (lane == 0) atomicExch(a.err, 105); break; }
                 ++n_item;
                 tc_fence_after();
                 const bool a_mn = GRADS && w.kind == 2, b_mn = GRADS;
                 const uint32_t idesc = idesc_f16(Half2<T>::FMT, BM, BN, b_mn) | ((uint32_t)a_mn << 15), d = tmem + s * BN;
+                // descriptors of the ring's first stage; a stage is STAGE >> 4 further
+                const Desc da = desc_of(a_mn ? make_desc_sw128_mn(ring, BK * 128, 1024) : make_desc_sw128(ring));
+                const Desc db = desc_of(b_mn ? make_desc_sw128_mn(ring + A_BYTES, BK * 128, 1024) : make_desc_sw128(ring + A_BYTES));
+                const uint32_t a_step = a_mn ? 128 : 2;
                 for (int k = 0; k < w.nkb; ++k, ++it) {
                     const uint32_t st = it % STAGES;
-                    if (!mbar_wait(&b->full[st], (it / STAGES) & 1)) { atomicExch(a.err, 106); ok = false; break; }
+                    if (!warp_wait(&b->full[st], (it / STAGES) & 1)) { if (lane == 0) atomicExch(a.err, 106); ok = false; break; }
                     tc_fence_after();
-                    const uint32_t pa = smem_u32(smem + st * STAGE);
-                    const uint64_t da = a_mn ? make_desc_sw128_mn(pa, BK * 128, 1024) : make_desc_sw128(pa);
-                    const uint64_t db = b_mn ? make_desc_sw128_mn(pa + A_BYTES, BK * 128, 1024) : make_desc_sw128(pa + A_BYTES);
+                    const uint32_t al = da.lo + st * (STAGE >> 4), bl = db.lo + st * (STAGE >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k4 = 0; k4 < BK / 16; ++k4)
-                        tile_mma<PAIR>(d, da + (a_mn ? 128 : 2) * k4, db + (b_mn ? 128 : 2) * k4, idesc, (k > 0 || k4 > 0) ? 1u : 0u);
-                    tile_commit<PAIR>(&b->empty[st]);
+                        for (int k4 = 0; k4 < BK / 16; ++k4)
+                            tile_mma<PAIR>(d, al + a_step * k4, da.hi, bl + (b_mn ? 128 : 2) * k4, db.hi, idesc, (k > 0 || k4 > 0) ? 1u : 0u);
+                        tile_commit<PAIR>(&b->empty[st]);
+                    }
+                    __syncwarp();
                 }
-                tile_commit<PAIR>(&b->acc_full[s]);
+                if (elect_one()) tile_commit<PAIR>(&b->acc_full[s]);
+                __syncwarp();
             }
         }
     } else if (warp < 8) {
