@@ -14,8 +14,8 @@
 // runs under the next tile's products; a running pair takes over the tiles of pairs that have not started (cluster launch control), so
 // long and short tiles balance without a counter in memory.  Up to 128 rows a CTA works alone (PAIR = false, 128 x 256): the pair's second
 // half of A would be empty (13 rows x 32,000 x 2,048: a pass without gradients 54 us in pairs, 50 alone, the gradients' products 71 and 67).
-// 4,096 rows, without gradients 334 and 364 us, the products 748 and 848.  The products are issued by one lane of a warp that stays together,
-// from descriptors in two words: with a lane that runs by itself and 64-bit descriptors the pass without gradients took 357 us.
+// 4,096 rows: without gradients 334 us in pairs, 364 alone; the products 674 and 736.  Loads and products are issued by one lane of a warp that
+// stays together, products from descriptors in two words: with lanes that ran by themselves these took 357 and 748 us in pairs.
 #include "sg_native.h"
 #include "tc_half.cuh"
 #include "per_device.h"
@@ -228,35 +228,46 @@ __global__ void __launch_bounds__(THREADS, 1) lce_sm100_kernel(const __grid_cons
             }
         }
     } else if (warp == 8) {
-        if (lane == 0) {
-            uint32_t n_item = 0, it = 0;
-            bool ok = true;
-            while (ok) {
-                LItem w;
-                if (!take(n_item, w)) { atomicExch(a.err, 100); break; }
-                release(n_item++);
-                if (w.kind == 0) break;
-                const int m0 = w.m0 + 128 * (int)rank, n0 = w.n0 + S::B_ROWS * (int)rank;       // this CTA's rows of A, of B
+        uint32_t n_item = 0, it = 0;
+        bool ok = true;
+        while (ok) {
+            LItem w;
+            if (!__all_sync(0xffffffffu, take(n_item, w))) { if (lane == 0) atomicExch(a.err, 100); break; }
+            __syncwarp();
+            if (lane == 0) release(n_item);
+            ++n_item;
+            if (w.kind == 0) break;
+            const int m0 = w.m0 + 128 * (int)rank, n0 = w.n0 + S::B_ROWS * (int)rank;       // this CTA's rows of A, of B
+            auto steps = [&](auto load) {
                 for (int k = 0; k < w.nkb; ++k, ++it) {                   // what lies past the end of an operand is filled with zeros
                     const uint32_t st = it % STAGES;
-                    if (it >= STAGES && !mbar_wait(&b->empty[st], ((it / STAGES) & 1) ^ 1)) { atomicExch(a.err, 102); ok = false; break; }
-                    uint8_t* dst = smem + st * STAGE;
-                    const int kc = (w.kb0 + k) * BK;
-                    const uint32_t bar = in_cta(&b->full[st], 0);
-                    if (rank == 0) mbar_expect_tx(&b->full[st], S::CTAS * STAGE);       // what both CTAs load
-                    if constexpr (!GRADS) {
-                        tile_load<PAIR>(dst, &map_a1, kc, m0, bar);
-                        tile_load<PAIR>(dst + A_BYTES, &map_b1, kc, n0, bar);
-                    } else {
-                        if (w.kind == 1) tile_load<PAIR>(dst, &map_a1, kc, m0, bar);
-                        else {
-                            tile_load<PAIR>(dst, &map_a2, m0, kc, bar);
-                            tile_load<PAIR>(dst + BK * 128, &map_a2, m0 + 64, kc, bar);
-                        }
-#pragma unroll
-                        for (int c = 0; c < S::B_ROWS / 64; ++c) tile_load<PAIR>(dst + A_BYTES + c * (BK * 128), w.kind == 1 ? &map_b1 : &map_b2, n0 + 64 * c, kc, bar);
+                    if (it >= STAGES && !warp_wait(&b->empty[st], ((it / STAGES) & 1) ^ 1)) { if (lane == 0) atomicExch(a.err, 102); ok = false; break; }
+                    if (elect_one()) {
+                        const uint32_t bar = in_cta(&b->full[st], 0);
+                        if (rank == 0) mbar_expect_tx(&b->full[st], S::CTAS * STAGE);       // what both CTAs load
+                        load(smem + st * STAGE, (w.kb0 + k) * BK, bar);
                     }
+                    __syncwarp();
                 }
+            };
+            if constexpr (!GRADS) {
+                steps([&](uint8_t* dst, int kc, uint32_t bar) {
+                    tile_load<PAIR>(dst, &map_a1, kc, m0, bar);
+                    tile_load<PAIR>(dst + A_BYTES, &map_b1, kc, n0, bar);
+                });
+            } else if (w.kind == 1) {
+                steps([&](uint8_t* dst, int kc, uint32_t bar) {
+                    tile_load<PAIR>(dst, &map_a1, kc, m0, bar);
+#pragma unroll
+                    for (int c = 0; c < S::B_ROWS / 64; ++c) tile_load<PAIR>(dst + A_BYTES + c * (BK * 128), &map_b1, n0 + 64 * c, kc, bar);
+                });
+            } else {
+                steps([&](uint8_t* dst, int kc, uint32_t bar) {
+                    tile_load<PAIR>(dst, &map_a2, m0, kc, bar);
+                    tile_load<PAIR>(dst + BK * 128, &map_a2, m0 + 64, kc, bar);
+#pragma unroll
+                    for (int c = 0; c < S::B_ROWS / 64; ++c) tile_load<PAIR>(dst + A_BYTES + c * (BK * 128), &map_b2, n0 + 64 * c, kc, bar);
+                });
             }
         }
     } else if (warp == 9) {
