@@ -83,7 +83,7 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& q_, const Tensor& k_, const Te
     TORCH_CHECK(lo.numel() == (q.scalar_type() == at::kFloat ? 0 : q.numel()) && lo.is_contiguous() && lo.scalar_type() == q.scalar_type(), "attention_packed: rest of out");
     TORCH_CHECK(lse.is_contiguous() && lse.scalar_type() == at::kFloat && lse.numel() == q.size(0) * q.size(1), "attention_packed: lse fp32 [heads, rows]");
     Tensor dq = at::empty(q.sizes(), out.options()), dk = at::empty(k.sizes(), out.options()), dv = at::empty(v.sizes(), out.options());
-    if (q.numel() == 0) return {dq, dk, dv};
+    if (q.numel() == 0) return {dq, dk.zero_(), dv.zero_()};               // no rows, or no query heads
     Tensor delta = at::empty_like(lse);
     p.out = out.data_ptr(); p.out_lo = lo.numel() ? lo.data_ptr() : nullptr;
     p.lse = lse.data_ptr<float>(); p.dout = dout.data_ptr(); p.delta = delta.data_ptr<float>();

@@ -224,3 +224,11 @@ def test_many_backward_passes_agree():
     gemm.check(q.device)
     for a, b in zip(first, again):
         assert torch.equal(a, b)
+
+
+def test_no_query_heads():
+    k, v = (torch.randn(10, 2, 32, device="cuda", dtype=torch.bfloat16).requires_grad_(True) for _ in range(2))
+    q = torch.empty(10, 0, 32, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    out = nn_ops.attention_packed(q, k, v, torch.tensor([0, 10], device="cuda"))
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), torch.empty_like(out))
+    assert out.shape == dq.shape == q.shape and not dk.any() and not dv.any()
