@@ -498,14 +498,14 @@ template <typename T, bool PAIR> int logits(const LceArgs& a, int* err, cudaStre
 
 bool in_pairs(int rows) { return rows > 128; }
 
-// Pieces that a tile of dx is cut into along the vocabulary: so many that one takes about a quarter of what a CTA (or pair) does on average
-// (a half: 769 x 50,021 x 1,000 in 279 us, some pairs busy twice as long as the average; a quarter: 198).  A tile costs its 64-deep steps
-// and about six more for its epilogue.
+// Pieces that a tile of dx is cut into along the vocabulary: so many that one takes about half of what a CTA (or pair) does on average
+// (769 x 50,021 x 1,000: all of it 177 us, a half 138, a quarter 142, an eighth 153; 1,536 x 50,048 x 1,024: 304, 210, 216, 230).  A tile costs
+// its 64-deep steps and about six more for its epilogue.
 int dx_splits(int rows, int V, int D, bool with_dw) {
     const int64_t bm = in_pairs(rows) ? 256 : 128, teams = device_sms() / (bm / 128);
     const int64_t tn = (D + BN - 1) / BN, tx = (rows + bm - 1) / bm * tn, kx = (V + BK - 1) / BK, tw = with_dw ? (V + bm - 1) / bm * tn : 0, kw = (rows + BK - 1) / BK;
     const int64_t share = (tx * (kx + 6) + tw * (kw + 6)) / (teams > 0 ? teams : 1) + 1;
-    int64_t s = (4 * kx + share / 2) / share;
+    int64_t s = (2 * kx + share / 2) / share;
     if (s > kx / 8) s = kx / 8;                                           // eight steps at least, or the partial sums cost more than the products
     if (s > 64) s = 64;
     return s < 1 ? 1 : (int)s;
