@@ -22,8 +22,8 @@
 // Against a pass that recomputes z for the gradient this saves a fourth of all products (6 N V D operations instead of 8) and costs
 // reading and writing u once more.
 //
-// Every kernel behind lce_gather is launched early; the passes over rows let the next one in at once, the product kernels, which leave no room
-// for another CTA, when they end (13 rows x 32,000 x 2,048: 108 -> 100 us).
+// Every kernel behind lce_gather is launched early; the passes over rows let the next one in at once, the tensor-core products, which leave no
+// room for another CTA, when they end (13 rows x 32,000 x 2,048: 108 -> 100 us).
 //
 // This file: the passes over the rows, and products on the CUDA cores for fp32 operands and for 16-bit ones that TMA cannot address.  Their
 // 128 x 128 tiles take 8 x 8 outputs per thread in steps of 16, the next step's operands on their way to registers under this one's
