@@ -90,10 +90,12 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& q_, const Tensor& k_, const Te
     p.dq = dq.data_ptr(); p.dk = dk.data_ptr(); p.dv = dv.data_ptr();
     const int dt = dtype_code(q);
     auto st = at::cuda::getCurrentCUDAStream();
-    Tensor parts;
+    Tensor parts, units;
     if (sg::packed_attn_sm100_takes(dt, p)) {
         const int split = sg::packed_attn_sm100_split(p);
         if (split > 1) { parts = at::empty({2 * split * k.numel()}, lse.options()); p.kv_parts = parts.data_ptr<float>(); }
+        const int64_t n = sg::packed_attn_sm100_units(dt, p);
+        if (n > 0) { units = at::empty({n}, lse.options()); p.units = units.data_ptr<float>(); }
     }
     const int rc = sg::packed_attn_sm100_takes(dt, p) ? sg::packed_attn_sm100_bwd(dt, p, err.data_ptr<int>(), st) : sg::packed_attn_bwd(dt, p, st);
     TORCH_CHECK(rc == 0, "attention_packed: launch of the backward pass failed (code ", rc, ")");

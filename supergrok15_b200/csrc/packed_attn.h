@@ -15,6 +15,7 @@ struct PackedAttn {
     float* delta;                       // scratch [heads, total]
     void *dq, *dk, *dv;                 // dense
     float* kv_parts;                    // scratch of 2 * packed_attn_sm100_split(p) * total * key heads * hd floats, where that is above 1
+    float* units;                       // scratch of packed_attn_sm100_units(dtype, p) floats, where that is above 0
     PackedSeqs seqs;
     int heads, group, hd, causal;
     float scale;
@@ -31,6 +32,7 @@ inline bool packed_tma_view(const void* base, int64_t ld, int64_t hs, int64_t ro
 // The tensor-core kernels; `err` (a device word) becomes non-zero when a wait inside a kernel ran out.
 bool packed_attn_sm100_takes(int dtype, const PackedAttn& p);
 int packed_attn_sm100_split(const PackedAttn& p);
+int64_t packed_attn_sm100_units(int dtype, const PackedAttn& p);
 int packed_attn_sm100_fwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st);
 int packed_attn_sm100_bwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st);
 

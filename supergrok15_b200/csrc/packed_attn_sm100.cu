@@ -425,7 +425,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
 // The two kernels do not depend on each other: dQ's CTAs start as those of dK/dV leave their SMs, knowing that delta is complete because every
 // CTA of dK/dV has seen that, and wait for the whole of dK/dV at their end, for what comes behind both (14 documents in 8,192 rows, 16 heads of 128,
 // forward and backward: 409 -> 395 us).
-// P and dS are rounded to 16 bits to be operands (half a step of each value); everything they come from and are added to is fp32.
+// P and dS are rounded to 16 bits to be operands (half a step of each value); everything they come from and are added to is fp32.  bf16 has the
+// exponents of fp32.  In fp16 a value below 2^-14 has fewer bits than that (8,192 flat keys and dO of 2^-10: dS near 2^-20, dq 0.8 % off), and one
+// above 65,504 is infinite, so dS carries a power of two of its accumulator's row, which the epilogue takes back: a row of dK or dQ is a
+// row of dS times Q or K.  |dS_ij| <= |dO_i| |v_j| + |delta_i| as P <= 1; the pass that forms delta leaves the norms and the largest of each 32 rows,
+// and the threads of an item look for the largest of the rows that it meets while its predecessor ends.  The bound times the row's unit lies
+// between 2^14 and 2^15, so dS keeps all its bits down to 2^-29 of the bound.  Rows with NaN or infinity do not count: what they meet is NaN anyhow.
 constexpr int BWD_THREADS = 640;
 constexpr int BWD_REGS = 104, BWD_REGS_OTHERS = 64;                       // 512 x 104 + 128 x 64 = 640 x 96, the registers of the launch
 constexpr int BWD_PITCH = 48;                                             // 32 bytes of a row and a pad
@@ -434,13 +439,26 @@ struct BwdBars {
     // Two, because a warp that has parked the values of tile n + 1 can be done with tile n before another warp has looked whether those of tile n
     // are there: on one barrier that warp would miss its phase and wait for good.  Those of tile n + 2 need every warp's part of tile n.
     uint64_t vec_full[2];
+    uint64_t unit_full[2];                                                // the warps' shares of an item's largest norms (fp16)
+    float2 peak[2][16];
     uint4 answer;
     Item item[2];
     uint32_t tmem_slot;
 };
 
+constexpr int UNIT_ROWS = 32;                                             // rows of a block of PackedAttn::units
+// a power of two u with 2^14 <= bound * u < 2^15 (bounds from 2^-60 to 2^63)
+__device__ __forceinline__ float unit_for(float bound) {
+    const int e = min(max(__float_as_int(bound) >> 23, 127 - 60), 127 + 63);
+    return __int_as_float((2 * 127 + 14 - e) << 23);
+}
+__device__ __forceinline__ float inverse_of_power(float u) { return __int_as_float((254 << 23) - __float_as_int(u)); }
+
 struct BwdArgs {
     const float *lse, *delta;
+    const float2* peak;                                                   // fp16: [heads, then key heads][blocks] largest |dO| and |delta|, largest |v|
+    const float* norm;                                                    // fp16: [heads, then key heads][total] |dO|, |v|
+    int blocks;
     void *out0, *out1;                                                    // dV, dK, or dQ
     PackedSeqs seqs;
     int heads, group, hd, causal, slots;
@@ -455,6 +473,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                                                                           const __grid_constant__ BwdArgs a) {
     constexpr int HALVES = HD / 64;
     constexpr uint32_t TILE = HALVES * HALF_TILE;
+    constexpr bool UNIT = Half2<T>::FMT == 0;                             // fp16: dS carries a power of two
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sR0 = smem;
@@ -472,7 +491,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b->item_full[i], 1); mbar_init(&b->item_empty[i], 17); mbar_init(&b->ring_full[i], 1); mbar_init(&b->ring_empty[i], 1);
-            mbar_init(&b->vec_full[i], 8);
+            mbar_init(&b->vec_full[i], 8); mbar_init(&b->unit_full[i], 16);
         }
         mbar_init(&b->clc, 1); mbar_init(&b->res_full, 1); mbar_init(&b->res_empty, 1); mbar_init(&b->tail, 1); mbar_init(&b->a_full, 1); mbar_init(&b->b_full, 1);
         mbar_init(&b->pa_full, 16); mbar_init(&b->pb_full, 16); mbar_init(&b->done, 1);
@@ -525,9 +544,39 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             return __ldcg((tl < 128 ? a.lse : a.delta) + (int64_t)h * a.seqs.total + r);      // scaled when it is parked: nothing here waits for the load
         };
         const float vmul = tl < 128 ? -LOG2E : 1.f;
-        float v0 = 0.f, v1 = 0.f;
+        float v0 = 0.f, v1 = 0.f, own = 0.f, unit = 1.f;                  // own: |v| or |dO| of the thread's row
+        uint32_t n_unit = 0;                                              // items with a unit so far
+        // This warp's share of the largest norms that the item's rows meet: whole blocks from their table, the rows at both ends one by one.  Two
+        // buffers are enough: a warp that parks for item n + 2 has seen every warp store the last dS of item n.
+        auto park_peaks = [&](const Item& w) {
+            const int r0 = w.lo + first_tile(w) * 128, r1 = !KV && a.causal && w.row0 + 128 < w.hi ? w.row0 + 128 : w.hi;
+            const int h0 = KV ? w.head * group : a.heads + w.head / a.group, heads = KV ? group : 1;
+            int b0 = (r0 + UNIT_ROWS - 1) / UNIT_ROWS, b1 = r1 / UNIT_ROWS;
+            if (b1 <= b0) { b0 = (r1 + UNIT_ROWS - 1) / UNIT_ROWS; b1 = b0; }             // no whole block: all rows stand before b0
+            const int before = min(b0 * UNIT_ROWS, r1) - r0, behind = max(r1 - b1 * UNIT_ROWS, 0), each = (b1 - b0) + before + behind;
+            float x = 0.f, y = 0.f;
+#pragma unroll 4
+            for (int i = tl; i < heads * each; i += 512) {
+                const int64_t h = h0 + i / each;
+                const int k = i % each;
+                if (k < b1 - b0) {
+                    const float2 p = __ldcg(a.peak + h * a.blocks + b0 + k);
+                    x = fmaxf(x, p.x); y = fmaxf(y, p.y);
+                } else {
+                    const int e = k - (b1 - b0), r = e < before ? r0 + e : b1 * UNIT_ROWS + (e - before);
+                    x = fmaxf(x, __ldcg(a.norm + h * a.seqs.total + r));
+                    if (KV) { const float d = fabsf(__ldcg(a.delta + h * a.seqs.total + r)); if (d < INFINITY) y = fmaxf(y, d); }
+                }
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) { x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off)); y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, off)); }
+            if (lane == 0) b->peak[n_unit & 1][warp] = make_float2(x, y);
+            warp_arrive(&b->unit_full[n_unit & 1]);
+            own = w.row0 + row < w.hi ? __ldcg(a.norm + (int64_t)(KV ? a.heads + w.head / a.split : w.head) * a.seqs.total + w.row0 + row) : 0.f;
+        };
         auto fetch_first = [&](const Item& w) {
             if (w.kind != 1) return;
+            if constexpr (UNIT) park_peaks(w);
             if (KV) { if (carries) v0 = fetch(w, w.head * group, first_tile(w)); }
             else if (w.row0 + row < w.hi) {
                 const int64_t at = (int64_t)w.head * a.seqs.total + w.row0 + row;
@@ -543,6 +592,15 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             if (carries && n_it > 0) {
                 (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = v0 * vmul;    // buffer n & 1: every thread has left iteration n - 2
                 warp_arrive(&b->vec_full[n & 1]);
+            }
+            if (UNIT && n_it > 0) {
+                if (!warp_wait(&b->unit_full[n_unit & 1], (n_unit >> 1) & 1)) { atomicExch(a.err, 96); ok = false; break; }
+                const float2 p = b->peak[n_unit & 1][lane & 15];
+                float x = p.x, y = p.y;
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) { x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off)); y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, off)); }
+                unit = unit_for(x * own + (KV ? y : fabsf(del_row)));
+                ++n_unit;
             }
             int h = KV ? w.head * group : w.head, i = first_tile(w);
             const int i0 = i, i1 = i + per_head;
@@ -602,6 +660,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                     fma2(de.z, de.w, -1.f, -1.f, __uint_as_float(d[k + 2]), __uint_as_float(d[k + 3]), t2, t3);
                     fma2(__uint_as_float(r[k]), __uint_as_float(r[k + 1]), t0, t1, 0.f, 0.f, t0, t1);
                     fma2(__uint_as_float(r[k + 2]), __uint_as_float(r[k + 3]), t2, t3, 0.f, 0.f, t2, t3);
+                    if constexpr (UNIT) { fma2(t0, t1, unit, unit, 0.f, 0.f, t0, t1); fma2(t2, t3, unit, unit, 0.f, 0.f, t2, t3); }
                     pk[k / 2] = Half2<T>::pack(t0, t1);
                     pk[k / 2 + 1] = Half2<T>::pack(t2, t3);
                 }
@@ -631,7 +690,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 const int64_t at = (int64_t)row0 * ld + (int64_t)head * a.hd;
                 T* base = (T*)(second ? a.out1 : a.out0) + at;
                 float* part = KV && a.split > 1 ? (float*)(second ? a.out1 : a.out0) + (int64_t)(cur.head % a.split) * a.seqs.total * ld + at + lane * ld : nullptr;
-                const float f = KV && !second ? 1.f : a.scale;
+                const float f = KV && !second ? 1.f : (UNIT ? a.scale * inverse_of_power(unit) : a.scale);
                 const uint32_t acc = (second ? tm_acc1 : tm_acc0) + lane_addr;
                 const int c0 = KV ? (g & 1) * (HD / 64) : g, c1 = KV ? c0 + HD / 64 : (g < HD / 32 ? g + 1 : g);
 #pragma unroll 1
@@ -896,6 +955,55 @@ __global__ void __launch_bounds__(256) packed_delta_sm100_kernel(PackedAttn p) {
     if (live && part == 0) p.delta[(item % p.heads) * p.seqs.total + item / p.heads] = acc;
 }
 
+// The same for fp16, with what the units need: a CTA takes 32 rows of one head of dO (delta and |dO|) or of v (|v|), and leaves the largest
+// finite norm and |delta| among them.
+template <int LANES>
+__global__ void __launch_bounds__(256) packed_norms_sm100_kernel(PackedAttn p, float2* peak, float* norm, int blocks) {
+    let_next_start();
+    __shared__ float2 sh[8];
+    const int hk = p.heads / p.group, all = p.heads + hk, h = (int)(blockIdx.x % (unsigned)all), blk = (int)(blockIdx.x / (unsigned)all);
+    const int part = (int)(threadIdx.x % LANES);
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int r = 0; r < UNIT_ROWS; r += 256 / LANES) {
+        const int row = blk * UNIT_ROWS + r + (int)threadIdx.x / LANES;
+        const bool live = row < p.seqs.total;
+        float acc = 0.f, sq = 0.f;
+        if (live && part * 8 < p.hd) {
+            const int64_t at = ((int64_t)row * p.heads + h) * p.hd + part * 8;
+            const uint4 d = h < p.heads ? *reinterpret_cast<const uint4*>((const __half*)p.dout + at)
+                                        : *reinterpret_cast<const uint4*>((const __half*)p.v + row * p.v_ld + (h - p.heads) * p.v_hs + part * 8);
+            uint4 o = make_uint4(0u, 0u, 0u, 0u), e = o;
+            if (h < p.heads) { o = *reinterpret_cast<const uint4*>((const __half*)p.out + at); e = *reinterpret_cast<const uint4*>((const __half*)p.out_lo + at); }
+            const uint32_t ov[4] = {o.x, o.y, o.z, o.w}, ev[4] = {e.x, e.y, e.z, e.w}, dv[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 a = Half2<__half>::unpack(ov[k]), b = Half2<__half>::unpack(ev[k]), z = Half2<__half>::unpack(dv[k]);
+                acc = fmaf(a.x + b.x, z.x, fmaf(a.y + b.y, z.y, acc));
+                sq = fmaf(z.x, z.x, fmaf(z.y, z.y, sq));
+            }
+        }
+#pragma unroll
+        for (int off = LANES / 2; off > 0; off >>= 1) { acc += __shfl_xor_sync(0xffffffffu, acc, off); sq += __shfl_xor_sync(0xffffffffu, sq, off); }
+        const float n = sq < INFINITY ? sqrtf(sq) : 0.f;                  // false for NaN too
+        if (live && part == 0) {
+            norm[(int64_t)h * p.seqs.total + row] = n;
+            if (h < p.heads) p.delta[(int64_t)h * p.seqs.total + row] = acc;
+        }
+        x = fmaxf(x, n);
+        if (fabsf(acc) < INFINITY) y = fmaxf(y, fabsf(acc));
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) { x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off)); y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, off)); }
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(x, y);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) { x = fmaxf(x, sh[i].x); y = fmaxf(y, sh[i].y); }
+        peak[(int64_t)h * blocks + blk] = make_float2(x, y);
+    }
+}
+
 bool head_map(CUtensorMap* m, const void* base, const PackedAttn& p, int heads, int64_t ld, int64_t hs) {
     return make_map_heads(m, base, p.seqs.total, heads, p.hd, ld, hs, 128);
 }
@@ -930,10 +1038,14 @@ template <typename T, int HD> int bwd(const PackedAttn& p, int* err, cudaStream_
     const int slots = packed_slots(p.seqs.n, p.seqs.total, 128);
     const int split = p.kv_parts ? packed_attn_sm100_split(p) : 1;
     const int64_t n_kv = (int64_t)p.seqs.total * hk * p.hd;
-    BwdArgs a{p.lse, p.delta, split > 1 ? (void*)p.kv_parts : p.dv, split > 1 ? (void*)(p.kv_parts + split * n_kv) : p.dk, p.seqs, p.heads, p.group, p.hd, p.causal, slots,
+    const int blocks = (p.seqs.total + UNIT_ROWS - 1) / UNIT_ROWS;
+    float2* peak = reinterpret_cast<float2*>(p.units);
+    float* norm = p.units ? p.units + (int64_t)2 * (p.heads + hk) * blocks : nullptr;
+    BwdArgs a{p.lse, p.delta, peak, norm, blocks, split > 1 ? (void*)p.kv_parts : p.dv, split > 1 ? (void*)(p.kv_parts + split * n_kv) : p.dk, p.seqs, p.heads, p.group, p.hd, p.causal, slots,
               split, p.scale, err};
     count_launch(split > 1 ? 4 : 3);
-    packed_delta_sm100_kernel<T, LANES><<<(unsigned)(((int64_t)p.seqs.total * p.heads * LANES + 255) / 256), 256, 0, st>>>(p);
+    if constexpr (Half2<T>::FMT == 0) packed_norms_sm100_kernel<LANES><<<(unsigned)blocks * (unsigned)(p.heads + hk), 256, 0, st>>>(p, peak, norm, blocks);
+    else packed_delta_sm100_kernel<T, LANES><<<(unsigned)(((int64_t)p.seqs.total * p.heads * LANES + 255) / 256), 256, 0, st>>>(p);
     if (cudaGetLastError() != cudaSuccess ||
         launch_early(packed_bwd_sm100_kernel<T, HD, true>, dim3((unsigned)slots * (unsigned)(hk * split)), BWD_THREADS, smem, st, mq, mk, mv, md, a) != cudaSuccess) return 12;
     a.out0 = p.dq; a.out1 = nullptr;
@@ -964,6 +1076,10 @@ int packed_attn_sm100_split(const PackedAttn& p) {
     const int64_t want = ((p.hd > 64 ? 1 : 2) * (int64_t)device_sms() + hk * tiles - 1) / (hk * tiles);
     for (int s = 1; s < p.group; ++s) if (p.group % s == 0 && s >= want) return s;
     return p.group;
+}
+int64_t packed_attn_sm100_units(int dtype, const PackedAttn& p) {
+    if (dtype != F16) return 0;
+    return (int64_t)(p.heads + p.heads / p.group) * (2 * (int64_t)((p.seqs.total + UNIT_ROWS - 1) / UNIT_ROWS) + p.seqs.total);
 }
 int packed_attn_sm100_fwd(int dtype, const PackedAttn& p, int* err, cudaStream_t st) {
     if (p.hd > 64) return dtype == BF16 ? fwd<__nv_bfloat16, 128>(p, err, st) : fwd<__half, 128>(p, err, st);
