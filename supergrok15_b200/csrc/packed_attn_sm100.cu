@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
 // row of dS times Q or K.  |dS_ij| <= |dO_i| |v_j| + |delta_i| as P <= 1; the pass that forms delta leaves the norms and the largest of each 32 rows,
 // and the threads of an item look for the largest of the rows that it meets while its predecessor ends.  The bound times the row's unit lies
 // between 2^14 and 2^15, so dS keeps all its bits down to 2^-29 of the bound.  Rows with NaN or infinity do not count: what they meet is NaN anyhow.
+// P as operand of dV carries 2^15, which the exponent takes up for nothing.
 constexpr int BWD_THREADS = 640;
 constexpr int BWD_REGS = 104, BWD_REGS_OTHERS = 64;                       // 512 x 104 + 128 x 64 = 640 x 96, the registers of the launch
 constexpr int BWD_PITCH = 48;                                             // 32 bytes of a row and a pad
@@ -446,6 +447,7 @@ struct BwdBars {
     uint32_t tmem_slot;
 };
 
+constexpr float P_UNIT_LOG2 = 15.f, P_UNIT = 32768.f;                     // fp16: dK/dV's probabilities are multiplied by this (P <= 1)
 constexpr int UNIT_ROWS = 32;                                             // rows of a block of PackedAttn::units
 // a power of two u with 2^14 <= bound * u < 2^15 (bounds from 2^-60 to 2^63)
 __device__ __forceinline__ float unit_for(float bound) {
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             if (r >= w.hi) return tl < 128 ? INFINITY : 0.f;
             return __ldcg((tl < 128 ? a.lse : a.delta) + (int64_t)h * a.seqs.total + r);      // scaled when it is parked: nothing here waits for the load
         };
-        const float vmul = tl < 128 ? -LOG2E : 1.f;
+        const float vmul = tl < 128 ? -LOG2E : 1.f, vadd = UNIT && tl < 128 ? P_UNIT_LOG2 : 0.f;        // -lse log2 e, with the unit of P; delta
         float v0 = 0.f, v1 = 0.f, own = 0.f, unit = 1.f;                  // own: |v| or |dO| of the thread's row
         uint32_t n_unit = 0;                                              // items with a unit so far
         // This warp's share of the largest norms that the item's rows meet: whole blocks from their table, the rows at both ends one by one.  Two
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
             const int per_head = w.kind == 1 ? tiles(w) : 0, n_it = KV ? per_head * group : per_head;
             const float lse_row = v0 * LOG2E, del_row = v1;
             if (carries && n_it > 0) {
-                (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = v0 * vmul;    // buffer n & 1: every thread has left iteration n - 2
+                (tl < 128 ? s_lse : s_del)[(n & 1) * 128 + (tl & 127)] = fmaf(v0, vmul, vadd);    // buffer n & 1: every thread has left iteration n - 2
                 warp_arrive(&b->vec_full[n & 1]);
             }
             if (UNIT && n_it > 0) {
@@ -600,6 +602,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
 #pragma unroll
                 for (int off = 8; off > 0; off >>= 1) { x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off)); y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, off)); }
                 unit = unit_for(x * own + (KV ? y : fabsf(del_row)));
+                if (KV) unit *= 1.f / P_UNIT;                             // the probabilities carry theirs already
                 ++n_unit;
             }
             int h = KV ? w.head * group : w.head, i = first_tile(w);
@@ -668,7 +671,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 tc_wait_st();
                 tc_fence_before();
                 warp_arrive(&b->pb_full);
-                if (carries && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = nx * vmul; warp_arrive(&b->vec_full[bs ^ 1]); }
+                if (carries && it + 1 < n_it) { (tl < 128 ? s_lse : s_del)[(bs ^ 1) * 128 + (tl & 127)] = fmaf(nx, vmul, vadd); warp_arrive(&b->vec_full[bs ^ 1]); }
             }
             if (!ok) break;
             const Item cur = w;
@@ -690,7 +693,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) packed_bwd_sm100_kernel(const 
                 const int64_t at = (int64_t)row0 * ld + (int64_t)head * a.hd;
                 T* base = (T*)(second ? a.out1 : a.out0) + at;
                 float* part = KV && a.split > 1 ? (float*)(second ? a.out1 : a.out0) + (int64_t)(cur.head % a.split) * a.seqs.total * ld + at + lane * ld : nullptr;
-                const float f = KV && !second ? 1.f : (UNIT ? a.scale * inverse_of_power(unit) : a.scale);
+                constexpr float p_inv = UNIT && KV ? 1.f / P_UNIT : 1.f;
+                const float f = KV && !second ? p_inv : (UNIT ? a.scale * inverse_of_power(unit) * p_inv : a.scale);
                 const uint32_t acc = (second ? tm_acc1 : tm_acc0) + lane_addr;
                 const int c0 = KV ? (g & 1) * (HD / 64) : g, c1 = KV ? c0 + HD / 64 : (g < HD / 32 ? g + 1 : g);
 #pragma unroll 1

@@ -100,3 +100,25 @@ def test_no_gradient_at_all(dtype):
     assert not any(t.any() for t in got[1:])
     got, _ = both(q, k, v * 0, do, cu, True)
     assert not any(t.any() for t in got[:3]) and got[3].any()
+
+
+def one_key_above_the_others(T, hd, gap, dtype, alike=False):
+    """Every query gives the first key a score `gap` powers of two above the others'."""
+    q, k, v, do, cu = tensors([T], 1, 1, hd, dtype, 0.0, 0.0)
+    q[:, 0, 0] = 4.0
+    k[0, 0, 0] = gap * 0.6931471805599453 / 4.0
+    if alike:
+        do[:] = 1.0
+        v[:] = 1.0
+        v[0] = 0.0
+    return q, k, v, do, cu
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [16.7, 20.3, 24.6])
+def test_unlikely_keys_have_their_gradient(gap, dtype):
+    """dv_j = sum_i p_ij do_i of thousands of queries that all find a key equally unlikely: the rounding of the probability is the same in all of them."""
+    got, want = both(*one_key_above_the_others(4096, 64, gap, dtype, True), False, 1.0)
+    compare([t[1:] for t in got[3:]] * 4, [t[1:] for t in want[3:]] * 4)
+
+
