@@ -52,7 +52,8 @@ template <int HALVES> __device__ __forceinline__ void zero_rows(uint8_t* tile, i
 // buffer and accumulator in tensor memory and its own group of 128 softmax threads (one row per thread).  The tensor cores alternate
 //     O_A += P_A(j) V_j,  S_A(j+1) = Q_A K_{j+1}^T,  O_B += P_B(j) V_j,  S_B(j+1)
 // so a group's softmax runs under the other tile's products.  P overwrites S in place (the first 64 columns of its buffer) and is read
-// from tensor memory; O stays there, and a row is rescaled only when its maximum has grown by more than 2^8.
+// from tensor memory; O stays there, and a row is rescaled only when its maximum has grown by more than 2^8.  P is at most 2^8 then, and in fp16
+// is multiplied by 2^7 besides, so that it has all its bits down to 2^-21 of the largest; the sum carries the factor too.
 //   warps 0-3, 4-7   softmax and epilogue of tile A, of tile B
 //   warp 8           takes items, loads Q and the rings of two K and two V tiles      warp 9   issues the products
 // A row of 128 scores is held in registers: the softmax warpgroups take 208 per thread and leave 88 to the third (256 x 208 + 128 x 88 =
@@ -83,6 +84,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdArgs a) {
     constexpr int HALVES = HD / 64;
+    constexpr bool FP16 = Half2<T>::FMT == 0;
     constexpr uint32_t TILE = HALVES * HALF_TILE;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                         tc_st32(to + c * 32, u);
                     }
                 }
-                const float mc = -m_ref * c2;
+                const float mc = FP16 ? fmaf(-m_ref, c2, 7.f) : -m_ref * c2;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) packed_fwd_sm100_kernel(const 
                         __syncwarp();
                     }
                 }
-                if (a.lse && lane < live) a.lse[(int64_t)w.head * a.seqs.total + row0 + lane] = n > 0 ? m_ref * a.scale + logf(l) : 0.f;
+                if (a.lse && lane < live) a.lse[(int64_t)w.head * a.seqs.total + row0 + lane] = n > 0 ? m_ref * a.scale + logf(FP16 ? l * 0x1p-7f : l) : 0.f;
             }
             if (n > 0) { tc_fence_before(); warp_arrive(&b->o_empty[t]); }
         }

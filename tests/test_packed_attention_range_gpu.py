@@ -122,3 +122,12 @@ def test_unlikely_keys_have_their_gradient(gap, dtype):
     compare([t[1:] for t in got[3:]] * 4, [t[1:] for t in want[3:]] * 4)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [19.4, 20.6])
+def test_unlikely_keys_have_their_share(gap, dtype):
+    """One key above thousands of equally unlikely ones that alone have something to say, before and behind them."""
+    q, k, v, do, cu = one_key_above_the_others(4096, 64, gap, dtype, True)
+    for at in (0, 2000, 4095):
+        k2, v2 = k.roll(at, 0), v.roll(at, 0)
+        got, want = both(q, k2, v2, do, cu, False, 1.0)
+        compare(got[:1], want[:1])
