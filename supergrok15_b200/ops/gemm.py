@@ -38,13 +38,13 @@ def _splitk_ws(dev, slot: int = 0) -> torch.Tensor:
 
 
 def check(dev=None) -> None:
-    """Raise if a GEMM pipeline wait timed out since the last check (one device-to-host read)."""
+    """Raise if a wait inside a tensor-core kernel (GEMM, attention, linear head) timed out since the last check (one device-to-host read)."""
     for d, t in _err.items():
         if dev is None or d == dev:
             v = int(t.item())
             if v:
                 t.zero_()
-                raise RuntimeError(f"tcgen05 GEMM pipeline wait timed out (site {v}) on {d}")
+                raise RuntimeError(f"tcgen05 pipeline wait timed out (site {v}) on {d}")
 
 
 def gemm_tn(a: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None, *, alpha: float = 1.0, beta: float = 0.0,

@@ -26,7 +26,8 @@ all-gather kernel on this rank's slice of the bucket, while backward carries on 
 With ``comm="nccl"`` (and on CPU / gloo) the bucket's all-reduce is started asynchronously at the same point instead.
 
 Waits on peers are bounded on the device (``timeout_s``); ``check()`` raises ``CommTimeout`` when a wait
-ran out, leaving the CUDA context usable.
+ran out, leaving the CUDA context usable.  It raises ``RuntimeError`` when a wait inside a tensor-core kernel of the
+model ran out (``ops.gemm.check``); without it, a step launched after that is known raises.
 """
 from __future__ import annotations
 
@@ -36,6 +37,7 @@ from typing import Dict, List, Optional
 import torch
 import torch.nn.functional as F
 
+from ..ops import gemm as _gemm
 from ..ops import nn_ops
 
 from .. import _build
@@ -196,6 +198,9 @@ class ZeroEngine:
         # the status word is copied to pinned host memory after every step and looked at before the next one is launched
         self._status_host = torch.zeros(1, dtype=torch.int32).pin_memory() if self.cuda else None
         self._status_event = None
+        # so is the word in which the tensor-core kernels record a wait that ran out (it exists once one of them has been called)
+        self._kernel_host = torch.zeros(1, dtype=torch.int32).pin_memory() if self.cuda else None
+        self._kernel_event = None
         self.heartbeat = heartbeat
         # NVLS (in-switch reduction / replication through the multicast mapping) needs multicast addresses for both buffers
         self.nvls = self.comm == "nvls" and self.world > 1 and self.gbuf.multicast_ptr != 0 and self.pbuf.multicast_ptr != 0
@@ -406,10 +411,12 @@ class ZeroEngine:
         raise CommTimeout(f"rank {self.rank}: wait on peer {(s >> 8) & 0xff} timed out at site {(s >> 16) & 0xff}")
 
     def check(self):
-        """Raise if a device-side wait timed out since the last check (reads one int from the device)."""
+        """Raise if a device-side wait timed out since the last check, on a peer or inside a kernel (reads two ints from the device)."""
         s = int(self.status.item())
         if s & 0xff:
             self._raise_timeout(s)
+        if self.cuda:
+            _gemm.check(self.device)
 
     def _poll_status(self):
         """Called before a step is launched: looks at the copy of the status word that the previous step left in pinned host
@@ -424,12 +431,28 @@ class ZeroEngine:
             s = int(self._status_host[0])
             if s & 0xff:
                 self._raise_timeout(s)
+        self._poll_kernel_word()
 
     def _publish_status(self):
         if self.cuda and self.world > 1 and self._status_event is None:
             self._status_host.copy_(self.status, non_blocking=True)
             self._status_event = torch.cuda.Event()
             self._status_event.record()
+        self._publish_kernel_word()
+
+    def _poll_kernel_word(self):
+        """The same for the kernels' own waits.  What such a kernel left unfinished has gone into the step before this raise."""
+        if self._kernel_event is not None and self._kernel_event.query():
+            self._kernel_event = None
+            if int(self._kernel_host[0]):
+                _gemm.check(self.device)
+
+    def _publish_kernel_word(self):
+        word = _gemm._err.get(self.device) if self.cuda else None
+        if word is not None and self._kernel_event is None:
+            self._kernel_host.copy_(word, non_blocking=True)
+            self._kernel_event = torch.cuda.Event()
+            self._kernel_event.record()
 
     # ------------------------------------------------------------------ step
     def zero_grad(self):
@@ -601,7 +624,10 @@ class ZeroEngine:
         if self.overlap:
             if not self._armed:                                       # step() after a backward that train_step did not drive
                 self._arm()
-            return self._finish_overlapped_step()
+            self._finish_overlapped_step()
+            self._poll_kernel_word()
+            self._publish_kernel_word()
+            return
         if self.cuda:
             self._poll_status()
         if self.device_step:
