@@ -694,11 +694,12 @@ class ZeroEngine:
         self.param_version += 1
         self._publish_status()
 
-    def _fwd_bwd(self, x: torch.Tensor, y: torch.Tensor, micro_batches: int) -> torch.Tensor:
+    def _fwd_bwd(self, x: torch.Tensor, y: torch.Tensor, micro_batches: int, cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Zero the flat gradient buffer, then forward + loss + backward of every micro-batch (gradients accumulate in the buffer)."""
         self.zero_grad()
         total = None
-        chunks = list(zip(x.chunk(micro_batches), y.chunk(micro_batches)))
+        packed = () if cu_seqlens is None else (cu_seqlens,)              # one row of documents, not to be cut
+        chunks = [(x, y)] if packed else list(zip(x.chunk(micro_batches), y.chunk(micro_batches)))
         # Parameter gradients are added to the flat buffer by the backward kernels themselves (no accumulation kernel per
         # parameter; weight-gradient GEMMs on a side stream).  Not with overlap: its buckets fire from autograd's accumulation hooks.
         sink = self.cuda and not self.overlap and os.environ.get("SG_GRAD_SINK", "1") != "0"
@@ -709,9 +710,9 @@ class ZeroEngine:
                 if self.overlap and k == len(chunks) - 1:
                     self._arm()                                       # the gradients of this backward pass complete the step
                 if self.model_loss:
-                    loss = self.model.loss(xb, yb)
+                    loss = self.model.loss(xb, yb, *packed)
                 else:
-                    logits = self.model(xb)
+                    logits = self.model(xb, *packed)
                     if logits.dim() == 3:                             # language modelling: one target per position
                         logits, yb = logits.reshape(-1, logits.shape[-1]), yb.reshape(-1)
                     if self.criterion is None:                        # reads the low-precision logits directly (fp32 arithmetic inside)
@@ -724,85 +725,95 @@ class ZeroEngine:
                 total = loss.detach() if total is None else total + loss.detach()
         return total
 
-    def _fwd_bwd_graphed(self, x: torch.Tensor, y: torch.Tensor, micro_batches: int, with_step: bool = False) -> torch.Tensor:
+    def _fwd_bwd_graphed(self, x: torch.Tensor, y: torch.Tensor, micro_batches: int, with_step: bool = False,
+                         cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Forward + backward (and, ``with_step``, the kernels of the sharded step) through a CUDA graph captured per
         (shape, dtype, micro-batch count).  The first ``graph_warmup`` calls of a shape run eagerly (lazy initialisation,
         workspace growth); a capture that fails switches graphs off.  Every rank captures at the same call, and the barriers
         inside the graph take their epochs from the device table, so a replay is a complete step."""
-        def body(xx, yy):
-            total = self._fwd_bwd(xx, yy, micro_batches)
+        def body(xx, yy, *packed):
+            total = self._fwd_bwd(xx, yy, micro_batches, *packed)
             if with_step:
                 self._device_step()
             return total
-        key = (tuple(x.shape), x.dtype, tuple(y.shape), y.dtype, micro_batches, self.model.training, with_step)
+        batch = (x, y) if cu_seqlens is None else (x, y, cu_seqlens)
+        key = (*((tuple(t.shape), t.dtype) for t in batch), micro_batches, self.model.training, with_step)
         entry = self._graphs.get(key)
         if entry is None:
             seen = self._graph_seen.get(key, 0)
             self._graph_seen[key] = seen + 1
             if seen < self.graph_warmup:
-                return body(x.to(self.device, non_blocking=True), y.to(self.device, non_blocking=True))
-            sx = torch.empty(x.shape, dtype=x.dtype, device=self.device)
-            sy = torch.empty(y.shape, dtype=y.dtype, device=self.device)
-            sx.copy_(x, non_blocking=True)
-            sy.copy_(y, non_blocking=True)
+                return body(*(t.to(self.device, non_blocking=True) for t in batch))
+            static = [torch.empty(t.shape, dtype=t.dtype, device=self.device) for t in batch]
+            for s, t in zip(static, batch):
+                s.copy_(t, non_blocking=True)
             C = _build.require()
             try:
                 torch.cuda.synchronize(self.device)
                 g = torch.cuda.CUDAGraph()
                 l0 = C.launch_count()
                 with torch.cuda.graph(g):
-                    total = body(sx, sy)
-                entry = (g, sx, sy, total, C.launch_count() - l0)
-                C.add_launches(-entry[4])                             # enqueued for the capture only; counted again at every replay
+                    total = body(*static)
+                entry = (g, static, total, C.launch_count() - l0)
+                C.add_launches(-entry[3])                             # enqueued for the capture only; counted again at every replay
                 self._graphs[key] = entry
             except Exception as exc:  # noqa: BLE001
                 import warnings
                 warnings.warn(f"CUDA graph capture of the step failed ({type(exc).__name__}: {exc}); running eagerly")
                 self.use_graph = False
                 torch.cuda.synchronize(self.device)
-                return body(x.to(self.device, non_blocking=True), y.to(self.device, non_blocking=True))
-        g, sx, sy, total, n_launch = entry
-        sx.copy_(x, non_blocking=True)
-        sy.copy_(y, non_blocking=True)
+                return body(*(t.to(self.device, non_blocking=True) for t in batch))
+        g, static, total, n_launch = entry
+        for s, t in zip(static, batch):
+            s.copy_(t, non_blocking=True)
         g.replay()
         _build.require().add_launches(n_launch)
         return total.clone()                                          # the graph's own loss tensor is overwritten by the next replay
 
     # ------------------------------------------------------------------ the call a user makes
-    def train_step(self, x: torch.Tensor, y: torch.Tensor, micro_batches: int = 1, **metrics) -> torch.Tensor:
+    def train_step(self, x: torch.Tensor, y: torch.Tensor, micro_batches: int = 1, cu_seqlens: Optional[torch.Tensor] = None, **metrics) -> torch.Tensor:
         """Host (pinned) or device batch in, loss tensor out: H2D copy, forward, backward, sharded fused step.
-        ``micro_batches`` > 1 splits the batch and accumulates gradients in the flat buffer (activation memory)."""
+        ``micro_batches`` > 1 splits the batch and accumulates gradients in the flat buffer (activation memory).
+        ``cu_seqlens``: the batch is one row of documents of different lengths, and these are their offsets (for models that take them as the
+        argument behind the batch, like ``Llama``).  Such a row is not split; steps of one length and number of documents share a graph."""
+        if cu_seqlens is not None and micro_batches != 1:
+            raise ValueError(f"a packed row of documents is not split into micro_batches, got {micro_batches}")
         if self.use_graph and self.cuda and self.device_step:
             # the whole step is one graph launch: host work is the schedule update and one table-writing kernel
             self._poll_status()
             self._host_pre(metrics)
-            total = self._fwd_bwd_graphed(x, y, micro_batches, with_step=True)
+            total = self._fwd_bwd_graphed(x, y, micro_batches, with_step=True, cu_seqlens=cu_seqlens)
             self._host_post()
             return total
         if self.use_graph and self.cuda:
-            total = self._fwd_bwd_graphed(x, y, micro_batches)
+            total = self._fwd_bwd_graphed(x, y, micro_batches, cu_seqlens=cu_seqlens)
         else:
             if x.device != self.device:
                 x = x.to(self.device, non_blocking=True)
                 y = y.to(self.device, non_blocking=True)
-            total = self._fwd_bwd(x, y, micro_batches)
+            if cu_seqlens is not None:
+                cu_seqlens = cu_seqlens.to(self.device, non_blocking=True)
+            total = self._fwd_bwd(x, y, micro_batches, cu_seqlens)
         self.step(**metrics)
         return total
 
-    def profile_step(self, x: torch.Tensor, y: torch.Tensor, micro_batches: int = 1, **metrics) -> Dict[str, float]:
+    def profile_step(self, x: torch.Tensor, y: torch.Tensor, micro_batches: int = 1, cu_seqlens: Optional[torch.Tensor] = None, **metrics) -> Dict[str, float]:
         """One eager step with CUDA events between its phases; returns milliseconds per phase on this rank.  The launches are
         queued behind a short device-side delay so that the phases run back to back, as they do when replayed from the graph
         (the host needs longer to enqueue the ~300 kernels of forward / backward than the GPU needs to run them)."""
         assert self.cuda and self.device_step, "per-phase timing covers the device step (in-kernel collectives)"
         from ..utils.timers import StepTimer
+        if cu_seqlens is not None and micro_batches != 1:
+            raise ValueError(f"a packed row of documents is not split into micro_batches, got {micro_batches}")
         timer = StepTimer()
         x, y = x.to(self.device), y.to(self.device)
+        cu_seqlens = None if cu_seqlens is None else cu_seqlens.to(self.device)
         self._poll_status()
         self._host_pre(metrics)
         torch.cuda.synchronize(self.device)
         torch.cuda._sleep(int(3e7))
         timer.start()
-        self._fwd_bwd(x, y, micro_batches)
+        self._fwd_bwd(x, y, micro_batches, cu_seqlens)
         timer.mark("fwd+bwd")
         self._device_step(hook=timer.mark)
         self._host_post()
