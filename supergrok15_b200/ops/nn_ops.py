@@ -368,10 +368,15 @@ def _gemm_err_flag(device: torch.device) -> torch.Tensor:
     return gemm._err_flag(device)
 
 
+def _wanted(*tensors: torch.Tensor):
+    """What an autograd function is given: with gradients off, tensors that ask for none (inside, it cannot tell)."""
+    return tensors if torch.is_grad_enabled() else tuple(t.detach() for t in tensors)
+
+
 class _AttnPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, causal, scale):
-        out, rest, lse = _build.require().packed_attn_fwd(q, k, v, cu, causal, scale, True, _gemm_err_flag(q.device))
+        out, rest, lse = _build.require().packed_attn_fwd(q, k, v, cu, causal, scale, any(ctx.needs_input_grad[:3]), _gemm_err_flag(q.device))
         ctx.save_for_backward(q, k, v, cu, out, rest, lse)
         ctx.args = causal, scale
         return out
@@ -408,7 +413,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if not q.is_cuda:
         return attention_packed_reference(q, k, v, cu_seqlens, causal, scale)
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in _wanted(q, k, v))
     return _AttnPacked.apply(q, k, v, cu_seqlens.to(torch.int32).contiguous(), causal, scale)
 
 
@@ -584,6 +589,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise ValueError("linear_cross_entropy: x and weight need one dtype, target int64, and all tensors one device")
     if not x.is_cuda:
         return linear_cross_entropy_reference(x, weight, target, ignore_index)
+    x, weight = _wanted(x, weight)
     x2, t = x.reshape(-1, x.shape[-1]), target.reshape(-1).contiguous()
     x2, w = (a if a.stride(1) == 1 else a.contiguous() for a in (x2, weight))
     return _LinearCrossEntropy.apply(x2, w, t, ignore_index)
