@@ -124,9 +124,14 @@ struct PackedAttnNode : Function<PackedAttnNode> {
 
 // ---- cross-entropy of a linear head
 // Rows of a piece: u (rows x vocabulary, the type of x) takes 256 MB at most, but at least 256 rows go together, so that w is not read for
-// less work than that.  A pass without gradients keeps two floats per row and tile of columns only.
+// less work than that.  A pass without gradients keeps two floats per row and tile of columns only, to the same bound.  65,536 rows at most:
+// tile rows are the second dimension of a grid, which has 65,535, and dw is one chain of fp32 additions over a piece, in which terms below half a
+// step of the sum are lost (8,400,000 rows of 5 columns in two pieces: dw 0.2 % off).
 int64_t lce_piece_rows(int64_t rows, int64_t ldu, int64_t elem, bool train) {
-    int64_t most = train ? ((int64_t)256 << 20) / (ldu * elem) / 256 * 256 : 65536;
+    const int64_t each = train ? ldu * elem : (ldu + sg::LCE_COLUMNS - 1) / sg::LCE_COLUMNS * (int64_t)sizeof(float2), top = 65536;
+    int64_t most = ((int64_t)256 << 20) / each;
+    if (most > top) most = top;
+    most = most / 256 * 256;
     if (most < 256) most = 256;
     if (rows <= most) return rows;
     const int64_t pieces = (rows + most - 1) / most;

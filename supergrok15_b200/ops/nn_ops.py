@@ -576,7 +576,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
     Positions whose target is ``ignore_index`` or lies outside the vocabulary are not counted: they are left out before anything is computed, so
     they cost nothing, whatever stands in their rows of ``x`` reaches nothing, and their rows of the gradient are zero (no counted position: loss 0).  bf16, fp16 and fp32 on CUDA, for any vocabulary.  At most 256 MB (or 256 rows) of
-    [rows, vocabulary] values exist at a time, in the type of ``x``; a pass with gradients takes the rows in pieces of that size, and from the
+    [rows, vocabulary] values exist at a time, in the type of ``x``; a pass with gradients takes the rows in pieces of that size (65,536 at most), and from the
     second piece on holds the weight's gradient in fp32 between forward and backward.  The gradients' products of all pieces but the last
     are formed in the forward pass.  Sums are fp32 and added in a fixed order.  A wait that runs out inside a kernel leaves its results
     unfinished and is recorded on the device; ``ops.gemm.check`` raises for it."""
