@@ -1,6 +1,7 @@
 // Kernels that are launched programmatically: such a kernel may be set up while the one before it in the stream still runs, and touches
-// nothing in global memory before after_previous() has seen all of that kernel (and, since that one waited too, of what came before it).  A kernel that starts without the wait, because what it reads comes from
-// an earlier one, says at its place why it may, and waits at its end instead, for what comes behind it.
+// nothing in global memory before after_previous() has seen all of that kernel (and, since that one waited too, of what came before it).  A
+// kernel that starts without the wait, because what it reads comes from an earlier one, says at its place why it may, and waits at its end
+// instead, for what comes behind it.
 // What an earlier kernel wrote is therefore not read through the read-only path (no __ldg, no const __restrict__), whose loads the compiler
 // may move.  let_next_start() lets the next kernel's CTAs in as soon as every CTA of this one has called it or ended.
 #pragma once

@@ -16,7 +16,7 @@
 // maximum: it is 0 while the tile's largest |z| stays below 64 log 2 = 44, else the nearest multiple of 64 powers of two.  All tiles of nearly
 // every row then share one reference, u needs no second pass, and s moves into the products: dx = s (u w) in the epilogue, dw = u^T (s x)
 // with the rows of x scaled in place (tiles with another reference are rescaled, by a power of two, exactly).  8,188 x 32,000: 256 us of
-// reading and writing u become 20.  Between z and a product stand at most two roundings to 16 bits (u and d, or u and s x), each at
+// reading and writing u become 29.  Between z and a product stand at most two roundings to 16 bits (u and d, or u and s x), each at
 // most half a step of the value itself.
 //
 // Against a pass that recomputes z for the gradient this saves a fourth of all products (6 N V D operations instead of 8) and costs

@@ -1,7 +1,7 @@
 // Products of the linear-head cross-entropy on the 5th-generation tensor cores (tcgen05 / TMEM / TMA), sm_100a only: 16-bit operands,
 // fp32 accumulators.  linear_ce.cu has the mathematics and the pass over the rows that stands between the two kernels.
 //
-//   LOGITS   z = x w^T, a tile of 128 rows x 256 columns at a time; the epilogue leaves reference, sum and u of each row and
+//   LOGITS   z = x w^T, a tile of 256 rows x 256 columns at a time (128 x 256 up to 128 rows); the epilogue leaves reference, sum and u of each row and
 //            half tile (see linear_ce.cu): the logits never reach memory
 //   GRADS    dx = d w and dw = d^T x in one launch.  dx has few tiles with a long sum (the vocabulary), dw many with a short one; the long
 //            ones start first and are cut along the sum when one alone would take longer than everything spread over the SMs.  d, w and x are

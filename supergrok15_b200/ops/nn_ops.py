@@ -398,7 +398,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     its sequence up to itself.  ``scale`` multiplies the scores (default ``hd ** -0.5``).  Rows of no sequence (padding behind the last one)
     are neither read nor counted: their output and their gradients are zero.  The offsets stay on the device (no host synchronisation, and a
     captured call follows offsets rewritten in place); offsets that do not ascend give undefined rows.  bf16, fp16 and fp32; head sizes up to
-    128 on CUDA.  Sums, softmax statistics and gradient accumulators are fp32 and added in a fixed order.  A wait that runs out inside a kernel
+    128 on CUDA.  Sums, softmax statistics and gradient accumulators are fp32 and added in a fixed order;
+    with 16-bit inputs the probabilities and their gradients are rounded to that type to be multiplied.  A wait that runs out inside a kernel
     leaves its results unfinished and is recorded on the device; ``ops.gemm.check`` raises for it."""
     if q.is_cuda and _cpp_node(q, k, v, cu_seqlens):                     # checks its arguments like the lines below
         return _build.require().packed_attn_node(q, k, v, cu_seqlens, causal, scale, _gemm_err_flag(q.device))
@@ -578,7 +579,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     they cost nothing, whatever stands in their rows of ``x`` reaches nothing, and their rows of the gradient are zero (no counted position: loss 0).  bf16, fp16 and fp32 on CUDA, for any vocabulary.  At most 256 MB (or 256 rows) of
     [rows, vocabulary] values exist at a time, in the type of ``x``; a pass with gradients takes the rows in pieces of that size (65,536 at most), and from the
     second piece on holds the weight's gradient in fp32 between forward and backward.  The gradients' products of all pieces but the last
-    are formed in the forward pass.  Sums are fp32 and added in a fixed order.  A wait that runs out inside a kernel leaves its results
+    are formed in the forward pass.  Sums are fp32 and added in a fixed order; with 16-bit inputs the exponentials, and in bf16 the scaled rows of ``x``,
+    are rounded to that type to be multiplied.  A wait that runs out inside a kernel leaves its results
     unfinished and is recorded on the device; ``ops.gemm.check`` raises for it."""
     if x.is_cuda and _cpp_node(x, weight, target):                       # checks its arguments like the lines below
         return _build.require().lce_node(x, weight, target, ignore_index, _gemm_err_flag(x.device))
