@@ -131,3 +131,40 @@ def test_unlikely_keys_have_their_share(gap, dtype):
         k2, v2 = k.roll(at, 0), v.roll(at, 0)
         got, want = both(q, k2, v2, do, cu, False, 1.0)
         compare(got[:1], want[:1])
+
+
+def test_many_backward_passes_agree_in_fp16():
+    """Warps drift apart, and the units of an item are looked for while its predecessor ends: no wait may miss its phase, no value may be overwritten."""
+    for lens, H, Hk, hd in (([42, 120, 77, 464, 33, 56, 409, 783, 2309, 36, 1897, 272, 1676, 18], 16, 2, 128), ([26] * 90 + [0, 3, 160], 8, 2, 64)):
+        q, k, v, do, cu = tensors(lens, H, Hk, hd, torch.float16)
+        a = [t.requires_grad_(True) for t in (q, k, v)]
+        out = nn_ops.attention_packed(*a, cu)
+        first = torch.autograd.grad(out, a, do, retain_graph=True)
+        for _ in range(400):
+            again = torch.autograd.grad(out, a, do, retain_graph=True)
+        gemm.check(q.device)
+        assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
+def test_captured_fp16_step_follows_new_offsets_and_values():
+    q, k, v, do, cu = tensors([100, 156, 44, 12], 4, 2, 64, torch.float16)
+    a = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def step():
+        out = nn_ops.attention_packed(*a, cu)
+        return [out.detach(), *torch.autograd.grad(out, a, do)]
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step()
+        graphs.append((g, res))
+    for offs, gain in (([0, 100, 256, 300, 312], 1.0), ([0, 1, 1, 312, 312], 2.0 ** -9), ([0, 7, 200, 310, 311], 2.0 ** 11)):
+        cu.copy_(torch.tensor(offs, dtype=torch.int32))
+        do.mul_(gain)
+        for g, _ in graphs:
+            g.replay()
+        for want, x, y in zip(step(), graphs[0][1], graphs[1][1]):
+            assert torch.equal(want, x) and torch.equal(want, y)
